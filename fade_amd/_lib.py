@@ -154,6 +154,52 @@ class ReassignArgs(ctypes.Structure):
     ]
 
 
+class PageSlotsArgs(ctypes.Structure):
+    """``fade_page_slots_args`` of include/fade_hip.h."""
+
+    _fields_ = [
+        ("B", _i64), ("pages_per_row", _i64), ("n_tokens", _i64), ("n_free", _i64),
+        ("lens", _p), ("new_tokens", _p), ("reset", _p), ("table", _p), ("free_pages", _p), ("ring", _p),
+        ("table_out", _p), ("lens_out", _p), ("starts", _p), ("slots", _p), ("positions", _p), ("ring_out", _p),
+        ("status", _p),
+    ]
+
+
+SLOTS_MAX_ROWS = 4096
+SLOTS_STATUS = {1: "more pages needed than are free", 2: "a row would pass its table's pages",
+                4: "more new tokens than n_tokens", 8: "a negative or impossible count"}
+
+ROPE_MAX_FREQS = 128
+
+
+class RopeRows(ctypes.Structure):
+    _fields_ = [("src", _p), ("dst", _p), ("src_sb", _i64), ("src_sh", _i64), ("src_ss", _i64),
+                ("dst_sb", _i64), ("dst_sh", _i64), ("dst_ss", _i64)]
+
+
+class RopeArgs(ctypes.Structure):
+    """``fade_rope_args`` of include/fade_hip.h."""
+
+    _fields_ = [
+        ("B", _i64), ("S", _i64), ("D", _i64), ("Hq", _i64), ("Hkv", _i64), ("n_freqs", _i64),
+        ("dtype", _i32), ("inverse", _i32), ("pos64", _i32), ("reserved", _i32),
+        ("positions", _p), ("pos_sa", _i64), ("pos_sb", _i64), ("pos_ss", _i64),
+        ("q", RopeRows), ("k", RopeRows), ("v", RopeRows), ("slots", _p), ("n_pages", _i64),
+        ("turn", ctypes.c_uint64 * ROPE_MAX_FREQS), ("axis", ctypes.c_uint8 * ROPE_MAX_FREQS),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """``fade_paged_attn_args`` of include/fade_hip.h."""
+
+    _fields_ = [
+        ("B", _i64), ("T", _i64), ("Hq", _i64), ("Hkv", _i64), ("D", _i64), ("n_pages", _i64), ("pages_per_row", _i64),
+        ("q", _p), ("q_st", _i64), ("q_sh", _i64), ("out", _p), ("o_st", _i64), ("o_sh", _i64),
+        ("k_pages", _p), ("v_pages", _p), ("table", _p), ("lens", _p), ("starts", _p),
+        ("sm_scale", ctypes.c_float), ("mask_mode", _i32), ("dtype", _i32), ("zero_tail", _i32),
+    ]
+
+
 # name -> argtypes; every function returns int (status) unless listed in _RESTYPES.
 _SIGNATURES: dict[str, list] = {
     "fade_hip_abi_version": [],
@@ -200,6 +246,11 @@ _SIGNATURES: dict[str, list] = {
     "fade_tiered_prefill_attn": [ctypes.POINTER(PrefillArgs), _p],
     "fade_tiered_prefill_workspace_bytes": [ctypes.POINTER(PrefillArgs), _pi64],
     "fade_tiered_prefill_attn_ws": [ctypes.POINTER(PrefillArgs), _p, _i64, _p],
+    "fade_page_slots": [ctypes.POINTER(PageSlotsArgs), _p],
+    "fade_rope_axes": [ctypes.POINTER(RopeArgs), _p],
+    "fade_paged_append": [ctypes.POINTER(RopeArgs), _p],
+    "fade_paged_attn_workspace_bytes": [ctypes.POINTER(PagedAttnArgs), _pi64],
+    "fade_paged_attn": [ctypes.POINTER(PagedAttnArgs), _p, _i64, _p],
 }
 _RESTYPES = {"fade_hip_last_error": ctypes.c_char_p}
 
@@ -252,6 +303,35 @@ def check(rc: int, what: str) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
+
+
+def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
+    """An entry point of one argument struct, on the current stream of ``device`` (made the
+    current device: the default stream's handle is the current device's)."""
+    fn = getattr(load(), name)
+    if device.index == torch.cuda.current_device():
+        check(fn(ctypes.byref(args), current_stream_handle(device)), name)
+        return
+    with torch.cuda.device(device):
+        check(fn(ctypes.byref(args), current_stream_handle(device)), name)
+
+
+def no_gradient(op: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse a call that would have to record a gradient: the op has no backward pass."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{op}: has no backward pass (call it under torch.no_grad())")
+
+
+def written(op: str, *tensors: torch.Tensor) -> None:
+    """Tensors of the caller's that a kernel is about to write: an in-place write, to autograd as well."""
+    for t in tensors:
+        if t.is_inference():
+            if not torch.is_inference_mode_enabled():
+                raise RuntimeError(f"{op}: in-place write to an inference tensor outside inference mode")
+        else:
+            torch.autograd.graph.increment_version(t)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

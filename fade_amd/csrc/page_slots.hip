@@ -1,0 +1,253 @@
+// Block tables and slot maps of a paged cache, built on the GPU from the rows'
+// token counts.
+//
+// Row b holds lens[b] tokens and gets new[b] more; a row with reset[b] starts
+// anew (its pages go back to the free ones, its tokens count from 0).  With
+// pages(x) = ceil(x / 64), held_b = lens[b] (0 for a row that starts anew) and
+// need_b = pages(held_b + new_b) - pages(held_b), page j >= pages(held_b) of row b
+// is the free page number sum_{a < b} need_a + j - pages(held_b), and token i of the
+// row's new ones sits at position held_b + i, slot 64 * page + position % 64.
+// Free pages are a ring: taken at its head, put back behind its tail.  What this
+// call puts back lies outside what it takes, so nothing waits for another
+// workgroup, and a call repeated on the same inputs writes the same values.
+//
+// One launch.  Every workgroup sums the counts of all rows by itself (in LDS: the
+// rows' token starts, page starts and returned-page starts) and then writes its
+// share of the outputs: entries of the table and slots of the new tokens.  What
+// bounds it is latency (the counts' loads, the sums' barriers, a token's search
+// and table read), not the bytes.
+#include "fade_common.h"
+
+namespace fade {
+namespace {
+
+constexpr int kPage = 64;
+constexpr int kThreads = 256;
+
+struct SlotParams {
+  int B, ppr, n_tokens, cap;
+  const int32_t* lens;
+  const int32_t* fresh;
+  const uint8_t* reset;
+  const int32_t* table;
+  int32_t* free_pages;
+  const int32_t* ring;
+  int32_t* table_out;
+  int32_t* lens_out;
+  int32_t* starts;
+  int32_t* slots;
+  int32_t* positions;
+  int32_t* ring_out;
+  int32_t* status;
+};
+
+__device__ __forceinline__ int pages_of(int tokens) { return (tokens + (kPage - 1)) / kPage; }
+
+// ROWS: the most rows of the instance.
+template <int ROWS>
+__global__ __launch_bounds__(kThreads) void page_slots_kernel(SlotParams p) {
+  constexpr int PER = ROWS / kThreads;  // rows per thread
+  __shared__ int32_t s_start[ROWS + 1];  // first new token of a row
+  __shared__ int32_t s_need[ROWS + 1];   // its first free page, counted from the head
+  __shared__ int32_t s_back[ROWS + 1];   // the first place behind the tail for its returned pages
+  __shared__ int32_t s_lens[ROWS];       // tokens held; ~tokens where the row starts anew
+  __shared__ int64_t s_wave[2][kThreads / 64];
+  __shared__ int32_t s_bad;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row_cap = static_cast<int64_t>(p.ppr) * kPage;
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+
+  // this thread's rows tid * PER ..: their counts, summed over the workgroup (tokens
+  // in 64 bits; needed and returned pages, at most B * ppr < 2^31 each, side by side)
+  int n_tok[PER], n_need[PER], n_back[PER];
+  int64_t tok = 0, pg = 0;
+  int bad = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int b = tid * PER + i;
+    n_tok[i] = n_need[i] = n_back[i] = 0;
+    if (b < p.B) {
+      int held = p.lens[b], add = p.fresh[b];
+      const bool again = p.reset != nullptr && p.reset[b] != 0;
+      if (held < 0 || held > row_cap || add < 0) {
+        bad |= FADE_SLOTS_BAD_COUNT;
+        held = add = 0;
+      }
+      const int from = again ? 0 : held;
+      if (from + static_cast<int64_t>(add) > row_cap) {
+        bad |= FADE_SLOTS_ROW_FULL;
+        add = 0;
+      }
+      s_lens[b] = again ? ~held : held;
+      n_tok[i] = add;
+      n_need[i] = pages_of(from + add) - pages_of(from);
+      n_back[i] = again ? pages_of(held) : 0;
+      tok += n_tok[i];
+      pg += (static_cast<int64_t>(n_back[i]) << 32) + n_need[i];
+    }
+  }
+  if (bad) atomicOr(&s_bad, bad);
+  int64_t it = tok, ip = pg;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t a = __shfl_up(it, o, 64), c = __shfl_up(ip, o, 64);
+    if (lane >= o) {
+      it += a;
+      ip += c;
+    }
+  }
+  if (lane == 63) {
+    s_wave[0][wave] = it;
+    s_wave[1][wave] = ip;
+  }
+  __syncthreads();
+  int64_t all_tok = 0, all_pg = 0;
+  it -= tok;
+  ip -= pg;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < wave) {
+      it += s_wave[0][w];
+      ip += s_wave[1][w];
+    }
+    all_tok += s_wave[0][w];
+    all_pg += s_wave[1][w];
+  }
+  const int need = static_cast<int>(all_pg & 0xFFFFFFFF), back = static_cast<int>(all_pg >> 32);
+  const int head = p.ring[0], count = p.ring[1];
+  int fail = s_bad;
+  if (head < 0 || head >= p.cap || count < 0 || count > p.cap - back) fail |= FADE_SLOTS_BAD_COUNT;
+  else if (need > count) fail |= FADE_SLOTS_EXHAUSTED;
+  if (all_tok > p.n_tokens) fail |= FADE_SLOTS_TOO_MANY;
+  int64_t rt = it, rp = ip;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int b = tid * PER + i;
+    if (b < p.B) {
+      s_start[b] = static_cast<int32_t>(rt);
+      s_need[b] = static_cast<int32_t>(rp & 0xFFFFFFFF);
+      s_back[b] = static_cast<int32_t>(rp >> 32);
+    }
+    rt += n_tok[i];
+    rp += (static_cast<int64_t>(n_back[i]) << 32) + n_need[i];
+  }
+  if (tid == 0) {
+    s_start[p.B] = static_cast<int32_t>(all_tok);
+    s_need[p.B] = need;
+    s_back[p.B] = back;
+  }
+  __syncthreads();
+
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
+  const int64_t entries = static_cast<int64_t>(p.B) * p.ppr;
+  if (fail) {  // nothing changes
+    for (int64_t e = first; e < entries; e += stride) p.table_out[e] = p.table[e];
+    for (int64_t t = first; t < p.n_tokens; t += stride) {
+      p.slots[t] = -1;
+      p.positions[t] = 0;
+    }
+    for (int64_t b = first; b < p.B; b += stride) p.lens_out[b] = p.lens[b];
+    for (int64_t b = first; b <= p.B; b += stride) p.starts[b] = 0;
+    if (first == 0) {
+      p.ring_out[0] = head;
+      p.ring_out[1] = count;
+      p.status[0] = fail;
+    }
+    return;
+  }
+  // free page number j from the head, place j behind the tail (sums below 2^32)
+  const uint32_t cap = static_cast<uint32_t>(p.cap);
+  auto taken = [&](int j) { return p.free_pages[(static_cast<uint32_t>(head) + static_cast<uint32_t>(j)) % cap]; };
+  for (int64_t e = first; e < entries; e += stride) {
+    const int b = static_cast<int>(e / p.ppr), j = static_cast<int>(e - static_cast<int64_t>(b) * p.ppr);
+    const int raw = s_lens[b], old = pages_of(raw < 0 ? ~raw : raw), have = raw < 0 ? 0 : old;
+    const int mine = s_need[b + 1] - s_need[b];
+    int id = 0;
+    if (j < old) {
+      id = p.table[e];
+      if (raw < 0) {
+        p.free_pages[(static_cast<uint64_t>(head) + count + s_back[b] + j) % cap] = id;
+        id = 0;
+      }
+    }
+    if (j >= have && j < have + mine) id = taken(s_need[b] + j - have);
+    p.table_out[e] = id;
+  }
+  for (int64_t t = first; t < p.n_tokens; t += stride) {
+    int slot = -1, pos = 0;
+    if (t < all_tok) {
+      // the last row that starts at or before t
+      int lo = 0, hi = p.B;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_start[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int raw = s_lens[lo], from = raw < 0 ? 0 : raw, have = pages_of(from);
+      pos = from + static_cast<int>(t) - s_start[lo];
+      const int j = pos / kPage;
+      const int id = j < have ? p.table[static_cast<int64_t>(lo) * p.ppr + j] : taken(s_need[lo] + j - have);
+      slot = id * kPage + pos % kPage;
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+  }
+  for (int64_t b = first; b <= p.B; b += stride) {
+    p.starts[b] = s_start[b];
+    if (b < p.B) p.lens_out[b] = (s_lens[b] < 0 ? 0 : s_lens[b]) + s_start[b + 1] - s_start[b];
+  }
+  if (first == 0) {
+    p.ring_out[0] = static_cast<int32_t>((static_cast<uint32_t>(head) + static_cast<uint32_t>(need)) % cap);
+    p.ring_out[1] = count - need + back;
+    p.status[0] = 0;
+  }
+}
+
+}  // namespace
+}  // namespace fade
+
+using namespace fade;
+
+FADE_API int fade_page_slots(const fade_page_slots_args* a, void* stream) {
+  if (a == nullptr) return einval("fade_page_slots: null args");
+  if (a->B < 1 || a->B > FADE_SLOTS_MAX_ROWS)
+    return einval("fade_page_slots: 1 to %d rows, got %lld", FADE_SLOTS_MAX_ROWS, (long long)a->B);
+  if (a->pages_per_row < 1 || a->pages_per_row > (1 << 24) || a->B * a->pages_per_row >= (1ll << 31))
+    return einval("fade_page_slots: pages_per_row must be 1 to 2^24 with fewer than 2^31 table entries");
+  if (a->n_tokens < 0 || a->n_tokens >= (1ll << 31)) return einval("fade_page_slots: n_tokens must be 0 to 2^31 - 1");
+  if (a->n_free < 1 || a->n_free >= (1ll << 31) / kPage - 1) return einval("fade_page_slots: bad size of the free ring");
+  if (!a->lens || !a->new_tokens || !a->table || !a->free_pages || !a->ring || !a->table_out || !a->lens_out || !a->starts ||
+      !a->ring_out || !a->status || (a->n_tokens > 0 && (!a->slots || !a->positions)))
+    return einval("fade_page_slots: null pointer");
+  if (a->lens_out == a->lens || a->ring_out == a->ring || a->lens_out == a->new_tokens || a->starts == a->lens ||
+      a->starts == a->new_tokens)
+    return einval("fade_page_slots: lens_out, starts and ring_out must be other memory than the counts and the ring "
+                  "(every workgroup reads them)");
+  SlotParams p;
+  p.B = static_cast<int>(a->B);
+  p.ppr = static_cast<int>(a->pages_per_row);
+  p.n_tokens = static_cast<int>(a->n_tokens);
+  p.cap = static_cast<int>(a->n_free);
+  p.lens = a->lens;
+  p.fresh = a->new_tokens;
+  p.reset = a->reset;
+  p.table = a->table;
+  p.free_pages = a->free_pages;
+  p.ring = a->ring;
+  p.table_out = a->table_out;
+  p.lens_out = a->lens_out;
+  p.starts = a->starts;
+  p.slots = a->slots;
+  p.positions = a->positions;
+  p.ring_out = a->ring_out;
+  p.status = a->status;
+  const int64_t most = a->B * a->pages_per_row > a->n_tokens ? a->B * a->pages_per_row : a->n_tokens;
+  int64_t blocks = cdiv(most, kThreads);
+  if (blocks > 2 * num_cus()) blocks = 2 * num_cus();
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (a->B <= 256) hipLaunchKernelGGL(page_slots_kernel<256>, grid, dim3(kThreads), 0, as_stream(stream), p);
+  else hipLaunchKernelGGL(page_slots_kernel<FADE_SLOTS_MAX_ROWS>, grid, dim3(kThreads), 0, as_stream(stream), p);
+  return check_launch("fade_page_slots");
+}

@@ -1,0 +1,211 @@
+// Rotary positions of several axes (time, height, width), and the append of
+// rotated keys and of values to a paged cache.
+//
+// With r rotated channels of D, frequency i < r / 2 turns the channel pair
+// (i, i + r / 2) of a token by the angle pos[axis(i)] * inv_freq_i:
+//   y_i = x_i cos - x_{i + r/2} sin,   y_{i + r/2} = x_{i + r/2} cos + x_i sin
+// and the channels past r stay as they are.  An angle is only needed modulo a
+// full turn, so a frequency comes as a 64-bit fraction of a turn per position,
+// round(inv_freq / (2 pi) * 2^64): position * fraction modulo 2^64 is one
+// wrapping integer product, exact to 2^-65 of a turn per position (2^-34 at
+// position 2^31), where a 32-bit float product has lost the angle long before.
+// Its top 32 bits, as a float in [-1/2, 1/2) turns, go to the hardware's sine
+// and cosine, which take turns (measured against 64 bits over 2^24 angles: 1.3e-7
+// off at most; fp32 tensors use the library's sincospi).  The products are in
+// fp32, rounded once.
+//
+// Bound by HBM: every row is read and written once.  A thread keeps one token's
+// V = 16 bytes' worth of frequencies (their sines and cosines in registers) and
+// walks the heads with them, so the trigonometry is paid once per workgroup's
+// heads and a wave's access covers whole 128-byte runs of the rows.
+#include "fade_common.h"
+
+namespace fade {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPage = 64;
+
+// Rows of one tensor [B, heads, S, D]: element strides, unit stride along D.
+struct Rows {
+  const void* src;
+  void* dst;
+  int64_t s_sb, s_sh, s_ss;
+  int64_t d_sb, d_sh, d_ss;
+};
+
+struct RopeParams {
+  int64_t tokens, S;  // B * S of them
+  int D, half;        // channels of a row, rotated pairs
+  int Hq, Hkv, Hv;    // heads of q, k, v (v only in an append)
+  int heads_per_block;
+  int inverse, append;
+  const void* pos;    // axis a of token (b, s) at a * pos_sa + b * pos_sb + s * pos_ss
+  int64_t pos_sa, pos_sb, pos_ss;
+  int pos64;
+  Rows q, k, v;       // append: k.dst, v.dst are pages [n_pages][Hkv][64][D]
+  const int32_t* slots;
+  int64_t n_pages;
+  uint64_t turn[FADE_ROPE_MAX_FREQS];
+  uint8_t axis[FADE_ROPE_MAX_FREQS];
+};
+
+// sine and cosine of an angle in turns
+template <typename T>
+__device__ __forceinline__ void sincos_turns(float t, float& s, float& c) {
+  if constexpr (sizeof(T) == 4) {
+    sincospif(2.0f * t, &s, &c);
+  } else {
+    s = __builtin_amdgcn_sinf(t);
+    c = __builtin_amdgcn_cosf(t);
+  }
+}
+
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Vec {
+  T e[V];
+};
+
+// T: uint16_t (fp16 bits), Bf16 or float; V: channels per access.  A unit of
+// work is 2 V channels of a row: pairs V u .. of the rotated halves, or the
+// channels r + 2 V (u - half / V) .. past them.
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
+  typedef Vec<T, V> Vt;
+  const int units = p.D / (2 * V);
+  const int per_block = kThreads / units;
+  const int u = threadIdx.x % units;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / units;
+  if (threadIdx.x >= per_block * units || t >= p.tokens) return;
+  const int64_t b = t / p.S, s = t - b * p.S;
+  const int rot_units = p.half / V;
+  const bool rot = u < rot_units;
+  const int c0 = rot ? V * u : 2 * p.half + 2 * V * (u - rot_units);  // the unit's first channel
+  const int c1 = rot ? c0 + p.half : c0 + V;                          // and the first of its other V
+
+  float sn[V], cs[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    sn[i] = 0.0f;
+    cs[i] = 1.0f;
+    if (rot && p.pos != nullptr) {
+      const int f = c0 + i;
+      const int64_t at = p.axis[f] * p.pos_sa + b * p.pos_sb + s * p.pos_ss;
+      const int64_t ps = p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : static_cast<const int32_t*>(p.pos)[at];
+      const uint64_t a = static_cast<uint64_t>(ps) * p.turn[f];
+      sincos_turns<T>(static_cast<float>(static_cast<int32_t>(a >> 32)) * 0x1p-32f, sn[i], cs[i]);
+      if (p.inverse) sn[i] = -sn[i];
+    }
+  }
+  int64_t page = 0, off = 0;
+  bool store = true;
+  if (p.append) {
+    const int32_t slot = p.slots[t];
+    page = slot / kPage;
+    off = slot % kPage;
+    store = slot >= kPage && page < p.n_pages;  // page 0 holds no tokens
+  }
+  const int h0 = blockIdx.y * p.heads_per_block, all = p.Hq + p.Hkv + p.Hv;
+  const int h1 = h0 + p.heads_per_block < all ? h0 + p.heads_per_block : all;
+#pragma unroll 4
+  for (int hh = h0; hh < h1; ++hh) {
+    const bool is_q = hh < p.Hq, is_k = !is_q && hh < p.Hq + p.Hkv;
+    const Rows& r = is_q ? p.q : (is_k ? p.k : p.v);
+    const int h = is_q ? hh : (is_k ? hh - p.Hq : hh - p.Hq - p.Hkv);
+    const bool paged = p.append && !is_q;
+    if (paged && !store) continue;
+    const T* src = static_cast<const T*>(r.src) + b * r.s_sb + h * r.s_sh + s * r.s_ss;
+    T* dst = static_cast<T*>(r.dst) + (paged ? ((page * p.Hkv + h) * kPage + off) * p.D : b * r.d_sb + h * r.d_sh + s * r.d_ss);
+    const Vt x = *reinterpret_cast<const Vt*>(src + c0), y = *reinterpret_cast<const Vt*>(src + c1);
+    Vt a = x, c = y;
+    if (rot && (is_q || is_k)) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float xf = to_f32(x.e[i]), yf = to_f32(y.e[i]);
+        a.e[i] = from_f32<T>(xf * cs[i] - yf * sn[i]);
+        c.e[i] = from_f32<T>(yf * cs[i] + xf * sn[i]);
+      }
+    }
+    *reinterpret_cast<Vt*>(dst + c0) = a;
+    *reinterpret_cast<Vt*>(dst + c1) = c;
+  }
+}
+
+template <typename T>
+int rope_launch(RopeParams& p, bool wide, void* stream) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  const int units = p.D / (2 * (wide ? V : 1));
+  const int64_t bx = cdiv(p.tokens, kThreads / units);
+  const int all = p.Hq + p.Hkv + p.Hv;
+  // heads are spread over workgroups while there are fewer than four per CU
+  int split = 1;
+  while (bx * split < 4 * num_cus() && split < all) split *= 2;
+  if (split > all) split = all;
+  p.heads_per_block = static_cast<int>(cdiv(all, split));
+  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(cdiv(all, p.heads_per_block)));
+  if (wide) hipLaunchKernelGGL((rope_kernel<T, V>), grid, dim3(kThreads), 0, as_stream(stream), p);
+  else hipLaunchKernelGGL((rope_kernel<T, 1>), grid, dim3(kThreads), 0, as_stream(stream), p);
+  return check_launch("fade_rope_axes");
+}
+
+int rope_any(const fade_rope_args* a, bool append, const char* what, void* stream) {
+  if (a == nullptr) return einval("%s: null args", what);
+  if (a->dtype != FADE_DTYPE_F16 && a->dtype != FADE_DTYPE_BF16 && (append || a->dtype != FADE_DTYPE_F32))
+    return einval("%s: unknown dtype %d", what, a->dtype);
+  if (a->D < 2 || a->D > 2 * FADE_ROPE_MAX_FREQS || a->D % 2) return einval("%s: head_dim must be even, 2 to 256, got %lld", what, (long long)a->D);
+  if (a->n_freqs < 0 || 2 * a->n_freqs > a->D) return einval("%s: %lld frequencies for head_dim %lld", what, (long long)a->n_freqs, (long long)a->D);
+  if (a->B < 0 || a->S < 0 || a->Hq < 0 || a->Hkv < 0 || a->Hq > 65535 || a->Hkv > 65535) return einval("%s: bad shape", what);
+  if (append && a->B > 1) return einval("%s: tokens come as one row", what);
+  if (a->S != 0 && a->B > (1ll << 31) / a->S) return einval("%s: shape too large", what);
+  const int64_t tokens = a->B * a->S;
+  if (tokens == 0 || a->Hq + a->Hkv == 0) return FADE_OK;
+  if ((a->Hq > 0 && (!a->q.src || !a->q.dst)) || (a->Hkv > 0 && (!a->k.src || !a->k.dst))) return einval("%s: null q or k", what);
+  if (append && (!a->slots || (a->Hkv > 0 && (!a->v.src || !a->v.dst)) || a->n_pages < 1 || a->n_pages >= (1ll << 31) / kPage))
+    return einval("%s: null v or slots, or a bad number of pages", what);
+  if (!append && a->n_freqs > 0 && a->positions == nullptr) return einval("%s: null positions", what);
+  RopeParams p{};
+  p.tokens = tokens;
+  p.S = a->S;
+  p.D = static_cast<int>(a->D);
+  p.half = static_cast<int>(a->n_freqs);
+  p.Hq = static_cast<int>(a->Hq);
+  p.Hkv = static_cast<int>(a->Hkv);
+  p.Hv = append ? p.Hkv : 0;
+  p.inverse = a->inverse;
+  p.append = append;
+  p.pos = a->positions;
+  p.pos_sa = a->pos_sa;
+  p.pos_sb = a->pos_sb;
+  p.pos_ss = a->pos_ss;
+  p.pos64 = a->pos64;
+  p.slots = a->slots;
+  p.n_pages = a->n_pages;
+  for (int i = 0; i < p.half; ++i) {
+    p.turn[i] = a->turn[i];
+    p.axis[i] = a->axis[i];
+  }
+  // 16-byte accesses: whole units of both halves and aligned rows
+  const int V = a->dtype == FADE_DTYPE_F32 ? 4 : 8, size = 16 / V;
+  bool wide = p.D % (2 * V) == 0 && p.half % V == 0;
+  auto rows = [&](const fade_rope_rows& x, bool paged) {
+    Rows r{x.src, x.dst, x.src_sb, x.src_sh, x.src_ss, x.dst_sb, x.dst_sh, x.dst_ss};
+    uintptr_t m = reinterpret_cast<uintptr_t>(x.src) | reinterpret_cast<uintptr_t>(x.dst);
+    m |= static_cast<uintptr_t>((a->B > 1 ? r.s_sb : 0) | r.s_sh | r.s_ss) * size;
+    if (!paged) m |= static_cast<uintptr_t>((a->B > 1 ? r.d_sb : 0) | r.d_sh | r.d_ss) * size;
+    if (m % 16) wide = false;
+    return r;
+  };
+  if (p.Hq) p.q = rows(a->q, false);
+  if (p.Hkv) p.k = rows(a->k, append);
+  if (p.Hv) p.v = rows(a->v, append);
+  if (a->dtype == FADE_DTYPE_F16) return rope_launch<uint16_t>(p, wide, stream);
+  if (a->dtype == FADE_DTYPE_BF16) return rope_launch<Bf16>(p, wide, stream);
+  return rope_launch<float>(p, wide, stream);
+}
+
+}  // namespace
+}  // namespace fade
+
+FADE_API int fade_rope_axes(const fade_rope_args* a, void* stream) { return fade::rope_any(a, false, "fade_rope_axes", stream); }
+
+FADE_API int fade_paged_append(const fade_rope_args* a, void* stream) { return fade::rope_any(a, true, "fade_paged_append", stream); }

@@ -16,7 +16,12 @@ own pages point at it, so gathering a row's pages back into a padded tensor
 gives zeros past the row's tokens, which is what the quantizers write for the
 zero-padded rows of the unpaged layout: ``gather(store(x))`` is ``x``.
 
-Pages are allocated and freed on the host (a free list); the copies into and
+``TokenPagePool`` holds whole 16-bit rows (a prompt's tokens before the compression,
+rows of different lengths) in the same 64-token pages.  Its block tables, slot maps
+and free pages stay on the GPU: ``page_slots`` makes them from the rows' token counts
+in one launch.
+
+``MiddlePagePool``: pages are allocated and freed on the host (a free list); the copies into and
 out of the pool run on the current stream, so a page freed by one
 reassignment and reused by the next is overwritten only after every earlier
 read of it in stream order.
@@ -24,8 +29,12 @@ read of it in stream order.
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 from torch import Tensor
+
+from . import _lib
 
 PAGE_TOKENS = 64
 
@@ -153,4 +162,145 @@ class MiddlePagePool:
         return one(self.k_codes), one(self.v_codes), one(self.v_scale)
 
 
-__all__ = ["MiddlePagePool", "PAGE_TOKENS"]
+@dataclass
+class PageSlots:
+    """What ``page_slots`` writes (int32, on the GPU).
+
+    ``table`` [B, pages_per_row]: each row's pages, 0 past them.  ``lens`` [B]: its tokens,
+    the new ones included.  ``starts`` [B + 1]: the first of its new tokens among all.
+    ``slots`` / ``positions`` [n_tokens]: where each new token goes (64 * page + place in
+    it) and its position in the row; -1 and 0 past the last one.  ``ring`` [2]: the first
+    free page's place and the number of free pages.  ``status`` [1]: 0, or why nothing
+    was done (``check()``)."""
+
+    table: Tensor
+    lens: Tensor
+    starts: Tensor
+    slots: Tensor
+    positions: Tensor
+    ring: Tensor
+    status: Tensor
+
+    def check(self) -> "PageSlots":
+        """Raise RuntimeError where the call was not done (reads the status: a host synchronization)."""
+        word = int(self.status.item())
+        if word:
+            what = ", ".join(t for b, t in _lib.SLOTS_STATUS.items() if word & b)
+            raise RuntimeError(f"page_slots: {what} (nothing was changed)")
+        return self
+
+
+def page_slots(
+    lens: Tensor,
+    new: Tensor,
+    table: Tensor,
+    free: Tensor,
+    ring: Tensor,
+    n_tokens: int,
+    reset: Tensor | None = None,
+    out: PageSlots | None = None,
+) -> PageSlots:
+    """Block table and slot map of a step, from the rows' token counts, in one launch and
+    without a host synchronization.
+
+    Row b holds ``lens[b]`` tokens and gets ``new[b]`` more (int32 [B], B up to 4096);
+    with ``reset`` (bool or uint8 [B]) a marked row returns its pages first and starts
+    anew.  ``table`` int32 [B, pages_per_row] is the present block table, ``free``
+    int32 [n] the ring of free pages, written where pages are returned (those are handed out
+    from the next call on), ``ring`` int32 [2] its first entry and count.  ``n_tokens``
+    is the size of the slot map: at least the new tokens.  ``out`` takes the results
+    (its ``table`` may be ``table`` itself, its other tensors not the inputs).
+
+    All or nothing: where pages run out, a row's table is too short, ``n_tokens`` is too
+    small or a count is impossible, ``status`` says so, the table, the lengths and the
+    ring come out as they went in, and the slot map is empty.  The same inputs give the
+    same results again, so a captured graph can be replayed on them.
+    """
+    op = "page_slots"
+    _lib.require_gpu(lens, new, table, free, ring, reset, op=op)
+    if table.dim() != 2:
+        raise ValueError(f"{op}: table must be [B, pages_per_row], got {tuple(table.shape)}")
+    B, ppr = (int(x) for x in table.shape)
+    n = int(n_tokens)
+    if n < 0:
+        raise ValueError(f"{op}: n_tokens must be >= 0, got {n}")
+    for name, t, shape in (("lens", lens, (B,)), ("new", new, (B,)), ("table", table, (B, ppr)), ("free", free, (free.numel(),)),
+                           ("ring", ring, (2,))):
+        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} {list(t.shape)}")
+    if reset is not None and (reset.dtype not in (torch.bool, torch.uint8) or tuple(reset.shape) != (B,) or not reset.is_contiguous()):
+        raise ValueError(f"{op}: reset must be a contiguous bool or uint8 [B={B}], got {reset.dtype} {list(reset.shape)}")
+    sizes = [B * ppr, B, B + 1, n, n, 2, 1]
+    if out is None:
+        parts = torch.empty(sum(sizes), dtype=torch.int32, device=table.device).split(sizes)
+        out = PageSlots(parts[0].view(B, ppr), *parts[1:])
+    else:
+        for name, size in zip(("table", "lens", "starts", "slots", "positions", "ring", "status"), sizes):
+            t = getattr(out, name)
+            if t.dtype != torch.int32 or t.numel() != size or not t.is_contiguous() or t.device != table.device:
+                raise ValueError(f"{op}: out.{name} must be contiguous int32 of {size} elements on {table.device}")
+        _lib.written(op, out.table, out.lens, out.starts, out.slots, out.positions, out.ring, out.status)
+    _lib.written(op, free)
+    a = _lib.PageSlotsArgs()
+    a.B, a.pages_per_row, a.n_tokens, a.n_free = B, ppr, n, free.numel()
+    a.lens, a.new_tokens, a.reset = lens.data_ptr(), new.data_ptr(), _lib.ptr(reset)
+    a.table, a.free_pages, a.ring = table.data_ptr(), free.data_ptr(), ring.data_ptr()
+    a.table_out, a.lens_out, a.starts = out.table.data_ptr(), out.lens.data_ptr(), out.starts.data_ptr()
+    a.slots, a.positions = out.slots.data_ptr(), out.positions.data_ptr()
+    a.ring_out, a.status = out.ring.data_ptr(), out.status.data_ptr()
+    _lib.launch("fade_page_slots", a, table.device)
+    return out
+
+
+class TokenPagePool:
+    """``n_pages`` pages of 64 tokens of 16-bit K and V: ``k``, ``v`` [n_pages + 1, Hkv, 64, D]
+    of ``dtype`` (page 0 holds no tokens), and the free pages on the GPU.
+
+    One step of a batch: ``state = pool.step(state, new, n_tokens)`` gives every new
+    token its slot, ``paged_append`` writes K and V there, ``paged_attention`` reads
+    the rows' pages.  ``start`` gives the state of an empty batch.  Several layers share
+    one pool's tables by holding tensors like ``k`` and ``v`` of their own."""
+
+    def __init__(self, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16, device="cuda") -> None:
+        if n_pages < 1 or n_kv_heads < 1 or head_dim < 8 or head_dim % 8 or head_dim > 256:
+            raise ValueError(f"TokenPagePool needs n_pages >= 1, n_kv_heads >= 1 and a head_dim that is a multiple of 8 "
+                             f"up to 256, got {n_pages}, {n_kv_heads}, {head_dim}")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"TokenPagePool holds float16 or bfloat16, got {dtype}")
+        self.n_pages, self.n_kv_heads, self.head_dim = int(n_pages), int(n_kv_heads), int(head_dim)
+        shape = (self.n_pages + 1, self.n_kv_heads, PAGE_TOKENS, self.head_dim)
+        self.k = torch.zeros(shape, dtype=dtype, device=device)
+        self.v = torch.zeros(shape, dtype=dtype, device=device)
+        self.free = torch.arange(1, self.n_pages + 1, dtype=torch.int32, device=device)
+        self.ring = torch.tensor([0, self.n_pages], dtype=torch.int32, device=device)
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
+    def start(self, batch: int, pages_per_row: int) -> PageSlots:
+        """The state of ``batch`` empty rows of at most ``pages_per_row`` pages."""
+        z = lambda *s: torch.zeros(s, dtype=torch.int32, device=self.device)  # noqa: E731
+        return PageSlots(z(batch, pages_per_row), z(batch), z(batch + 1), z(0), z(0), self.ring, z(1))
+
+    def step(self, state: PageSlots, new: Tensor, n_tokens: int, reset: Tensor | None = None) -> PageSlots:
+        """``page_slots`` for the next ``new[b]`` tokens of every row; the pool keeps the ring."""
+        nxt = page_slots(state.lens, new, state.table, self.free, self.ring, n_tokens, reset=reset)
+        self.ring = nxt.ring
+        return nxt
+
+    def gather(self, table: Tensor, length: int) -> tuple[Tensor, Tensor]:
+        """K and V [B, Hkv, length, D] that a block table describes (what stands in a row's
+        pages past its own tokens included), e.g. to compress them."""
+        B, ppr = (int(d) for d in table.shape)
+        if length > ppr * PAGE_TOKENS:
+            raise ValueError(f"length {length} exceeds the table's {ppr} pages per row")
+        pages = table[:, : -(-length // PAGE_TOKENS)].long()
+
+        def one(x: Tensor) -> Tensor:
+            return x[pages].permute(0, 2, 1, 3, 4).reshape(B, self.n_kv_heads, -1, self.head_dim)[:, :, :length].contiguous()
+
+        return one(self.k), one(self.v)
+
+
+__all__ = ["MiddlePagePool", "PAGE_TOKENS", "PageSlots", "TokenPagePool", "page_slots"]

@@ -13,9 +13,12 @@ so that ``create_tiered_cache`` resolves the same scheme from an HF config.
 
 from __future__ import annotations
 
+import ctypes
 import math
+import struct
 import warnings
 from dataclasses import dataclass, field
+from fractions import Fraction
 
 import torch
 from torch import Tensor
@@ -29,6 +32,7 @@ DEFAULT_YARN_BETA_FAST: float = 32.0
 DEFAULT_YARN_BETA_SLOW: float = 1.0
 
 _HOST = torch.device("cpu")
+_PI = Fraction("3.14159265358979323846264338327950288419716939937511")
 
 
 def _vanilla_inv_freq(head_dim: int, theta: float, device=_HOST) -> Tensor:
@@ -44,6 +48,7 @@ class RopeScheme:
     theta: float = DEFAULT_ROPE_THETA
     head_dim: int = 64
     _inv_cache: Tensor | None = field(default=None, init=False, repr=False, compare=False)
+    _turn_cache: tuple | None = field(default=None, init=False, repr=False, compare=False)
 
     def _compute_inv_freq(self) -> Tensor:
         return _vanilla_inv_freq(self.head_dim, self.theta)
@@ -79,6 +84,28 @@ class RopeScheme:
     def is_rope(self) -> bool:
         return True
 
+    @property
+    def n_axes(self) -> int:
+        """Axes of the positions (time, height, width, ...) that the frequencies are shared out to."""
+        return 1
+
+    def freq_axes(self) -> list[int]:
+        """The axis whose position turns each frequency."""
+        return [0] * int(self.inv_freq().shape[0])
+
+    def _turn_fractions(self) -> list[Fraction]:
+        """Full turns per position of each frequency, from its fp32 inverse frequency."""
+        return [Fraction(f) / (2 * _PI) for f in self.inv_freq().tolist()]
+
+    def turns(self) -> tuple[bytes, bytes]:
+        """``fade_rope_args``' frequencies: each one's turns per position as a 64-bit fraction
+        (so that position * fraction modulo 2^64 is the angle, exactly reduced) in 8 bytes, and
+        its axis in one."""
+        if self._turn_cache is None:
+            frac = [round(f * 2**64) % 2**64 for f in self._turn_fractions()]
+            self._turn_cache = (struct.pack(f"={len(frac)}Q", *frac), bytes(self.freq_axes()))
+        return self._turn_cache
+
 
 @dataclass
 class Vanilla(RopeScheme):
@@ -93,6 +120,9 @@ class LinearScaled(RopeScheme):
 
     def _positions(self, positions: Tensor) -> Tensor:
         return positions.to(_HOST).float() / self.factor
+
+    def _turn_fractions(self) -> list[Fraction]:
+        return [f / Fraction(self.factor) for f in super()._turn_fractions()]
 
     def host_cos_sin(self, positions, model_dtype=torch.float16):
         # The reference always rounds through model_dtype for this scheme.
@@ -172,10 +202,15 @@ class Proportional(RopeScheme):
 
 @dataclass
 class MRope(RopeScheme):
-    """Qwen 3.5/3.6 multi-axis RoPE; text-only positions reduce to vanilla (fade/rope.py:228-272)."""
+    """Qwen 3.5/3.6 multi-axis RoPE; text-only positions reduce to vanilla (fade/rope.py:228-272).
+
+    ``mrope_section`` gives each axis its number of frequencies: the first section
+    to axis 0, the next to axis 1, ...; ``interleaved``: frequency i belongs to axis
+    i modulo the axes while that axis has frequencies left, the rest to axis 0."""
 
     partial_rotary_factor: float = 1.0
     mrope_section: list[int] | None = None
+    interleaved: bool = False
 
     @property
     def rotary_dim(self) -> int:
@@ -183,6 +218,23 @@ class MRope(RopeScheme):
 
     def _compute_inv_freq(self) -> Tensor:
         return _vanilla_inv_freq(self.rotary_dim, self.theta)
+
+    @property
+    def n_axes(self) -> int:
+        return len(self.mrope_section) if self.mrope_section else 1
+
+    def freq_axes(self) -> list[int]:
+        n, sec = int(self.inv_freq().shape[0]), self.mrope_section
+        if not sec:
+            return [0] * n
+        if self.interleaved:
+            axes = [i % len(sec) if i < len(sec) * sec[i % len(sec)] else 0 for i in range(n)]
+        else:
+            axes = [a for a, k in enumerate(sec) for _ in range(k)]
+        if len(axes) != n or [axes.count(a) for a in range(len(sec))] != list(sec):
+            raise ValueError(f"mrope_section {list(sec)} does not share out {n} frequencies"
+                             + (" (interleaved)" if self.interleaved else ""))
+        return axes
 
     def host_cos_sin(self, positions, model_dtype=torch.float16):
         emb = self._emb(positions)
@@ -198,6 +250,9 @@ class NoRope(RopeScheme):
     def host_cos_sin(self, positions, model_dtype=torch.float16):
         n = int(positions.shape[0])
         return torch.ones(n, self.head_dim), torch.zeros(n, self.head_dim)
+
+    def turns(self) -> tuple[bytes, bytes]:
+        return b"", b""
 
     @property
     def is_rope(self) -> bool:
@@ -260,7 +315,10 @@ def extract_rope_scheme(cfg, head_dim: int | None = None) -> RopeScheme:
         mrope = getattr(cfg, "mrope_section", None)
     if mrope is not None:
         prf = float(rp.get("partial_rotary_factor", 1.0)) if isinstance(rp, dict) else 1.0
-        return MRope(theta=theta, head_dim=hd, partial_rotary_factor=prf, mrope_section=list(mrope))
+        mixed = rp.get("mrope_interleaved") if isinstance(rp, dict) else None
+        if mixed is None:
+            mixed = getattr(cfg, "mrope_interleaved", False)
+        return MRope(theta=theta, head_dim=hd, partial_rotary_factor=prf, mrope_section=list(mrope), interleaved=bool(mixed))
 
     rs = getattr(cfg, "rope_scaling", None)
     if not isinstance(rs, dict):
@@ -370,6 +428,100 @@ def rerope_gather(
     return k_out, v_out
 
 
+def rope_args(scheme: RopeScheme, head_dim: int, op: str):
+    """``fade_rope_args`` with a scheme's frequencies; the scheme keeps them."""
+    from . import _lib
+
+    turn, axis = scheme.turns()
+    if 2 * len(axis) > head_dim or head_dim > 2 * _lib.ROPE_MAX_FREQS:
+        raise ValueError(f"{op}: the scheme rotates {2 * len(axis)} channels, the rows have {head_dim} (at most "
+                         f"{2 * _lib.ROPE_MAX_FREQS})")
+    a = _lib.RopeArgs()
+    at = ctypes.addressof(a)
+    ctypes.memmove(at + _lib.RopeArgs.turn.offset, turn, len(turn))
+    ctypes.memmove(at + _lib.RopeArgs.axis.offset, axis, len(axis))
+    a.n_freqs = len(axis)
+    return a
+
+
+def rope_axes(
+    q: Tensor | None,
+    k: Tensor | None,
+    positions: Tensor,
+    scheme: RopeScheme,
+    inverse: bool = False,
+    out: tuple[Tensor | None, Tensor | None] | None = None,
+) -> tuple[Tensor | None, Tensor | None]:
+    """Rotary positions of one or several axes for queries and keys, in one launch.
+
+    ``q`` [B, Hq, S, D], ``k`` [B, Hkv, S, D] (either may be None) fp16, bf16 or fp32 on
+    the GPU, any strides with a contiguous D axis.  ``positions`` integer [S], [B, S] or
+    [axes, B, S] (B may be 1: the same for every row): an ``MRope`` scheme turns each
+    frequency by its own axis's position (time, height, width), and takes positions
+    without an axis dimension as the same on every axis.  Frequency i mixes channels i
+    and i + rotated / 2; channels past the scheme's rotated ones are copied.
+    ``inverse`` turns back.  Angles are reduced exactly whatever the position; products
+    in fp32, one rounding to the dtype.  Returns new tensors (contiguous), or ``out``
+    = (q_out, k_out), which may be the inputs themselves.
+    """
+    from . import _lib
+
+    op = "rope_axes"
+    tensors = [t for t in (q, k) if t is not None]
+    if not tensors:
+        raise ValueError(f"{op}: q or k is needed")
+    _lib.require_gpu(*tensors, positions, op=op)
+    _lib.no_gradient(op, q, k)
+    ref = tensors[0]
+    if ref.dim() != 4 or tensors[-1].dim() != 4:
+        raise ValueError(f"{op}: q and k must be [B, H, S, D], got {[tuple(t.shape) for t in tensors]}")
+    B, _, S, D = ref.shape
+    for t in tensors:
+        if (t.shape[0], t.shape[2], t.shape[3]) != (B, S, D) or t.dtype != ref.dtype:
+            raise ValueError(f"{op}: q and k differ in batch, length, head_dim or dtype: {tuple(q.shape)} {q.dtype}, "
+                             f"{tuple(k.shape)} {k.dtype}")
+    if ref.dtype not in _lib.DTYPE_CODES:
+        raise ValueError(f"{op}: expected a float16, bfloat16 or float32 tensor, got {ref.dtype}")
+    a = rope_args(scheme, D, op)
+    a.B, a.S, a.D, a.dtype, a.inverse = B, S, D, _lib.DTYPE_CODES[ref.dtype], int(bool(inverse))
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{op}: positions must be int32 or int64, got {positions.dtype}")
+    shape, axes = tuple(positions.shape), scheme.n_axes
+    if positions.dim() not in (1, 2, 3) or shape[-1] != S or (len(shape) > 1 and shape[-2] not in (1, B)) \
+            or (len(shape) == 3 and shape[0] not in (1, axes)):
+        raise ValueError(f"{op}: positions must be [S], [B, S] or [{axes}, B, S] with B={B}, S={S}, got {shape}")
+    st = positions.stride()
+    a.positions, a.pos64, a.pos_ss = positions.data_ptr(), int(positions.dtype == torch.int64), st[-1]
+    a.pos_sb = st[-2] if len(shape) > 1 and shape[-2] > 1 else 0
+    a.pos_sa = st[0] if len(shape) == 3 and shape[0] > 1 else 0
+    dst = [None, None] if out is None else list(out)
+    res, keep = [], []
+    for name, t, o in (("q", q, dst[0]), ("k", k, dst[1])):
+        if t is None:
+            res.append(None)
+            continue
+        if t.is_neg() or t.stride(3) != 1:
+            t = t.resolve_neg().contiguous()
+            keep.append(t)
+        if o is None:
+            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        else:
+            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(3) != 1 or o.is_neg():
+                raise ValueError(f"{op}: out must be like the input with a contiguous head_dim axis, got {o.dtype} {tuple(o.shape)}")
+            _lib.no_gradient(op, o)
+            _lib.written(op, o)
+        r = a.q if name == "q" else a.k
+        r.src, r.src_sb, r.src_sh, r.src_ss = t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
+        r.dst, r.dst_sb, r.dst_sh, r.dst_ss = o.data_ptr(), o.stride(0), o.stride(1), o.stride(2)
+        if name == "q":
+            a.Hq = t.shape[1]
+        else:
+            a.Hkv = t.shape[1]
+        res.append(o)
+    _lib.launch("fade_rope_axes", a, ref.device)
+    return res[0], res[1]
+
+
 __all__ = [
     "LinearScaled",
     "Llama3",
@@ -383,4 +535,5 @@ __all__ = [
     "extract_rope_scheme",
     "extract_rope_schemes_per_layer",
     "rerope_gather",
+    "rope_axes",
 ]

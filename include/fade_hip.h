@@ -457,6 +457,108 @@ int fade_tiered_prefill_workspace_bytes(const fade_prefill_args* args, int64_t* 
 int fade_tiered_prefill_attn_ws(const fade_prefill_args* args, void* workspace, int64_t workspace_bytes,
                                 void* stream);
 
+/* ---------------- paged 16-bit cache -------------------------------------- */
+/* A pool of pages of 64 tokens, K and V each [n_pages][Hkv][64][D]; page 0 holds
+ * no tokens.  Row b's token at position i lies in page table[b][i / 64] at
+ * i % 64; its slot is 64 * page + i % 64.  No counterpart in the reference, whose
+ * roadmap item A1 asks for paged tiers. */
+#define FADE_SLOTS_MAX_ROWS 4096
+/* status bits of fade_page_slots; with any of them set nothing changes */
+#define FADE_SLOTS_EXHAUSTED 1 /* more pages needed than are free */
+#define FADE_SLOTS_ROW_FULL 2  /* a row would pass pages_per_row * 64 tokens */
+#define FADE_SLOTS_TOO_MANY 4  /* more new tokens than n_tokens */
+#define FADE_SLOTS_BAD_COUNT 8 /* a negative or impossible count, or a broken ring */
+/* Row b holds lens[b] tokens and gets new_tokens[b] more; reset[b] != 0 (optional)
+ * returns its pages first and counts from 0.  Free pages are a ring of n_free
+ * entries, ring = {first, count}: taken at the front, returned behind the back (a
+ * page returned by a call is handed out from the next one on).  Writes the
+ * block table (table_out may be table), lens_out, starts [B + 1] (first new token
+ * of each row), slots and positions of the new tokens [n_tokens] (-1 and 0 past
+ * the last one), ring_out and status [1].  lens_out, starts and ring_out must be
+ * other memory than the inputs.  The same inputs give the same outputs again. */
+typedef struct fade_page_slots_args {
+  int64_t B, pages_per_row, n_tokens, n_free;
+  const int32_t* lens;
+  const int32_t* new_tokens;
+  const uint8_t* reset; /* or NULL */
+  const int32_t* table; /* [B][pages_per_row] */
+  int32_t* free_pages;  /* [n_free] */
+  const int32_t* ring;  /* [2] */
+  int32_t* table_out;
+  int32_t* lens_out;
+  int32_t* starts;
+  int32_t* slots;
+  int32_t* positions;
+  int32_t* ring_out;
+  int32_t* status;
+} fade_page_slots_args;
+int fade_page_slots(const fade_page_slots_args* args, void* stream);
+
+/* Rotary positions of several axes.  Frequency i < n_freqs turns the channel
+ * pair (i, i + n_freqs) of every row by position * turn[i] / 2^64 of a full turn,
+ * the position read from axis axis[i]; channels from 2 * n_freqs on stay as they
+ * are.  Products in fp32, rounded once to dtype. */
+#define FADE_ROPE_MAX_FREQS 128
+typedef struct fade_rope_rows { /* [B, heads, S, D], element strides, unit stride along D */
+  const void* src;
+  void* dst; /* may be src */
+  int64_t src_sb, src_sh, src_ss;
+  int64_t dst_sb, dst_sh, dst_ss;
+} fade_rope_rows;
+typedef struct fade_rope_args {
+  int64_t B, S, D, Hq, Hkv; /* Hq or Hkv may be 0 */
+  int64_t n_freqs;
+  int32_t dtype;            /* FADE_DTYPE_* (fade_paged_append: F16 or BF16) */
+  int32_t inverse;          /* nonzero: turn back */
+  int32_t pos64;            /* positions are int64, else int32 */
+  int32_t reserved;
+  const void* positions;    /* axis a of token (b, s) at a * pos_sa + b * pos_sb + s * pos_ss */
+  int64_t pos_sa, pos_sb, pos_ss;
+  fade_rope_rows q, k;
+  fade_rope_rows v;         /* fade_paged_append */
+  const int32_t* slots;     /* fade_paged_append: [S] */
+  int64_t n_pages;          /* fade_paged_append */
+  uint64_t turn[FADE_ROPE_MAX_FREQS];
+  uint8_t axis[FADE_ROPE_MAX_FREQS];
+} fade_rope_args;
+int fade_rope_axes(const fade_rope_args* args, void* stream);
+/* The same for one row of S new tokens (B = 1), whose rotated k and whose v go to
+ * the pages k.dst, v.dst ([n_pages][Hkv][64][D], 16-bit) at slots[s]; tokens whose
+ * slot lies outside pages 1 .. n_pages - 1 are not written there.  The slots of one
+ * call are distinct.  q (Hq may be 0) is rotated to q.dst.  positions NULL: no
+ * rotation. */
+int fade_paged_append(const fade_rope_args* args, void* stream);
+
+/* Attention of ragged chunks of new tokens over the pages: row b's queries are
+ * tokens starts[b] .. starts[b + 1] - 1 of q, its keys the lens[b] tokens that its
+ * pages hold, the new ones included.  mask_mode FADE_MASK_BOTTOM_RIGHT: query i of
+ * n sees keys 0 .. lens[b] - n + i; FADE_MASK_NONE: all of them.  A query that sees no
+ * key gets zeros; what stands in a page past a row's tokens never counts.  Rows of
+ * out at and past starts[B] are left as they were, or zeroed (zero_tail).  Any
+ * Hq / Hkv; D a multiple of 8 up to 256; dtype FADE_DTYPE_F16 or FADE_DTYPE_BF16. */
+typedef struct fade_paged_attn_args {
+  int64_t B, T, Hq, Hkv, D;  /* T: rows of q and out */
+  int64_t n_pages, pages_per_row;
+  const void* q;             /* [T, Hq, D], rows 16-byte aligned */
+  int64_t q_st, q_sh;
+  void* out;                 /* [T, Hq, D], rows 8-byte aligned */
+  int64_t o_st, o_sh;
+  const void* k_pages;       /* [n_pages][Hkv][64][D], 16-byte aligned */
+  const void* v_pages;
+  const int32_t* table;      /* [B][pages_per_row] */
+  const int32_t* lens;       /* [B] */
+  const int32_t* starts;     /* [B + 1] */
+  float sm_scale;            /* positive */
+  int32_t mask_mode;
+  int32_t dtype;
+  int32_t zero_tail;
+} fade_paged_attn_args;
+/* The keys are split over workgroups by the rows' lengths, on the device; the
+ * splits' fp32 sums go through the workspace (16-byte aligned, contents arbitrary,
+ * not shared by calls that may overlap) and are joined in a fixed order. */
+int fade_paged_attn_workspace_bytes(const fade_paged_attn_args* args, int64_t* bytes);
+int fade_paged_attn(const fade_paged_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,167 @@
+"""The paged 16-bit cache on the CPU: what the C entry points refuse, how the attention's work is
+cut (a model of the device code's sums, in its precision), and the schemes' turns."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import random
+from fractions import Fraction
+
+import numpy as np
+import pytest
+import torch
+
+from fade_amd import _lib
+from fade_amd.pages import TokenPagePool
+from fade_amd.rope import LinearScaled, MRope, NoRope, Vanilla, extract_rope_scheme
+
+PI = Fraction("3.14159265358979323846264338327950288419716939937511")
+
+
+def _call(name, args, *more):
+    return getattr(_lib.load(), name)(ctypes.byref(args), *more)
+
+
+def _attn(**kw):
+    a = _lib.PagedAttnArgs()
+    base = dict(B=2, T=8, Hq=8, Hkv=2, D=128, n_pages=9, pages_per_row=4, q=1 << 20, q_st=1024, q_sh=128, out=1 << 20, o_st=1024, o_sh=128,
+                k_pages=1 << 20, v_pages=1 << 20, table=1 << 20, lens=1 << 20, starts=1 << 20, sm_scale=0.1, mask_mode=0, dtype=0)
+    for name, x in {**base, **kw}.items():
+        setattr(a, name, x)
+    return a
+
+
+def test_attention_arguments():
+    nb = ctypes.c_int64(-1)
+    assert _call("fade_paged_attn_workspace_bytes", _attn(), nb) == 0 and nb.value >= 0
+    for bad in (dict(D=12), dict(D=264), dict(D=0), dict(B=0), dict(T=-1), dict(Hq=7), dict(Hkv=0), dict(n_pages=0), dict(pages_per_row=0),
+                dict(q=None), dict(q=(1 << 20) + 8), dict(q_st=1020), dict(o_sh=126), dict(out=(1 << 20) + 4), dict(k_pages=None),
+                dict(v_pages=(1 << 20) + 2), dict(table=None), dict(lens=None), dict(starts=None), dict(sm_scale=0.0), dict(sm_scale=-1.0),
+                dict(sm_scale=math.nan), dict(sm_scale=math.inf), dict(mask_mode=1), dict(mask_mode=9), dict(dtype=2), dict(T=1 << 25),
+                dict(T=1 << 24, Hq=512, Hkv=512, q_st=1 << 16, o_st=1 << 16)):
+        a = _attn(**bad)
+        assert _call("fade_paged_attn_workspace_bytes", a, nb) == _lib.FADE_EINVAL, bad
+        assert _lib.load().fade_hip_last_error()
+        assert _call("fade_paged_attn", a, None, 0, None) == _lib.FADE_EINVAL, bad
+    a = _attn(pages_per_row=400)  # splits: a workspace, large enough and aligned
+    assert _call("fade_paged_attn_workspace_bytes", a, nb) == 0 and nb.value > 0
+    for ws, size in ((None, nb.value), (1 << 20, nb.value - 1), ((1 << 20) + 8, nb.value)):
+        assert _call("fade_paged_attn", a, ws, size, None) == _lib.FADE_EINVAL
+    assert _call("fade_paged_attn", _attn(T=0), None, 0, None) == 0  # no tokens: nothing is launched
+
+
+def test_slots_and_rope_arguments():
+    def slots(**kw):
+        a = _lib.PageSlotsArgs()
+        at = 1 << 20
+        names = [f for f, _ in _lib.PageSlotsArgs._fields_[4:]]
+        base = dict(B=2, pages_per_row=3, n_tokens=4, n_free=5, **{f: at + 4096 * i for i, f in enumerate(names)})
+        for name, x in {**base, **kw}.items():
+            setattr(a, name, x)
+        return a
+
+    for bad in (dict(B=0), dict(B=4097), dict(pages_per_row=0), dict(n_tokens=-1), dict(n_free=0), dict(n_free=1 << 26), dict(lens=None),
+                dict(table_out=None), dict(slots=None), dict(status=None), dict(lens_out=1 << 20), dict(pages_per_row=1 << 25)):
+        assert _call("fade_page_slots", slots(**bad), None) == _lib.FADE_EINVAL, bad
+
+    def rope(**kw):
+        a = _lib.RopeArgs()
+        for name, x in {**dict(B=1, S=4, D=64, Hq=2, Hkv=0, n_freqs=32, positions=1 << 20), **kw}.items():
+            setattr(a, name, x)
+        a.q.src = a.q.dst = 1 << 20
+        return a
+
+    for bad in (dict(dtype=3), dict(dtype=-1)):
+        assert _call("fade_rope_axes", rope(**bad), None) == _lib.FADE_EINVAL
+    for name, x in (("D", 63), ("D", 258), ("n_freqs", 33), ("n_freqs", -1), ("positions", None), ("B", -1), ("B", 1 << 31), ("Hkv", 1)):
+        a = rope()
+        setattr(a, name, x)
+        assert _call("fade_rope_axes", a, None) == _lib.FADE_EINVAL, name
+    a = rope()
+    assert _call("fade_paged_append", a, None) == _lib.FADE_EINVAL  # no slots
+    a.dtype = 2
+    assert _call("fade_paged_append", a, None) == _lib.FADE_EINVAL  # 16-bit pages
+    a = rope()
+    a.S = 0
+    assert _call("fade_rope_axes", a, None) == 0
+
+
+def test_work_is_cut_into_the_bound():
+    """The device's cut (find_item of paged_attn.hip), with its fp32 sums: the items stay inside
+    the workspace and the grid, and a row's splits cover its keys."""
+    rng = random.Random(0)
+    f = np.float32
+    for _ in range(300):
+        B, G, M = rng.choice((1, 2, 63, 64, 65, 200)), rng.choice((1, 4, 7, 20)), rng.choice((16, 64, 128, 256))
+        ppr = rng.choice((5, 100, 4000))
+        new = [rng.choice((0, 1, 1, rng.randint(0, 3000))) for _ in range(B)]
+        lens = [rng.randint(0, ppr * 64) if rng.random() < 0.7 else rng.randint(0, 90) for _ in range(B)]
+        T = sum(new) + rng.choice((0, 5))
+        target = rng.choice((3, 64, 129, 512))
+        tiles = [-(-n * G // M) for n in new]
+        bound = T * G // M + min(B, T) + target
+        work = f(0)
+        lanes = [f(0)] * 64
+        for b in range(B):
+            lanes[b % 64] = f(float(lanes[b % 64]) + float(f(tiles[b])) * float(f(lens[b])))
+        for x in lanes:
+            work = f(work + x)
+        work = f(work * f(f(1.00002) / f(target)))
+        chunk = max(256, -(-(int(work) + 1) // 64) * 64)
+        assert chunk * target >= sum(t * n for t, n in zip(tiles, lens))
+        splits = [max(1, -(-n // chunk)) for n in lens]
+        assert sum(t * s for t, s in zip(tiles, splits)) <= bound
+        assert all(s * chunk >= n > (s - 1) * chunk or s == 1 for n, s in zip(lens, splits))
+
+
+def _fractions(scheme):
+    turn, axis = scheme.turns()
+    return [int.from_bytes(turn[8 * i : 8 * i + 8], "little") for i in range(len(axis))], list(axis)
+
+
+def test_turns():
+    s = Vanilla(theta=1e6, head_dim=128)
+    turn, axis = _fractions(s)
+    assert axis == [0] * 64 and len(turn) == 64
+    for t, f in zip(turn, s.inv_freq().tolist()):
+        assert abs(Fraction(t, 2**64) - Fraction(f) / (2 * PI)) <= Fraction(1, 2**65)
+    lin = LinearScaled(theta=1e6, head_dim=128, factor=4.0)
+    assert all(abs(4 * a - b) <= 2 for a, b in zip(_fractions(lin)[0], turn))
+    assert NoRope(head_dim=64).turns() == (b"", b"")
+
+
+def test_axes_of_the_frequencies():
+    m = MRope(theta=1e6, head_dim=128, mrope_section=[16, 24, 24])
+    assert m.n_axes == 3 and m.freq_axes() == [0] * 16 + [1] * 24 + [2] * 24
+    m = MRope(theta=1e6, head_dim=128, mrope_section=[24, 20, 20], interleaved=True)
+    assert m.freq_axes() == [0, 1, 2] * 20 + [0] * 4
+    assert MRope(theta=1e6, head_dim=128).freq_axes() == [0] * 64 and MRope(theta=1e6, head_dim=128).n_axes == 1
+    for bad in (MRope(theta=1e6, head_dim=128, mrope_section=[16, 24, 23]), MRope(theta=1e6, head_dim=128, mrope_section=[16, 24, 24], interleaved=True)):
+        with pytest.raises(ValueError, match="share out"):
+            bad.turns()
+
+    class Cfg:
+        head_dim, rope_theta, rope_parameters = 256, 1e7, {"mrope_section": [11, 11, 10], "mrope_interleaved": True, "partial_rotary_factor": 0.25}
+
+    s = extract_rope_scheme(Cfg())
+    assert isinstance(s, MRope) and s.interleaved and s.n_axes == 3 and len(s.freq_axes()) == 32
+    Cfg.rope_parameters = {"mrope_section": [16, 24, 24]}
+    assert not extract_rope_scheme(Cfg(), head_dim=128).interleaved
+
+
+def test_pool():
+    pool = TokenPagePool(5, 2, 16, torch.bfloat16, "cpu")
+    assert pool.k.shape == (6, 2, 64, 16) and pool.free.tolist() == [1, 2, 3, 4, 5] and pool.ring.tolist() == [0, 5]
+    st = pool.start(3, 4)
+    assert st.table.shape == (3, 4) and st.lens.tolist() == [0, 0, 0] and st.starts.tolist() == [0, 0, 0, 0]
+    pool.k.copy_(torch.randn(pool.k.shape))
+    k, v = pool.gather(torch.tensor([[1, 4], [2, 0]], dtype=torch.int32), 70)
+    assert k.shape == (2, 2, 70, 16) and torch.equal(k[0, :, 64:], pool.k[4, :, :6]) and not v.any()
+    with pytest.raises(ValueError, match="exceeds"):
+        pool.gather(torch.zeros(1, 1, dtype=torch.int32), 65)
+    for bad in ((0, 1, 16), (1, 0, 16), (1, 1, 12), (1, 1, 264)):
+        with pytest.raises(ValueError):
+            TokenPagePool(*bad, device="cpu")
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        TokenPagePool(1, 1, 16, torch.float32, "cpu")
