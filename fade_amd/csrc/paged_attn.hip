@@ -30,7 +30,12 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -41,11 +46,14 @@ typedef __attribute__((address_space(4))) int32_t const_i32;
 constexpr int kThreads = 256;
 constexpr int kPage = 64;
 constexpr int kRows = 16;  // matrix rows of an item of the few-row kernel
+constexpr float kNegBig = -1.0e30f;
 
 template <int V>
 struct Int {
   static constexpr int value = V;
 };
+
+enum { kAll = 0, kFew = 1, kMany = 2 };
 
 struct Params {
   int64_t B, T, ppr, n_pages;
@@ -65,6 +73,7 @@ struct Params {
   int target;      // items per kv head the splits aim at; 0: no splits
   float per_item;  // a little over 1 / target
   uint32_t items;  // bound of the items per kv head
+  int rows_of;     // kAll, or the rows of the batch whose matrix rows fit one tile of 16 (kFew) or do not (kMany)
   int least;       // fewest keys of a split (a multiple of 64)
   float* part_o;   // [item][kv head][M][D]
   float2* part_ml; // [item][kv head][M]: maximum (log2 units), sum
@@ -127,7 +136,9 @@ __device__ __forceinline__ bool find_item(const Params& p, uint32_t idx, Item& i
   const int B = static_cast<int>(p.B);
   int q0 = 0, n = 0, len = 0;
   auto tiles_of = [&](int new_tokens) {
-    return (static_cast<uint32_t>(new_tokens) * static_cast<uint32_t>(p.G) + static_cast<uint32_t>(M - 1)) / static_cast<uint32_t>(M);
+    const uint32_t rows = static_cast<uint32_t>(new_tokens) * static_cast<uint32_t>(p.G);
+    if (p.rows_of != kAll && (rows <= kRows) != (p.rows_of == kFew)) return 0u;
+    return (rows + static_cast<uint32_t>(M - 1)) / static_cast<uint32_t>(M);
   };
   uint32_t chunk = INT32_MAX;
   if (p.target > 0) {
@@ -199,7 +210,7 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (BF) return pack_bf16(a, b);
-  else return static_cast<uint32_t>(f2h(a)) | (static_cast<uint32_t>(f2h(b)) << 16);
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
 }
 
 // ---- few rows: tiles of 16 matrix rows, every wave with keys of its own ----
@@ -422,6 +433,278 @@ __global__ __launch_bounds__(64 * Few<DP>::kWaves) void paged_few_kernel(Params 
   }
 }
 
+// ---- many rows: tiles of 32 NW MT matrix rows, the keys shared through LDS ----
+//
+// NW waves of MT blocks of 32 matrix rows each walk the item's keys page by page.
+// A page's K and V go straight to LDS, two pages deep, every wave loading its
+// share; one barrier per page.
+//   S^T = K Q^T   32x32x16 MFMAs, A = 32 keys x 16 channels, B = Q^T (registers):
+//                 lane (n, h) holds matrix row n, register i key 8 (i / 4) + 4 h + i % 4
+//   O^T += V^T P^T  A = V^T by transposing LDS reads, B = P^T straight from S^T's
+//                 registers: k slot (h, j) of step s is key 16 s + 4 h + j (j < 4),
+//                 16 s + 8 + 4 h + j - 4
+// so a row's maximum, sum and rescaling are lane-local.  The running maximum moves
+// only where a probability passes 2^8 (found on the 16-bit probabilities, two per
+// operation; the exact maximum is taken there alone), so most pages need neither a
+// maximum of the scores nor an exchange between lanes nor a rescaling.  P is
+// rounded to 16 bits (as the output is; the sum takes the same rounded values): a
+// second product for its rest would cost half the matrix work again.
+// LDS rows are DP channels, 16-byte units exchanged so that the eight (16) rows
+// that a read of K touches and the four that a transposing read of V touches lie
+// in different banks.
+template <int DP>
+__device__ __forceinline__ int wide_k_unit(int row, int u) {
+  if constexpr (DP == 64) return u ^ ((row >> 1) & 7);
+  else return u ^ (row & 15);
+}
+template <int DP>
+__device__ __forceinline__ int wide_v_unit(int row, int u) {
+  if constexpr (DP == 64) return u ^ (4 * ((row >> 1) & 1));
+  else return u ^ (4 * (row & 3));
+}
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <int DP, int NW, int MT, bool BF>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void paged_wide_kernel(Params p) {
+  constexpr int M = 32 * NW * MT;
+  constexpr int NKS = DP / 16, NCB = DP / 32, UNITS = DP / 8;
+  constexpr int TENSOR = kPage * DP * 2, STAGE = 2 * TENSOR;
+  constexpr int LPW = TENSOR / 1024 / NW;  // direct loads of K, and of V, per wave and page
+  static_assert(TENSOR % (1024 * NW) == 0, "a page is shared out evenly");
+  const int kvh = blockIdx.x % p.Hkv;
+  const uint32_t idx = blockIdx.x / static_cast<uint32_t>(p.Hkv);
+  const int lane = threadIdx.x & 63, n32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (p.zero_tail) zero_tail(p, idx, gridDim.x / p.Hkv, kvh);
+  Item it;
+  if (!find_item<M, false>(p, idx, it)) return;
+  const int D = p.D;
+  const int all = it.n * p.G;  // the row's matrix rows
+  auto limit = [&](int i) {
+    const int x = p.causal ? it.len - it.n + i + 1 : it.len;
+    return x < 0 ? 0 : x;
+  };
+  const int last = it.tile * M + M < all ? it.tile * M + M : all;  // past the item's last matrix row
+  const int hi = limit((last - 1) / p.G);
+  const int k0 = __builtin_amdgcn_readfirstlane(it.split * it.chunk);
+  const int k1 = __builtin_amdgcn_readfirstlane(it.splits > 1 && k0 + it.chunk < hi ? k0 + it.chunk : hi);
+  // this wave's matrix rows, and the fewest and the most keys they see
+  const int r0 = it.tile * M + 32 * MT * wave;
+  const bool active = r0 < all;
+  const int rl = r0 + 32 * MT < all ? r0 + 32 * MT : all;
+  const int wlo = __builtin_amdgcn_readfirstlane(active ? limit(r0 / p.G) : 0);
+  const int whi = __builtin_amdgcn_readfirstlane(active ? limit((rl - 1) / p.G) : 0);
+  int lim[MT];
+
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+  const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds)));
+  if (D < DP) {  // units past the head_dim are never loaded: zeros
+    for (int i = 16 * threadIdx.x; i < 2 * STAGE; i += 1024 * NW) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+  }
+  // this lane's places of a page: load i fills unit 64 (LPW wave + i) + lane
+  uint32_t ko[LPW], vo[LPW];
+  bool kin[LPW], vin[LPW];
+#pragma unroll
+  for (int i = 0; i < LPW; ++i) {
+    const int pos = 64 * (LPW * wave + i) + lane, row = pos / UNITS, u = pos % UNITS;
+    const int ku = wide_k_unit<DP>(row, u), vu = wide_v_unit<DP>(row, u);
+    kin[i] = DP == D || 8 * ku < D;
+    vin[i] = DP == D || 8 * vu < D;
+    ko[i] = static_cast<uint32_t>(2 * (row * D + 8 * ku));
+    vo[i] = static_cast<uint32_t>(2 * (row * D + 8 * vu));
+  }
+  const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + it.b * p.ppr);
+  auto issue = [&](int id, int buf) {
+    id = id < 0 || id >= p.n_pages ? 0 : id;
+    const int64_t at = (static_cast<int64_t>(id) * p.Hkv + kvh) * kPage * D;
+    const uint32_t to = base + buf * STAGE + 1024 * LPW * wave;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      if (kin[i]) lds_dma16(p.kp + at, ko[i], to + 1024 * i);
+      if (vin[i]) lds_dma16(p.vp + at, vo[i], to + TENSOR + 1024 * i);
+    }
+  };
+  const int t0 = k0 / kPage, t1 = (k1 + kPage - 1) / kPage;
+  int next = 0;
+  if (t0 < t1) {
+    issue(__builtin_amdgcn_readfirstlane(trow[t0]), 0);
+    if (t0 + 1 < t1) next = __builtin_amdgcn_readfirstlane(trow[t0 + 1]);
+  }
+  u32x4 qf[MT][NKS];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = r0 + 32 * mt + n32;
+    const bool live = r < all;
+    const int qi = live ? r / p.G : 0;
+    lim[mt] = live ? limit(qi) : 0;
+    const uint16_t* qr = p.q + static_cast<int64_t>(it.q0 + qi) * p.q_st + static_cast<int64_t>(kvh * p.G + (live ? r - qi * p.G : 0)) * p.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) {
+      const int c = 16 * ks + 8 * h;
+      qf[mt][ks] = live && c < D ? *reinterpret_cast<const u32x4*>(qr + c) : u32x4{0, 0, 0, 0};
+    }
+  }
+  f32x16 acc[MT][NCB];
+  float m[MT], l[MT];  // of row n32: the running maximum (raw scores), the sum over this half's keys
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = kNegBig;
+    l[mt] = 0.0f;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[mt][cb][i] = 0.0f;
+  }
+  const float sl2 = p.scale_log2;
+
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wave's share of page t
+    __syncthreads();                           // everyone's; and page t - 1 is done with
+    uint8_t* const kt = lds + buf * STAGE;
+    uint8_t* const vt = kt + TENSOR;
+    const int key = t * kPage, cnt = it.len - key;
+    if (cnt < kPage) {  // rows that hold no token: whatever stands there must not count
+      for (int i = threadIdx.x; i < (kPage - cnt) * UNITS; i += 64 * NW) *reinterpret_cast<u32x4*>(vt + 16 * (cnt * UNITS + i)) = u32x4{0, 0, 0, 0};
+      __syncthreads();
+    }
+    if (t + 1 < t1) {
+      issue(next, buf ^ 1);
+      if (t + 2 < t1) next = __builtin_amdgcn_readfirstlane(trow[t + 2]);
+    }
+    if (key >= whi) continue;
+    f32x16 s[MT][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[mt][kb][i] = 0.0f;
+      const int row = 32 * kb + n32;
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * DP * 2 + 16 * wide_k_unit<DP>(row, 2 * ks + h));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][kb] = mfma32<BF>(a, qf[mt][ks], s[mt][kb]);
+      }
+    }
+    u32x4 pa[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if (key + kPage > wlo) {
+        const int left = lim[mt] - key;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * kb + 8 * (i >> 2) + 4 * h + (i & 3) >= left) s[mt][kb][i] = -INFINITY;
+      }
+      auto probs = [&]() {
+        const float nm = -m[mt] * sl2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            pa[mt][k][j] = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[mt][k >> 1][8 * (k & 1) + 2 * j], sl2, nm)),
+                                     __builtin_amdgcn_exp2f(fmaf(s[mt][k >> 1][8 * (k & 1) + 2 * j + 1], sl2, nm)));
+      };
+      probs();
+      // 16-bit patterns of the non-negative probabilities order as their values do
+      const u16x8 pm = __builtin_elementwise_max(
+          __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][0]), __builtin_bit_cast(u16x8, pa[mt][1])),
+          __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][2]), __builtin_bit_cast(u16x8, pa[mt][3])));
+      const auto p2 = __builtin_elementwise_max(__builtin_elementwise_max(pm.s01, pm.s23), __builtin_elementwise_max(pm.s45, pm.s67));
+      constexpr uint16_t kOver = BF ? 0x4380 : 0x5C00;  // 2^8
+      if (__builtin_amdgcn_ballot_w64(p2.x > kOver || p2.y > kOver) != 0) {
+        float mx = kNegBig;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[mt][kb][i], s[mt][kb][i + 1]));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mn = fmaxf(m[mt], mx);
+        const float alpha = __builtin_amdgcn_exp2f((m[mt] - mn) * sl2);
+        m[mt] = mn;
+        l[mt] *= alpha;
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[mt][cb][i] *= alpha;
+        probs();
+      }
+      float ps = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = pa[mt][k][j];  // (a bit cast of a vector's element itself takes element 0)
+          if constexpr (BF)
+            ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), (bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}), ps, false);
+          else
+            ps = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), (f16x2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}), ps, false);
+        }
+      l[mt] += ps;
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        // lane points at key 16 ks + 4 h + (l16 >> 2) (+ 8), channels 32 cb + 16 ((lane >> 4) & 1) + 4 (l16 & 3)
+        const int row = 16 * ks + 4 * h + ((lane & 15) >> 2), u = 4 * cb + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+        const uint8_t* at = vt + row * DP * 2 + 16 * wide_v_unit<DP>(row, u) + 8 * (lane & 1);
+        const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at)));
+        const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at + 8 * DP * 2)));  // (row + 8: the same exchange)
+        const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+        const u32x4 a = {w0.x, w0.y, w1.x, w1.y};
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt][cb] = mfma32<BF>(a, pa[mt][ks], acc[mt][cb]);
+      }
+    }
+  }
+
+  // ---- lane (n, h): row n, channels 32 cb + 8 q + 4 h .. + 3 ----
+  const bool part = it.splits > 1;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const float lt = l[mt] + __shfl_xor(l[mt], 32, 64);
+    const int r = r0 + 32 * mt + n32;
+    if (r >= all) continue;
+    if (part) {
+      const int64_t pr = static_cast<int64_t>(blockIdx.x) * M + 32 * (MT * wave + mt) + n32;
+      if (h == 0) p.part_ml[pr] = make_float2(m[mt] * sl2, lt);
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = 32 * cb + 8 * q + 4 * h;
+          if (c < D) *reinterpret_cast<f32x4*>(p.part_o + pr * D + c) = f32x4{acc[mt][cb][4 * q], acc[mt][cb][4 * q + 1], acc[mt][cb][4 * q + 2], acc[mt][cb][4 * q + 3]};
+        }
+    } else {
+      const int qi = r / p.G;
+      const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;  // no visible key: zeros
+      uint16_t* dst = p.out + static_cast<int64_t>(it.q0 + qi) * p.o_st + static_cast<int64_t>(kvh * p.G + r - qi * p.G) * p.o_sh;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = 32 * cb + 8 * q + 4 * h;
+          u32x2 w;
+          w.x = pack2<BF>(acc[mt][cb][4 * q] * inv, acc[mt][cb][4 * q + 1] * inv);
+          w.y = pack2<BF>(acc[mt][cb][4 * q + 2] * inv, acc[mt][cb][4 * q + 3] * inv);
+          if (c < D) *reinterpret_cast<u32x2*>(dst + c) = w;
+        }
+    }
+  }
+}
+
 // The splits of a tile's rows joined in split order: D / 4 threads per row.
 template <int M, bool BF>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(Params p) {
@@ -458,13 +741,32 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(Params p) {
 
 bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
 
-// How a call is cut, from the sizes the host knows.
+// How one kernel's work of a call is cut, from the sizes the host knows.
 struct Plan {
-  int M;
-  int64_t tiles, items;  // bounds: tiles of rows, items (per kv head)
+  int M = 0;              // matrix rows of a tile; 0: not launched
+  int rows_of = kAll;
+  int target = 0, least = 0;
+  int64_t tiles = 0, items = 0;  // bounds: tiles of rows, items (per kv head)
+};
+struct Plans {
+  Plan few, wide;
 };
 
-int plan_of(const fade_paged_attn_args* a, Params& p, Plan& pl) {
+template <int DP>
+struct Wide {  // waves and blocks of 32 rows per wave
+  static constexpr int NW = DP > 128 ? 4 : 8, MT = 1, M = 32 * NW * MT;
+};
+int wide_rows(int D) { return D > 128 ? Wide<256>::M : Wide<128>::M; }
+
+void bound_items(const Params& p, Plan& pl, int64_t tiles, int64_t pieces, int least) {
+  pl.tiles = tiles;
+  pl.target = static_cast<int>(cdiv(pieces, p.Hkv));
+  pl.least = least;
+  if (p.ppr * kPage <= least) pl.target = 0;
+  pl.items = pl.tiles + pl.target;
+}
+
+int plan_of(const fade_paged_attn_args* a, Params& p, Plans& pl) {
   const char* what = "fade_paged_attn";
   if (a == nullptr) return einval("%s: null args", what);
   if (a->D < 8 || a->D > 256 || a->D % 8)
@@ -508,35 +810,72 @@ int plan_of(const fade_paged_attn_args* a, Params& p, Plan& pl) {
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   p.causal = a->mask_mode == FADE_MASK_BOTTOM_RIGHT;
   p.zero_tail = a->zero_tail;
-  pl.M = kRows;
-  // sum_b ceil(n_b G / M) <= T G / M + (rows with new tokens)
-  pl.tiles = p.T * p.G / pl.M + (p.B < p.T ? p.B : p.T);
-  // two workgroups' worth of work per CU, in pieces of 256 keys or more
-  p.target = static_cast<int>(cdiv(2 * num_cus(), p.Hkv));
-  p.least = 256;
-  if (p.ppr * kPage <= p.least) p.target = 0;
-  p.per_item = p.target > 0 ? 1.00002f / static_cast<float>(p.target) : 0.0f;
-  pl.items = pl.tiles + p.target;
-  if (pl.items * p.Hkv >= (1ll << 24)) return einval("%s: shape too large (%lld items of work)", what, (long long)(pl.items * p.Hkv));
-  p.items = static_cast<uint32_t>(pl.items);
+  // Rows whose matrix rows fit one tile of 16 go to the few-row kernel, the others
+  // to the wide one; a call of at most 16 matrix rows per row on average is taken to
+  // be a decoding step, all of it the few-row kernel's.
+  const int64_t rows = p.T * p.G, live = p.B < p.T ? p.B : p.T;
+  const bool step = rows <= kRows * p.B;
+  pl.few.M = kRows;
+  pl.few.rows_of = step ? kAll : kFew;
+  // sum_b ceil(n_b G / M) <= T G / M + (rows with new tokens); two workgroups' worth of work per CU, in pieces of 256 keys or more
+  bound_items(p, pl.few, step ? rows / kRows + live : live, 2 * num_cus(), 256);
+  if (!step) {
+    pl.wide.M = wide_rows(p.D);
+    pl.wide.rows_of = kMany;
+    const int64_t tiles = rows / pl.wide.M + live;
+    // no splits where whole tiles fill the chip several times over
+    bound_items(p, pl.wide, tiles, rows / pl.wide.M * p.Hkv >= 8 * num_cus() ? 0 : 2 * num_cus(), 512);
+  }
+  for (const Plan* k : {&pl.few, &pl.wide})
+    if (k->items * p.Hkv >= (1ll << 24)) return einval("%s: shape too large (%lld items of work)", what, (long long)(k->items * p.Hkv));
   return FADE_OK;
 }
 
-int64_t part_rows(const Params& p, const Plan& pl) { return p.target == 0 ? 0 : pl.items * p.Hkv * pl.M; }
-int64_t part_bytes(const Params& p, const Plan& pl) { return part_rows(p, pl) * (p.D * 4 + static_cast<int64_t>(sizeof(float2))); }
+int64_t part_rows(const Params& p, const Plan& pl) { return pl.target == 0 ? 0 : pl.items * p.Hkv * pl.M; }
+// (the kernels run one after the other: their sums lie in the same memory)
+int64_t part_rows(const Params& p, const Plans& pl) {
+  const int64_t a = part_rows(p, pl.few), b = part_rows(p, pl.wide);
+  return a > b ? a : b;
+}
+int64_t part_bytes(const Params& p, const Plans& pl) { return part_rows(p, pl) * (p.D * 4 + static_cast<int64_t>(sizeof(float2))); }
+
+void apply(Params& p, const Plan& pl) {
+  p.rows_of = pl.rows_of;
+  p.target = pl.target;
+  p.least = pl.least;
+  p.per_item = pl.target > 0 ? 1.00002f / static_cast<float>(pl.target) : 0.0f;
+  p.items = static_cast<uint32_t>(pl.items);
+}
+
+template <int M, bool BF>
+int merge(const Params& p, const Plan& pl, hipStream_t st) {
+  if (pl.target == 0) return FADE_OK;
+  const dim3 grid(static_cast<unsigned>(p.Hkv * pl.tiles), static_cast<unsigned>(cdiv(M, kThreads / (p.D / 4))));
+  hipLaunchKernelGGL((paged_merge_kernel<M, BF>), grid, dim3(kThreads), 0, st, p);
+  return check_launch("fade_paged_attn (merge)");
+}
+
+template <int DP, bool BF>
+int launch(Params& p, const Plans& pl, hipStream_t st) {
+  apply(p, pl.few);
+  hipLaunchKernelGGL((paged_few_kernel<DP, BF>), dim3(static_cast<unsigned>(p.Hkv * pl.few.items)), dim3(64 * Few<DP>::kWaves), 0, st, p);
+  int rc = check_launch("fade_paged_attn");
+  if (!rc) rc = merge<kRows, BF>(p, pl.few, st);
+  if (rc || pl.wide.M == 0) return rc;
+  typedef Wide<DP> W;
+  apply(p, pl.wide);
+  p.zero_tail = 0;
+  hipLaunchKernelGGL((paged_wide_kernel<DP, W::NW, W::MT, BF>), dim3(static_cast<unsigned>(p.Hkv * pl.wide.items)), dim3(64 * W::NW), 0, st, p);
+  rc = check_launch("fade_paged_attn");
+  return rc ? rc : merge<W::M, BF>(p, pl.wide, st);
+}
 
 template <bool BF>
-int launch(Params& p, const Plan& pl, void* stream) {
+int launch_any(Params& p, const Plans& pl, void* stream) {
   hipStream_t st = as_stream(stream);
-  const dim3 grid(static_cast<unsigned>(p.Hkv * pl.items));
-  if (p.D <= 64) hipLaunchKernelGGL((paged_few_kernel<64, BF>), grid, dim3(64 * Few<64>::kWaves), 0, st, p);
-  else if (p.D <= 128) hipLaunchKernelGGL((paged_few_kernel<128, BF>), grid, dim3(64 * Few<128>::kWaves), 0, st, p);
-  else hipLaunchKernelGGL((paged_few_kernel<256, BF>), grid, dim3(64 * Few<256>::kWaves), 0, st, p);
-  const int rc = check_launch("fade_paged_attn");
-  if (rc || p.target == 0) return rc;
-  const dim3 mgrid(static_cast<unsigned>(p.Hkv * pl.tiles), static_cast<unsigned>(cdiv(kRows, kThreads / (p.D / 4))));
-  hipLaunchKernelGGL((paged_merge_kernel<kRows, BF>), mgrid, dim3(kThreads), 0, st, p);
-  return check_launch("fade_paged_attn (merge)");
+  if (p.D <= 64) return launch<64, BF>(p, pl, st);
+  if (p.D <= 128) return launch<128, BF>(p, pl, st);
+  return launch<256, BF>(p, pl, st);
 }
 
 }  // namespace
@@ -549,7 +888,7 @@ using namespace fade::paged;
 FADE_API int fade_paged_attn_workspace_bytes(const fade_paged_attn_args* a, int64_t* bytes) {
   if (bytes == nullptr) return einval("fade_paged_attn_workspace_bytes: null output");
   Params p;
-  Plan pl;
+  Plans pl;
   const int rc = plan_of(a, p, pl);
   if (rc) return rc;
   *bytes = part_bytes(p, pl);
@@ -558,7 +897,7 @@ FADE_API int fade_paged_attn_workspace_bytes(const fade_paged_attn_args* a, int6
 
 FADE_API int fade_paged_attn(const fade_paged_attn_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
   Params p;
-  Plan pl;
+  Plans pl;
   const int rc = plan_of(a, p, pl);
   if (rc) return rc;
   if (p.T == 0) return FADE_OK;
@@ -569,5 +908,5 @@ FADE_API int fade_paged_attn(const fade_paged_attn_args* a, void* workspace, int
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + part_rows(p, pl) * p.D);
   }
-  return a->dtype == FADE_DTYPE_BF16 ? launch<true>(p, pl, stream) : launch<false>(p, pl, stream);
+  return a->dtype == FADE_DTYPE_BF16 ? launch_any<true>(p, pl, stream) : launch_any<false>(p, pl, stream);
 }
