@@ -12,13 +12,15 @@
 // rows of (row b, kv head): row r is query r / G, head r % G, so any G and any
 // chunk length fill the same tiles and each key is read once per tile of rows.
 //
-// Work is cut on the device, from the lengths the host does not know: an item is
-// (row b, tile of M matrix rows, split of the keys), and a split holds
-// C = max(kLeast, ceil(sum_b tiles_b L_b / target)) keys, so that the items are about
-// `target` equal pieces whatever the rows' lengths are.  Every wave finds its own
-// item by a sum over the rows' counts (one load per lane for 64 rows).  A row that
-// is one split writes its output; the others' unnormalized fp32 sums are joined in
-// split order by a second launch, so results do not depend on timing.
+// Work is cut on the device, from the lengths the host does not know.  A tile is M
+// matrix rows of a (row b, kv head); its cost is the keys that it reads and a
+// constant for its start and end.  The tiles of all rows lie one after the other on
+// a line, and every workgroup of a kv head takes an equal piece of it, whatever the
+// rows' lengths are: the end of one tile, whole tiles, the beginning of another.  A
+// wave finds its place by a sum over the rows' costs (one load per lane for 64
+// rows).  Whole tiles are written out; a tile cut by a piece's border leaves
+// unnormalized fp32 sums, at most two per workgroup, which a second launch joins in
+// the order of the keys, so results do not depend on timing.
 #include <math.h>
 
 #include "fade_common.h"
@@ -70,22 +72,30 @@ struct Params {
   float scale_log2;
   int causal;
   int zero_tail;
-  int target;      // items per kv head the splits aim at; 0: no splits
-  float per_item;  // a little over 1 / target
-  uint32_t items;  // bound of the items per kv head
+  // the cut of one kernel's work
   int rows_of;     // kAll, or the rows of the batch whose matrix rows fit one tile of 16 (kFew) or do not (kMany)
-  int least;       // fewest keys of a split (a multiple of 64)
-  float* part_o;   // [item][kv head][M][D]
-  float2* part_ml; // [item][kv head][M]: maximum (log2 units), sum
+  int lm;          // log2 of the matrix rows of a tile
+  int per_tile;    // queries that a tile touches at most
+  int start_cost;  // of a tile, in keys
+  int pieces;      // workgroups per kv head
+  float per_piece; // a little over 1 / pieces
+  int least;       // fewest keys of a piece
+  float* part_o;   // [workgroup][2][M][D]: a tile's end (0), a tile's beginning (1)
+  float2* part_ml; // [workgroup][2][M]: maximum (log2 units), sum
+  int4* cuts;      // [workgroup]: the tile that begins in its piece and ends in another: first new token, its
+                   // first matrix row, matrix rows of the row, parts (0: none)
 };
 
-// What a wave works on (wave-uniform).
-struct Item {
-  int b, q0, n, len;    // row, its first new token, new tokens, tokens
-  int tile, split;      // tile of matrix rows, split of the keys
-  int tiles, splits;    // the row's
-  int chunk;            // keys per split
-  uint32_t first;       // the row's first item
+// A piece of a tile (wave-uniform): keys' pages or 32-key steps from `from` on, in keys.
+struct Tile {
+  int b, q0, n, len;   // row, its first new token, new tokens, tokens
+  int tile;            // of the row's tiles
+  uint64_t at, cost;   // its place on the line
+};
+// Where the search of the next tile starts: rows b0 .., their place on the line.
+struct Place {
+  int b0;
+  uint64_t before;
 };
 
 // A row's new tokens and length from device data, kept inside the tensors.
@@ -100,94 +110,146 @@ __device__ __forceinline__ void row_counts(const Params& p, int b, int& q0, int&
   n = e - s;
   len = l < 0 ? 0 : (l > cap ? cap : l);
 }
+__device__ __forceinline__ uint32_t tiles_of(const Params& p, int n) {
+  const uint32_t rows = static_cast<uint32_t>(n) * static_cast<uint32_t>(p.G);
+  if (p.rows_of != kAll && (rows <= kRows) != (p.rows_of == kFew)) return 0u;
+  return (rows + (1u << p.lm) - 1u) >> p.lm;
+}
+// Cost of a row's first t tiles: tile i reads at most base + step (i + 1) keys.
+__device__ __forceinline__ uint64_t cost_of(const Params& p, int n, int len, uint64_t t) {
+  const uint64_t step = p.causal ? p.per_tile : 0;
+  const int base = p.causal ? (len > n ? len - n : 0) : len;
+  return t * static_cast<uint64_t>(base + p.start_cost) + step * (t * (t + 1) / 2);
+}
 
 // Inclusive sums over the wave's lanes: shifts within rows of 16 lanes, then each
 // row's last lane to the next row (DPP: no LDS round trips).
-template <typename T, typename F>
-__device__ __forceinline__ T wave_scan(T v, F add) {
-  auto step = [&](auto ctrl, auto mask) {
-    const int x = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(mask)::value, 0xF, true);
-    v = add(v, __builtin_bit_cast(T, x));
-  };
-  step(Int<0x111>{}, Int<0xF>{});  // row_shr 1, 2, 4, 8
-  step(Int<0x112>{}, Int<0xF>{});
-  step(Int<0x114>{}, Int<0xF>{});
-  step(Int<0x118>{}, Int<0xF>{});
-  step(Int<0x142>{}, Int<0xA>{});  // row_bcast 15 to rows 1 and 3
-  step(Int<0x143>{}, Int<0xC>{});  // row_bcast 31 to rows 2 and 3
-  return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t scan_step(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, true);
+  return v + ((static_cast<uint64_t>(hi) << 32) | lo);
 }
-__device__ __forceinline__ uint32_t scan_u32(uint32_t v) {
-  return wave_scan(v, [](uint32_t a, uint32_t b) { return a + b; });
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  v = scan_step<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);  // row_bcast 15 to rows 1 and 3
+  return scan_step<0x143, 0xC>(v);  // row_bcast 31 to rows 2 and 3
 }
-__device__ __forceinline__ float sum_f32(float v) {
-  const float x = wave_scan(v, [](float a, float b) { return __fadd_rn(a, b); });
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), l), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
 }
-__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) {
-  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
+__device__ __forceinline__ uint64_t uniform(uint64_t v) { return lane_of(v, 0); }
+
+// A lane's row of the 64 that a wave looks at.
+struct Row {
+  int q0, n, len;
+  uint64_t cost;
+};
+__device__ __forceinline__ Row row_of(const Params& p, int b) {
+  Row r{0, 0, 0, 0};
+  if (b < p.B) {
+    row_counts(p, b, r.q0, r.n, r.len);
+    r.cost = cost_of(p, r.n, r.len, tiles_of(p, r.n));
+  }
+  return r;
 }
 
-// Item `idx` (BY_TILE: the idx-th tile of rows, all its splits) of a kernel of M
-// matrix rows; false past the last one.  All lanes of the wave call it.
-template <int M, bool BY_TILE>
-__device__ __forceinline__ bool find_item(const Params& p, uint32_t idx, Item& it) {
-  const int lane = threadIdx.x & 63;
-  const int B = static_cast<int>(p.B);
-  int q0 = 0, n = 0, len = 0;
-  auto tiles_of = [&](int new_tokens) {
-    const uint32_t rows = static_cast<uint32_t>(new_tokens) * static_cast<uint32_t>(p.G);
-    if (p.rows_of != kAll && (rows <= kRows) != (p.rows_of == kFew)) return 0u;
-    return (rows + static_cast<uint32_t>(M - 1)) / static_cast<uint32_t>(M);
-  };
-  uint32_t chunk = INT32_MAX;
-  if (p.target > 0) {
-    // (every wave of both launches does the same operations in the same order; the
-    // factor keeps chunk * target at or above the work despite the roundings)
-    float work = 0.0f;
-    for (int b = lane; b < B; b += 64) {
-      row_counts(p, b, q0, n, len);
-      work = __fmaf_rn(static_cast<float>(tiles_of(n)), static_cast<float>(len), work);
-    }
-    work = __fmul_rn(sum_f32(work), p.per_item);
-    const uint32_t c = work < 1.0e9f ? static_cast<uint32_t>(work) + 1u : 1000000000u;
-    chunk = (c + (kPage - 1)) / kPage * kPage;
-    if (chunk < static_cast<uint32_t>(p.least)) chunk = static_cast<uint32_t>(p.least);
-    chunk = __builtin_amdgcn_readfirstlane(chunk);
-  }
-  uint32_t items = 0, tiles_before = 0;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int b = b0 + lane;
-    uint32_t tiles = 0, splits = 1;
-    if (b < B) {
-      if (B > 64 || p.target == 0) row_counts(p, b, q0, n, len);
-      tiles = tiles_of(n);
-      if (static_cast<uint32_t>(len) > chunk) splits = (static_cast<uint32_t>(len) + chunk - 1) / chunk;
-    }
-    const uint32_t cnt = tiles * splits;
-    const uint32_t to_items = items + scan_u32(cnt), to_tiles = tiles_before + scan_u32(tiles);
-    const bool mine = BY_TILE ? (idx < to_tiles && idx >= to_tiles - tiles) : (idx < to_items && idx >= to_items - cnt);
-    const uint64_t who = __builtin_amdgcn_ballot_w64(mine);
+// Length of the line, and of a piece of it; `first`: the lane's row of rows 0 .. 63.
+// All lanes of the wave call it.
+__device__ __forceinline__ void line_of(const Params& p, uint64_t& all, uint64_t& piece, Row& first) {
+  const int B = static_cast<int>(p.B), lane = threadIdx.x & 63;
+  first = row_of(p, lane);
+  uint64_t work = first.cost;
+  for (int b = lane + 64; b < B; b += 64) work += row_of(p, b).cost;
+  all = lane_of(wave_scan(work), 63);
+  // (the factor keeps piece * pieces at or above the line's length despite the roundings)
+  piece = uniform(static_cast<uint64_t>(static_cast<float>(all) * p.per_piece) + 1);
+  if (piece < static_cast<uint64_t>(p.least)) piece = p.least;
+}
+
+// The tile at place x of the line, at or after `from`'s rows; false past the end.
+__device__ __forceinline__ bool find_tile(const Params& p, uint64_t x, const Row& first, Place& from, Tile& w) {
+  const int lane = threadIdx.x & 63, B = static_cast<int>(p.B);
+  for (int b0 = from.b0; b0 < B; b0 += 64) {
+    const Row r = b0 == 0 ? first : row_of(p, b0 + lane);
+    const uint64_t to = from.before + wave_scan(r.cost);
+    const uint64_t who = __builtin_amdgcn_ballot_w64(x < to && x >= to - r.cost);
     if (who != 0) {
       const int l = __builtin_ctzll(who);
-      it.b = b0 + l;
-      it.q0 = __builtin_amdgcn_readlane(q0, l);
-      it.n = __builtin_amdgcn_readlane(n, l);
-      it.len = __builtin_amdgcn_readlane(len, l);
-      it.tiles = static_cast<int>(lane_of(tiles, l));
-      it.splits = static_cast<int>(lane_of(splits, l));
-      it.first = lane_of(to_items - cnt, l);
-      it.chunk = static_cast<int>(chunk);
-      const uint32_t rem = idx - (BY_TILE ? lane_of(to_tiles - tiles, l) : it.first);
-      const uint32_t t = BY_TILE ? rem : rem / static_cast<uint32_t>(it.splits);
-      it.tile = it.tiles - 1 - static_cast<int>(t);  // the last rows first: they see the most keys
-      it.split = BY_TILE ? 0 : static_cast<int>(rem - t * static_cast<uint32_t>(it.splits));
+      w.b = b0 + l;
+      w.q0 = __builtin_amdgcn_readlane(r.q0, l);
+      w.n = __builtin_amdgcn_readlane(r.n, l);
+      w.len = __builtin_amdgcn_readlane(r.len, l);
+      const uint64_t row_at = lane_of(to - r.cost, l), off = x - row_at;
+      const int tiles = __builtin_amdgcn_readfirstlane(static_cast<int>(tiles_of(p, w.n)));
+      if (tiles == 1) {
+        w.tile = 0;
+        w.at = row_at;
+        w.cost = lane_of(r.cost, l);
+        return true;
+      }
+      // the tile: cost_of(tile) <= off < cost_of(tile + 1), by its real solution and a step to either side
+      const double step = p.causal ? p.per_tile : 0;
+      const double a = (p.causal ? (w.len > w.n ? w.len - w.n : 0) : w.len) + p.start_cost + 0.5 * step;
+      const double guess = step > 0.0 ? 2.0 * static_cast<double>(off) / (a + sqrt(a * a + 2.0 * step * static_cast<double>(off)))
+                                      : static_cast<double>(off) / a;
+      int t = __builtin_amdgcn_readfirstlane(static_cast<int>(guess));
+      t = t < 0 ? 0 : (t >= tiles ? tiles - 1 : t);
+      while (t > 0 && cost_of(p, w.n, w.len, t) > off) --t;
+      while (t + 1 < tiles && cost_of(p, w.n, w.len, t + 1) <= off) ++t;
+      w.tile = t;
+      const uint64_t c0 = cost_of(p, w.n, w.len, t);
+      w.at = row_at + c0;
+      w.cost = cost_of(p, w.n, w.len, t + 1) - c0;
       return true;
     }
-    items = lane_of(to_items, 63);
-    tiles_before = lane_of(to_tiles, 63);
+    from.b0 = b0 + 64;
+    from.before = lane_of(to, 63);
   }
   return false;
+}
+
+// One workgroup's walk over its piece of the line.
+struct Walk {
+  uint64_t x, end, piece;
+  Place from;
+  Row lane_row;     // the lane's row of rows 0 .. 63
+  Tile w;
+  int lo, hi;       // the keys of the tile in this piece: lo to hi (of steps of `grain` keys)
+  bool first, last; // the piece holds the tile's beginning, its end
+};
+__device__ __forceinline__ bool walk_start(const Params& p, int piece_index, Walk& k) {
+  uint64_t all, piece;
+  line_of(p, all, piece, k.lane_row);
+  k.x = piece * static_cast<uint64_t>(piece_index);
+  k.end = k.x + piece < all ? k.x + piece : all;
+  k.from = Place{0, 0};
+  k.piece = piece;
+  k.first = k.last = false;
+  return k.x < k.end;
+}
+// The next tile of the piece; `grain`: keys that are not divided.
+__device__ __forceinline__ bool walk_next(const Params& p, int grain, Walk& k) {
+  if (k.x >= k.end || !find_tile(p, k.x, k.lane_row, k.from, k.w)) return false;
+  const Tile& w = k.w;
+  const uint64_t tile_end = w.at + w.cost;
+  if (tile_end <= k.x) return false;  // (counts that contradict each other)
+  const int rows = w.n * p.G, last_row = ((w.tile + 1) << p.lm) < rows ? ((w.tile + 1) << p.lm) : rows;
+  int seen = p.causal ? w.len - w.n + (last_row - 1) / p.G + 1 : w.len;  // keys that the tile's last row sees
+  seen = seen < 0 ? 0 : seen;
+  k.first = k.x == w.at;
+  k.last = tile_end <= k.end;
+  const int a = static_cast<int>(k.x - w.at) / grain * grain, e = static_cast<int>(k.end - w.at) / grain * grain;
+  k.lo = a < seen ? a : seen;
+  k.hi = k.last || e > seen ? seen : e;
+  k.lo = __builtin_amdgcn_readfirstlane(k.lo);
+  k.hi = __builtin_amdgcn_readfirstlane(k.hi);
+  k.x = tile_end;
+  return true;
 }
 
 // Rows of q past the last sequence: zeros, where the caller asked for them.
@@ -200,6 +262,19 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t block, int64_
       p.out[t * p.o_st + (static_cast<int64_t>(kvh) * G + i / p.D) * p.o_sh + i % p.D] = 0;
 }
 
+// The end of a workgroup.  What the second launch has to join: the piece's last
+// tile, if it begins here and ends elsewhere.
+__device__ __forceinline__ void finish(const Params& p, const Walk& k, bool any) {
+  if (p.zero_tail) zero_tail(p, blockIdx.x / p.Hkv, gridDim.x / p.Hkv, blockIdx.x % p.Hkv);
+  if (p.pieces < 2 || threadIdx.x != 0) return;
+  int parts = 0;
+  if (any && k.first && !k.last) {
+    const uint64_t rest = k.w.at + k.w.cost - k.end;  // > 0: in the next pieces
+    parts = 1;
+    for (uint64_t at = 0; at < rest && parts < p.pieces; at += k.piece) ++parts;
+  }
+  p.cuts[blockIdx.x] = make_int4(k.w.q0, k.w.tile << p.lm, k.w.n * p.G, parts);
+}
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (BF)
@@ -213,12 +288,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
 }
 
-// ---- few rows: tiles of 16 matrix rows, every wave with keys of its own ----
+// ---- few rows: tiles of 16 matrix rows, one wave per workgroup ----
 //
-// A wave takes every fourth (head_dim over 128: second) tile of 32 keys of the
-// item's split.  K and V rows go
-// from the page straight to the wave's own LDS (no register holds them, no barrier
-// is needed), two tiles deep: the next tile's loads fly while this one is computed.
+// The wave walks its piece in steps of 32 keys.  K and V rows go from the page
+// straight to LDS (no register holds them, no barrier is needed), two steps deep:
+// the next step's loads fly while this one is computed.  Five such waves per CU
+// (head_dim 128) keep 80 KB of loads in flight, and one's start or end runs beside
+// the others' loads.
 //   S^T = K Q^T   16x16x32 MFMAs, A = 16 keys x 32 channels, B = Q^T (registers):
 //                 lane (n, g) holds query row n, keys 4 g + i of the 16
 //   O^T += V^T P^T  A = V^T by transposing LDS reads (4 keys x 16 channels each),
@@ -230,15 +306,46 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // 16-byte unit u of LDS row r lies at unit u ^ (2 (r & 7)) (mod the row), which the
 // loads' source addresses bring about: without it the 16 rows that a transposing
 // read touches would share their banks.
+#ifndef FEW_STAGES
+#define FEW_STAGES 2
+#endif
+#ifndef FEW_PER_CU
+#define FEW_PER_CU 4
+#endif
+#ifndef AHEAD256
+#define AHEAD256 2
+#endif
+#ifndef SCHEDB
+#define SCHEDB 0x6
+#endif
+#ifndef WIDE_ST
+#define WIDE_ST 3
+#endif
+#ifndef WIDE_ST256
+#define WIDE_ST256 4
+#endif
+#ifndef FEW_LEAST
+#define FEW_LEAST 64
+#endif
+#ifndef WIDE_NW
+#define WIDE_NW 8
+#endif
+#ifndef WIDE_START
+#define WIDE_START 192
+#endif
+#ifndef WIDE_PER_CU
+#define WIDE_PER_CU 1
+#endif
 template <int DP>
 struct Few {
-  static constexpr int kKeys = 32;                 // keys per tile
+  static constexpr int kKeys = 32;                 // keys per step
   static constexpr int kUnits = DP / 8;            // 16-byte units per row
-  static constexpr int kTensor = kKeys * DP * 2;   // bytes of a tile's K or V
+  static constexpr int kTensor = kKeys * DP * 2;   // bytes of a step's K or V
   static constexpr int kStage = 2 * kTensor;
-  static constexpr int kLoads = kStage / 1024;     // direct loads per tile
-  static constexpr int kWaves = DP > 128 ? 2 : 4;  // (a workgroup's LDS)
-  static constexpr int kLds = kWaves * 2 * kStage;
+  static constexpr int kLoads = kStage / 1024;     // direct loads per step
+  static constexpr int kStages = FEW_STAGES;
+  static constexpr int kQBytes = kRows * DP * 2;
+  static constexpr int kLds = kStages * kStage + kQBytes;
   static constexpr int kSwizzle = kUnits - 1;
 };
 
@@ -248,189 +355,183 @@ __device__ __forceinline__ int few_unit(int row, int u) {
 }
 
 template <int DP, bool BF>
-__global__ __launch_bounds__(64 * Few<DP>::kWaves) void paged_few_kernel(Params p) {
+__global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
   typedef Few<DP> F;
-  constexpr int NKS = DP / 32, NCB = DP / 16, NW = F::kWaves;
-  const int kvh = blockIdx.x % p.Hkv;
-  const uint32_t idx = blockIdx.x / static_cast<uint32_t>(p.Hkv);
-  const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (p.zero_tail) zero_tail(p, idx, gridDim.x / p.Hkv, kvh);
-  Item it;
-  if (!find_item<kRows, false>(p, idx, it)) return;
+  constexpr int NKS = DP / 32, NCB = DP / 16;
+  const int kvh = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
+  const int lane = threadIdx.x, n16 = lane & 15, g = lane >> 4;
+  Walk k;
+  k.w = Tile{};
+  if (!walk_start(p, index, k)) {
+    finish(p, k, false);
+    return;
+  }
   const int D = p.D;
-  const int rows = it.n * p.G - it.tile * kRows < kRows ? it.n * p.G - it.tile * kRows : kRows;
-  // this lane's matrix row: its query, head and visible keys
-  const int r = it.tile * kRows + n16;
-  const bool live = n16 < rows;
-  const int qi = live ? r / p.G : 0, hd = kvh * p.G + (live ? r - qi * p.G : 0);
-  auto limit = [&](int i) {
-    const int x = p.causal ? it.len - it.n + i + 1 : it.len;
-    return x < 0 ? 0 : x;
-  };
-  const int lim = live ? limit(qi) : 0;
-  const int lo = limit(it.tile * kRows / p.G), hi = limit((it.tile * kRows + rows - 1) / p.G);  // fewest, most keys of the tile's rows
-  const int k0 = __builtin_amdgcn_readfirstlane(it.split * it.chunk);  // (chunk INT32_MAX: split 0)
-  const int k1 = __builtin_amdgcn_readfirstlane(it.splits > 1 && k0 + it.chunk < hi ? k0 + it.chunk : hi);
 
   __shared__ __attribute__((aligned(16))) uint8_t lds[F::kLds];
-  uint8_t* const mine = &lds[wave * 2 * F::kStage];
-  const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)mine)));
+  const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds)));
   if (D < DP) {  // units past the head_dim are never loaded: zeros
-    for (int i = 16 * lane; i < 2 * F::kStage; i += 1024) *reinterpret_cast<u32x4*>(mine + i) = u32x4{0, 0, 0, 0};
+    for (int i = 16 * lane; i < F::kStages * F::kStage; i += 1024) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0, 0, 0, 0};
     __builtin_amdgcn_s_waitcnt(kLgkm0);
   }
+  while (walk_next(p, F::kKeys, k)) {
+    const Tile& w = k.w;
+    const int all = w.n * p.G, r = w.tile * kRows + n16;  // this lane's matrix row: its query, head and visible keys
+    const bool live = r < all;
+    const int qi = live ? r / p.G : 0, hd = kvh * p.G + (live ? r - qi * p.G : 0);
+    auto limit = [&](int i) {
+      const int x = p.causal ? w.len - w.n + i + 1 : w.len;
+      return x < 0 ? 0 : x;
+    };
+    const int lim = live ? limit(qi) : 0;
+    const int seen_by_all = __builtin_amdgcn_readfirstlane(limit(w.tile * kRows / p.G));  // the tile's first row sees the fewest
 
-  f32x4 acc[NCB];
+    const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + w.b * p.ppr);  // (scalar loads: vmcnt counts the steps' alone)
+    auto issue = [&](int key, int id, int buf) {
+      id = id < 0 || id >= p.n_pages ? 0 : id;
+      const int64_t at = ((static_cast<int64_t>(id) * p.Hkv + kvh) * kPage + key % kPage) * D;
+      const uint32_t to = base + buf * F::kStage;
 #pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) acc[cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float m = -INFINITY, l = 0.0f;  // of row n16 (l: over this lane's keys)
-
-  const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + it.b * p.ppr);  // (scalar loads: vmcnt counts the tiles' alone)
-  auto page_at = [&](int key) {
-    const int id = __builtin_amdgcn_readfirstlane(trow[key / kPage]);
-    return static_cast<int64_t>(id < 0 || id >= p.n_pages ? 0 : id);
-  };
-  auto issue = [&](int key, int64_t page, int buf) {
-    const int64_t at = ((page * p.Hkv + kvh) * kPage + key % kPage) * D;
-    const uint32_t to = base + buf * F::kStage;
-#pragma unroll
-    for (int i = 0; i < F::kLoads / 2; ++i) {
-      const int pos = 64 * i + lane, row = pos / F::kUnits;
-      const int u = few_unit<DP>(row, pos % F::kUnits);
-      if (DP == D || 8 * u < D) {
-        lds_dma16(p.kp + at + row * D + 8 * u, to + 1024 * i);
-        lds_dma16(p.vp + at + row * D + 8 * u, to + F::kTensor + 1024 * i);
+      for (int i = 0; i < F::kLoads / 2; ++i) {
+        const int pos = 64 * i + lane, row = pos / F::kUnits;
+        const int u = few_unit<DP>(row, pos % F::kUnits);
+        if (DP == D || 8 * u < D) {
+          lds_dma16(p.kp + at + row * D + 8 * u, to + 1024 * i);
+          lds_dma16(p.vp + at + row * D + 8 * u, to + F::kTensor + 1024 * i);
+        }
       }
-    }
-  };
-  const int step = NW * F::kKeys;
-  int key = k0 + wave * F::kKeys;
-  int64_t next_page = 0;
-  if (key < k1) {
-    issue(key, page_at(key), 0);
-    if (key + step < k1) next_page = page_at(key + step);
-  }
-  u32x4 qf[NKS];
-  const uint16_t* qr = p.q + static_cast<int64_t>(it.q0 + qi) * p.q_st + static_cast<int64_t>(hd) * p.q_sh;
+    };
+    // the query's rows to LDS ahead of the keys (16-byte unit i of the tile's 16 rows: row i / kUnits)
+    const uint32_t qlds = base + F::kStages * F::kStage;
 #pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
-    const int c = 32 * ks + 8 * g;
-    qf[ks] = live && c < D ? *reinterpret_cast<const u32x4*>(qr + c) : u32x4{0, 0, 0, 0};
-  }
-  // the query and the first tile; in the loop only the direct loads are in flight, which the compiler does not count
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  for (int t = 0; key < k1; key += step, t ^= 1) {
-    if (key + step < k1) {
-      issue(key + step, next_page, t ^ 1);
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
-      if (key + 2 * step < k1) next_page = page_at(key + 2 * step);
-    } else {
-      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    for (int i = 0; i < F::kQBytes / 1024 + (F::kQBytes % 1024 != 0); ++i) {
+      const int pos = 64 * i + lane, row = pos / F::kUnits, u = pos % F::kUnits;
+      const int rr = w.tile * kRows + row, ri = rr < all ? rr : all - 1, rq = ri / p.G;
+      if (DP == D || 8 * u < D)
+        lds_dma16(p.q + static_cast<int64_t>(w.q0 + rq) * p.q_st + static_cast<int64_t>(kvh * p.G + ri - rq * p.G) * p.q_sh + 8 * u, qlds + 1024 * i);
     }
-    asm volatile("" ::: "memory");
-    uint8_t* const kt = mine + t * F::kStage;
-    uint8_t* const vt = kt + F::kTensor;
-    const int cnt = it.len - key;  // rows from here on hold no token of the row: whatever stands there must not count
-    if (cnt < F::kKeys) {
-      for (int i = lane; i < (F::kKeys - cnt) * F::kUnits; i += 64)
-        *reinterpret_cast<u32x4*>(vt + 16 * (cnt * F::kUnits + i)) = u32x4{0, 0, 0, 0};
-    }
-    f32x4 s[2];
+    int key = k.lo, ahead = k.lo, next = 0;  // ahead: the first key not asked for
 #pragma unroll
-    for (int kt16 = 0; kt16 < 2; ++kt16) {
-      s[kt16] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      const int row = 16 * kt16 + n16;
+    for (int i = 0; i < F::kStages - 1; ++i)
+      if (ahead < k.hi) {
+        issue(ahead, __builtin_amdgcn_readfirstlane(trow[ahead / kPage]), i);
+        ahead += F::kKeys;
+      }
+    if (ahead < k.hi) next = trow[ahead / kPage];
+    u32x4 qf[NKS];
+    {
+      // the query's loads are done when no more than the steps' are in flight
+      const int steps = (ahead - key + F::kKeys - 1) / F::kKeys;
+      if (steps >= 2 && F::kStages > 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * F::kLoads));
+      else if (steps >= 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
+      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      asm volatile("" ::: "memory");
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * DP * 2 + 16 * few_unit<DP>(row, 4 * ks + g));
-        s[kt16] = mfma16<BF>(a, qf[ks], s[kt16]);
+        const int c = 32 * ks + 8 * g;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(lds + F::kStages * F::kStage + 2 * (n16 * DP + c));
+        qf[ks] = DP == D || c < D ? x : u32x4{0, 0, 0, 0};
       }
     }
-    float x[8], tm = -INFINITY;
-    const bool whole = key + F::kKeys <= lo;
+    f32x4 acc[NCB];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = s[i >> 2][i & 3] * p.scale_log2;
-      if (!whole && key + 16 * (i >> 2) + 4 * g + (i & 3) >= lim) x[i] = -INFINITY;
-      tm = fmaxf(tm, x[i]);
+    for (int cb = 0; cb < NCB; ++cb) acc[cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;  // of row n16 (l: over this lane's keys)
+    for (int t = 0; key < k.hi; key += F::kKeys, t = t + 1 == F::kStages ? 0 : t + 1) {
+      if (ahead < k.hi) {
+        issue(ahead, __builtin_amdgcn_readfirstlane(next), t == 0 ? F::kStages - 1 : t - 1);
+        ahead += F::kKeys;
+        if (ahead < k.hi) next = trow[ahead / kPage];
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((F::kStages - 1) * F::kLoads));
+      } else if (F::kStages > 2 && key + F::kKeys < k.hi) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
+      } else {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      }
+      asm volatile("" ::: "memory");
+      uint8_t* const kt = lds + t * F::kStage;
+      uint8_t* const vt = kt + F::kTensor;
+      const int cnt = w.len - key;  // rows from here on hold no token of the row: whatever stands there must not count
+      if (cnt < F::kKeys) {
+        for (int i = lane; i < (F::kKeys - cnt) * F::kUnits; i += 64)
+          *reinterpret_cast<u32x4*>(vt + 16 * (cnt * F::kUnits + i)) = u32x4{0, 0, 0, 0};
+      }
+      f32x4 s[2];
+#pragma unroll
+      for (int kt16 = 0; kt16 < 2; ++kt16) {
+        s[kt16] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const int row = 16 * kt16 + n16;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * DP * 2 + 16 * few_unit<DP>(row, 4 * ks + g));
+          s[kt16] = mfma16<BF>(a, qf[ks], s[kt16]);
+        }
+      }
+      float x[8], tm = -INFINITY;
+      const bool whole = key + F::kKeys <= seen_by_all;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = s[i >> 2][i & 3] * p.scale_log2;
+        if (!whole && key + 16 * (i >> 2) + 4 * g + (i & 3) >= lim) x[i] = -INFINITY;
+        tm = fmaxf(tm, x[i]);
+      }
+      tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
+      tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+      const float mn = fmaxf(m, tm);
+      const float ms = mn == -INFINITY ? 0.0f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - ms);
+      m = mn;
+      float ps = 0.0f;
+      u32x4 ph, pl;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float a = __builtin_amdgcn_exp2f(x[i] - ms), b = __builtin_amdgcn_exp2f(x[i + 1] - ms);
+        ps += a + b;
+        const uint32_t h = pack2<BF>(a, b);
+        ph[i / 2] = h;
+        pl[i / 2] = pack2<BF>(a - w2f<BF>(static_cast<uint16_t>(h)), b - w2f<BF>(static_cast<uint16_t>(h >> 16)));
+      }
+      l = l * alpha + ps;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        // lane (n, g) points at key 4 g + n / 4 (+ 16), channels 16 cb + 4 (n % 4) .. + 3
+        const int row = 4 * g + (n16 >> 2), u = 2 * cb + ((n16 >> 1) & 1);
+        const uint8_t* at = vt + row * DP * 2 + 16 * few_unit<DP>(row, u) + 8 * (n16 & 1);
+        const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at)));
+        const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at + 16 * DP * 2)));  // (row + 16: the same swizzle)
+        const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+        const u32x4 a = {w0.x, w0.y, w1.x, w1.y};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[cb][i] *= alpha;
+        acc[cb] = mfma16<BF>(a, ph, acc[cb]);
+        acc[cb] = mfma16<BF>(a, pl, acc[cb]);
+      }
     }
-    tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
-    tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-    const float mn = fmaxf(m, tm);
-    const float ms = mn == -INFINITY ? 0.0f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - ms);
-    m = mn;
-    float ps = 0.0f;
-    u32x4 ph, pl;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    // ---- lane (n, g): row n, channels 16 cb + 4 g .. + 3 ----
+    if (!live) continue;
+    if (k.first && k.last) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no visible key: zeros
+      uint16_t* dst = p.out + static_cast<int64_t>(w.q0 + qi) * p.o_st + static_cast<int64_t>(hd) * p.o_sh;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float a = __builtin_amdgcn_exp2f(x[i] - ms), b = __builtin_amdgcn_exp2f(x[i + 1] - ms);
-      ps += a + b;
-      const uint32_t h = pack2<BF>(a, b);
-      ph[i / 2] = h;
-      pl[i / 2] = pack2<BF>(a - w2f<BF>(static_cast<uint16_t>(h)), b - w2f<BF>(static_cast<uint16_t>(h >> 16)));
-    }
-    l = l * alpha + ps;
-#pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
-      // lane (n, g) points at key 4 g + n / 4 (+ 16), channels 16 cb + 4 (n % 4) .. + 3
-      const int row = 4 * g + (n16 >> 2), u = 2 * cb + ((n16 >> 1) & 1);
-      const uint8_t* at = vt + row * DP * 2 + 16 * few_unit<DP>(row, u) + 8 * (n16 & 1);
-      const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at)));
-      const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at + 16 * DP * 2)));  // (row + 16: the same swizzle)
-      const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-      const u32x4 a = {w0.x, w0.y, w1.x, w1.y};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[cb][i] *= alpha;
-      acc[cb] = mfma16<BF>(a, ph, acc[cb]);
-      acc[cb] = mfma16<BF>(a, pl, acc[cb]);
-    }
-  }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-
-  // ---- the waves' sums joined, in wave order ----
-  constexpr int PITCH = DP + 4;
-  static_assert(NW * kRows * PITCH * 4 <= F::kLds, "the waves' sums fit the tiles' LDS");
-  float* const so = reinterpret_cast<float*>(lds);
-  __shared__ float2 sml[NW][kRows];
-  __syncthreads();
-#pragma unroll
-  for (int cb = 0; cb < NCB; ++cb) *reinterpret_cast<f32x4*>(so + (wave * kRows + n16) * PITCH + 16 * cb + 4 * g) = acc[cb];
-  if (g == 0) sml[wave][n16] = make_float2(m, l);
-  __syncthreads();
-  const bool part = it.splits > 1;
-  const int64_t pr = static_cast<int64_t>(blockIdx.x) * kRows;
-  for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
-    const int row = i / (DP / 4), c = 4 * (i % (DP / 4));
-    if (c >= D) continue;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, sml[w][row].x);
-    const float ms = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sml[w][row].x - ms);
-      sum += sml[w][row].y * f;
-      o += *reinterpret_cast<const f32x4*>(so + (w * kRows + row) * PITCH + c) * f;
-    }
-    if (part) {
-      *reinterpret_cast<f32x4*>(p.part_o + (pr + row) * D + c) = o;
-      if (c == 0) p.part_ml[pr + row] = make_float2(mx, sum);
+      for (int cb = 0; cb < NCB; ++cb) {
+        const int c = 16 * cb + 4 * g;
+        if (c < D)
+          *reinterpret_cast<u32x2*>(dst + c) = u32x2{pack2<BF>(acc[cb][0] * inv, acc[cb][1] * inv), pack2<BF>(acc[cb][2] * inv, acc[cb][3] * inv)};
+      }
     } else {
-      const int rr = it.tile * kRows + row, qq = rr / p.G;
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no visible key: zeros
-      uint16_t* dst = p.out + static_cast<int64_t>(it.q0 + qq) * p.o_st + static_cast<int64_t>(kvh * p.G + rr - qq * p.G) * p.o_sh + c;
-      u32x2 w;
-      w.x = static_cast<uint32_t>(f2w<BF>(o[0] * inv)) | (static_cast<uint32_t>(f2w<BF>(o[1] * inv)) << 16);
-      w.y = static_cast<uint32_t>(f2w<BF>(o[2] * inv)) | (static_cast<uint32_t>(f2w<BF>(o[3] * inv)) << 16);
-      *reinterpret_cast<u32x2*>(dst) = w;
+      const int64_t pr = (static_cast<int64_t>(blockIdx.x) * 2 + (k.first ? 1 : 0)) * kRows + n16;
+      if (g == 0) p.part_ml[pr] = make_float2(m, l);
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        const int c = 16 * cb + 4 * g;
+        if (c < D) *reinterpret_cast<f32x4*>(p.part_o + pr * D + c) = acc[cb];
+      }
     }
   }
+  finish(p, k, true);
 }
 
 // ---- many rows: tiles of 32 NW MT matrix rows, the keys shared through LDS ----
@@ -462,6 +563,12 @@ __device__ __forceinline__ int wide_v_unit(int row, int u) {
   if constexpr (DP == 64) return u ^ (4 * ((row >> 1) & 1));
   else return u ^ (4 * (row & 3));
 }
+__device__ __forceinline__ u32x4 lds_read16(uint32_t at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(at);
+}
+__device__ __forceinline__ u32x2 lds_read_tr(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>(at)));
+}
 template <bool BF>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   if constexpr (BF)
@@ -470,72 +577,112 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <int DP, int NW, int MT, bool BF>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void paged_wide_kernel(Params p) {
+template <int DP, int NW, int MT, int KT, int NST, bool BF>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_wide_kernel(Params p) {
   constexpr int M = 32 * NW * MT;
   constexpr int NKS = DP / 16, NCB = DP / 32, UNITS = DP / 8;
-  constexpr int TENSOR = kPage * DP * 2, STAGE = 2 * TENSOR;
+  constexpr int TENSOR = KT * DP * 2, STAGE = 2 * TENSOR, NKB = KT / 32;
   constexpr int LPW = TENSOR / 1024 / NW;  // direct loads of K, and of V, per wave and page
   static_assert(TENSOR % (1024 * NW) == 0, "a page is shared out evenly");
-  const int kvh = blockIdx.x % p.Hkv;
-  const uint32_t idx = blockIdx.x / static_cast<uint32_t>(p.Hkv);
+  const int kvh = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   const int lane = threadIdx.x & 63, n32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (p.zero_tail) zero_tail(p, idx, gridDim.x / p.Hkv, kvh);
-  Item it;
-  if (!find_item<M, false>(p, idx, it)) return;
+  Walk k;
+  k.w = Tile{};
+  if (!walk_start(p, index, k)) {
+    finish(p, k, false);
+    return;
+  }
   const int D = p.D;
-  const int all = it.n * p.G;  // the row's matrix rows
+
+  __shared__ __attribute__((aligned(256))) uint8_t lds[NST * STAGE];
+  const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds)));
+  if (D < DP) {  // units past the head_dim are never loaded: zeros
+    for (int i = 16 * threadIdx.x; i < NST * STAGE; i += 1024 * NW) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+  }
+  // this lane's places of a step: load i fills unit 64 (LPW wave + i) + lane
+  auto place = [&](int i, int l, uint32_t& ko, uint32_t& vo, bool& kin, bool& vin) {
+    const int pos = 64 * (LPW * wave + i) + l, row = pos / UNITS, u = pos % UNITS;
+    const int ku = wide_k_unit<DP>(row, u), vu = wide_v_unit<DP>(row, u);
+    kin = DP == D || 8 * ku < D;
+    vin = DP == D || 8 * vu < D;
+    ko = static_cast<uint32_t>(2 * (row * D + 8 * ku));
+    vo = static_cast<uint32_t>(2 * (row * D + 8 * vu));
+  };
+  // (at head_dim over 128 no register is left to keep them: spilled, their reloads would wait for the loads in flight)
+  constexpr bool kKeep = DP <= 128;
+  uint32_t ko[kKeep ? LPW : 1], vo[kKeep ? LPW : 1];
+  bool kin[kKeep ? LPW : 1], vin[kKeep ? LPW : 1];
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) place(i, lane, ko[i], vo[i], kin[i], vin[i]);
+  }
+  // where this lane reads: K row n32 (+ 32), unit 2 ks + h; V row 4 h + (l16 >> 2) (+ 16 ks, + 8), channels
+  // 32 cb + 16 ((lane >> 4) & 1) + 4 (l16 & 3), l16 = lane & 15.  Units are exchanged by an exclusive or within
+  // 256 bytes, alike in rows 32, 16 and 8 apart: of an address, ks and cb change bits by one more of them, the
+  // rest is a constant.
+  constexpr int KA = NKS < 8 ? NKS : 8, VA = NCB < 4 ? NCB : 4;
+  static_assert(TENSOR % 256 == 0, "rows start at multiples of the exchanged units' span");
+  const int vrow = 4 * h + ((lane & 15) >> 2);
+  uint32_t kat = base + n32 * DP * 2 + 16 * wide_k_unit<DP>(n32, h);
+  uint32_t vat = base + TENSOR + vrow * DP * 2 + 16 * wide_v_unit<DP>(vrow, 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
+  int buf = 0;
+  auto flip = [&]() {  // the next buffer
+    const uint32_t d = buf == NST - 1 ? -static_cast<uint32_t>((NST - 1) * STAGE) : STAGE;
+    kat += d;
+    vat += d;
+    buf = buf == NST - 1 ? 0 : buf + 1;
+  };
+  const float sl2 = p.scale_log2;
+  while (walk_next(p, KT, k)) {
+  const Tile& w = k.w;
+  const int all = w.n * p.G;  // the row's matrix rows
   auto limit = [&](int i) {
-    const int x = p.causal ? it.len - it.n + i + 1 : it.len;
+    const int x = p.causal ? w.len - w.n + i + 1 : w.len;
     return x < 0 ? 0 : x;
   };
-  const int last = it.tile * M + M < all ? it.tile * M + M : all;  // past the item's last matrix row
-  const int hi = limit((last - 1) / p.G);
-  const int k0 = __builtin_amdgcn_readfirstlane(it.split * it.chunk);
-  const int k1 = __builtin_amdgcn_readfirstlane(it.splits > 1 && k0 + it.chunk < hi ? k0 + it.chunk : hi);
   // this wave's matrix rows, and the fewest and the most keys they see
-  const int r0 = it.tile * M + 32 * MT * wave;
+  const int r0 = w.tile * M + 32 * MT * wave;
   const bool active = r0 < all;
   const int rl = r0 + 32 * MT < all ? r0 + 32 * MT : all;
   const int wlo = __builtin_amdgcn_readfirstlane(active ? limit(r0 / p.G) : 0);
   const int whi = __builtin_amdgcn_readfirstlane(active ? limit((rl - 1) / p.G) : 0);
   int lim[MT];
-
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
-  const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds)));
-  if (D < DP) {  // units past the head_dim are never loaded: zeros
-    for (int i = 16 * threadIdx.x; i < 2 * STAGE; i += 1024 * NW) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0, 0, 0, 0};
-    __syncthreads();
-  }
-  // this lane's places of a page: load i fills unit 64 (LPW wave + i) + lane
-  uint32_t ko[LPW], vo[LPW];
-  bool kin[LPW], vin[LPW];
-#pragma unroll
-  for (int i = 0; i < LPW; ++i) {
-    const int pos = 64 * (LPW * wave + i) + lane, row = pos / UNITS, u = pos % UNITS;
-    const int ku = wide_k_unit<DP>(row, u), vu = wide_v_unit<DP>(row, u);
-    kin[i] = DP == D || 8 * ku < D;
-    vin[i] = DP == D || 8 * vu < D;
-    ko[i] = static_cast<uint32_t>(2 * (row * D + 8 * ku));
-    vo[i] = static_cast<uint32_t>(2 * (row * D + 8 * vu));
-  }
-  const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + it.b * p.ppr);
-  auto issue = [&](int id, int buf) {
+  const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + w.b * p.ppr);  // (scalar loads: vmcnt counts the steps' alone)
+  auto issue = [&](int key, int id, int buf) {
     id = id < 0 || id >= p.n_pages ? 0 : id;
-    const int64_t at = (static_cast<int64_t>(id) * p.Hkv + kvh) * kPage * D;
+    const int64_t at = ((static_cast<int64_t>(id) * p.Hkv + kvh) * kPage + key % kPage) * D;
     const uint32_t to = base + buf * STAGE + 1024 * LPW * wave;
+    if constexpr (kKeep) {
 #pragma unroll
-    for (int i = 0; i < LPW; ++i) {
-      if (kin[i]) lds_dma16(p.kp + at, ko[i], to + 1024 * i);
-      if (vin[i]) lds_dma16(p.vp + at, vo[i], to + TENSOR + 1024 * i);
+      for (int i = 0; i < LPW; ++i) {
+        if (kin[i]) lds_dma16(p.kp + at, ko[i], to + 1024 * i);
+        if (vin[i]) lds_dma16(p.vp + at, vo[i], to + TENSOR + 1024 * i);
+      }
+    } else {
+      int l = threadIdx.x & 63;
+      asm volatile("" : "+v"(l));  // (not computed ahead of the loop)
+#pragma unroll
+      for (int i = 0; i < LPW; ++i) {
+        uint32_t k_off, v_off;
+        bool k_in, v_in;
+        place(i, l, k_off, v_off, k_in, v_in);
+        if (k_in) lds_dma16(p.kp + at, k_off, to + 1024 * i);
+        if (v_in) lds_dma16(p.vp + at, v_off, to + TENSOR + 1024 * i);
+      }
     }
   };
-  const int t0 = k0 / kPage, t1 = (k1 + kPage - 1) / kPage;
-  int next = 0;
-  if (t0 < t1) {
-    issue(__builtin_amdgcn_readfirstlane(trow[t0]), 0);
-    if (t0 + 1 < t1) next = __builtin_amdgcn_readfirstlane(trow[t0 + 1]);
+  __syncthreads();  // the LDS is done with
+  int ahead = k.lo, next = 0;  // ahead: the first key not asked for
+  auto issue_next = [&](int to) {
+    issue(ahead, __builtin_amdgcn_readfirstlane(next), to);
+    ahead += KT;
+    if (ahead < k.hi) next = trow[ahead / kPage];
+  };
+  if (ahead < k.hi) {
+    next = trow[ahead / kPage];
+    issue_next(buf);
   }
   u32x4 qf[MT][NKS];
 #pragma unroll
@@ -544,7 +691,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const bool live = r < all;
     const int qi = live ? r / p.G : 0;
     lim[mt] = live ? limit(qi) : 0;
-    const uint16_t* qr = p.q + static_cast<int64_t>(it.q0 + qi) * p.q_st + static_cast<int64_t>(kvh * p.G + (live ? r - qi * p.G : 0)) * p.q_sh;
+    const uint16_t* qr = p.q + static_cast<int64_t>(w.q0 + qi) * p.q_st + static_cast<int64_t>(kvh * p.G + (live ? r - qi * p.G : 0)) * p.q_sh;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) {
       const int c = 16 * ks + 8 * h;
@@ -562,46 +709,63 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[mt][cb][i] = 0.0f;
   }
-  const float sl2 = p.scale_log2;
 
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // this wave's share of page t
-    __syncthreads();                           // everyone's; and page t - 1 is done with
-    uint8_t* const kt = lds + buf * STAGE;
-    uint8_t* const vt = kt + TENSOR;
-    const int key = t * kPage, cnt = it.len - key;
-    if (cnt < kPage) {  // rows that hold no token: whatever stands there must not count
-      for (int i = threadIdx.x; i < (kPage - cnt) * UNITS; i += 64 * NW) *reinterpret_cast<u32x4*>(vt + 16 * (cnt * UNITS + i)) = u32x4{0, 0, 0, 0};
+  // the query and the first step; in the loop only the direct loads are in flight, which the compiler does not count
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+#pragma unroll
+  for (int i = 1; i < NST - 1; ++i)
+    if (ahead < k.hi) issue_next(buf + i < NST ? buf + i : buf + i - NST);
+  for (int key = k.lo; key < k.hi; key += KT, flip()) {
+    // this wave's share of the step: later steps' may be in flight
+    const int later = ahead - key - KT;
+    if (NST > 3 && later > KT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(4 * LPW));
+    else if (NST > 2 && later > 0) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * LPW));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    __syncthreads();  // everyone's; and the step before is done with
+    uint8_t* const vt = lds + buf * STAGE + TENSOR;
+    const int cnt = w.len - key;
+    if (cnt < KT) {  // rows that hold no token: whatever stands there must not count
+      for (int i = threadIdx.x; i < (KT - cnt) * UNITS; i += 64 * NW) *reinterpret_cast<u32x4*>(vt + 16 * (cnt * UNITS + i)) = u32x4{0, 0, 0, 0};
       __syncthreads();
     }
-    if (t + 1 < t1) {
-      issue(next, buf ^ 1);
-      if (t + 2 < t1) next = __builtin_amdgcn_readfirstlane(trow[t + 2]);
-    }
-    if (key >= whi) continue;
-    f32x16 s[MT][2];
+    if (ahead < k.hi) issue_next(buf == 0 ? NST - 1 : buf - 1);
+    if (key >= whi) continue;  // (to flip())
+    // fragments are read AH ahead of their products
+    constexpr int AH = DP > 128 ? AHEAD256 : 4;
+    auto k_frag = [&](int f) { return lds_read16((kat ^ (32 * (f % NKS % KA))) + 32 * (f / NKS) * DP * 2 + 256 * (f % NKS / KA)); };
+    auto v_frag = [&](int f) {
+      const uint32_t at = (vat ^ (64 * (f % NCB % VA))) + 16 * (f / NCB) * DP * 2 + 256 * (f % NCB / VA);
+      const u32x2 w0 = lds_read_tr(at), w1 = lds_read_tr(at + 8 * DP * 2);  // (row + 8: the same exchange)
+      return u32x4{w0.x, w0.y, w1.x, w1.y};
+    };
+    f32x16 s[MT][NKB];
+    {
+      u32x4 kf[AH];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+      for (int f = 0; f < AH; ++f) kf[f] = k_frag(f);
+      __builtin_amdgcn_sched_barrier(SCHEDB);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int f = 0; f < NKS * NKB; ++f) {
+        const u32x4 a = kf[f % AH];
+        if (f + AH < NKS * NKB) kf[f % AH] = k_frag(f + AH);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[mt][kb][i] = 0.0f;
-      const int row = 32 * kb + n32;
+        for (int mt = 0; mt < MT; ++mt) {
+          if (f % NKS == 0) {
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * DP * 2 + 16 * wide_k_unit<DP>(row, 2 * ks + h));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[mt][kb] = mfma32<BF>(a, qf[mt][ks], s[mt][kb]);
+            for (int i = 0; i < 16; ++i) s[mt][f / NKS][i] = 0.0f;
+          }
+          s[mt][f / NKS] = mfma32<BF>(a, qf[mt][f % NKS], s[mt][f / NKS]);
+        }
+        __builtin_amdgcn_sched_barrier(SCHEDB);
       }
     }
-    u32x4 pa[MT][4];
+    u32x4 pa[MT][2 * NKB];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      if (key + kPage > wlo) {
+      if (key + KT > wlo) {
         const int left = lim[mt] - key;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (32 * kb + 8 * (i >> 2) + 4 * h + (i & 3) >= left) s[mt][kb][i] = -INFINITY;
@@ -609,23 +773,23 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
       auto probs = [&]() {
         const float nm = -m[mt] * sl2;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int st = 0; st < 2 * NKB; ++st)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            pa[mt][k][j] = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[mt][k >> 1][8 * (k & 1) + 2 * j], sl2, nm)),
-                                     __builtin_amdgcn_exp2f(fmaf(s[mt][k >> 1][8 * (k & 1) + 2 * j + 1], sl2, nm)));
+            pa[mt][st][j] = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[mt][st >> 1][8 * (st & 1) + 2 * j], sl2, nm)),
+                                      __builtin_amdgcn_exp2f(fmaf(s[mt][st >> 1][8 * (st & 1) + 2 * j + 1], sl2, nm)));
       };
       probs();
       // 16-bit patterns of the non-negative probabilities order as their values do
-      const u16x8 pm = __builtin_elementwise_max(
-          __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][0]), __builtin_bit_cast(u16x8, pa[mt][1])),
-          __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][2]), __builtin_bit_cast(u16x8, pa[mt][3])));
+      u16x8 pm = __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][0]), __builtin_bit_cast(u16x8, pa[mt][1]));
+      if constexpr (NKB == 2)
+        pm = __builtin_elementwise_max(pm, __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][2]), __builtin_bit_cast(u16x8, pa[mt][3])));
       const auto p2 = __builtin_elementwise_max(__builtin_elementwise_max(pm.s01, pm.s23), __builtin_elementwise_max(pm.s45, pm.s67));
       constexpr uint16_t kOver = BF ? 0x4380 : 0x5C00;  // 2^8
       if (__builtin_amdgcn_ballot_w64(p2.x > kOver || p2.y > kOver) != 0) {
         float mx = kNegBig;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
           for (int i = 0; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[mt][kb][i], s[mt][kb][i + 1]));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -641,44 +805,42 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
       }
       float ps = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int st = 0; st < 2 * NKB; ++st)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t w = pa[mt][k][j];  // (a bit cast of a vector's element itself takes element 0)
+          const uint32_t pw = pa[mt][st][j];  // (a bit cast of a vector's element itself takes element 0)
           if constexpr (BF)
-            ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), (bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}), ps, false);
+            ps = __builtin_amdgcn_fdot2c_f32_bf16(__builtin_bit_cast(bf16x2, pw), (bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}), ps, false);
           else
-            ps = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), (f16x2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}), ps, false);
+            ps = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pw), (f16x2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}), ps, false);
         }
       l[mt] += ps;
     }
+    {
+      u32x4 vf[AH];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
+      for (int f = 0; f < AH; ++f) vf[f] = v_frag(f);
+      __builtin_amdgcn_sched_barrier(SCHEDB);
 #pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        // lane points at key 16 ks + 4 h + (l16 >> 2) (+ 8), channels 32 cb + 16 ((lane >> 4) & 1) + 4 (l16 & 3)
-        const int row = 16 * ks + 4 * h + ((lane & 15) >> 2), u = 4 * cb + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-        const uint8_t* at = vt + row * DP * 2 + 16 * wide_v_unit<DP>(row, u) + 8 * (lane & 1);
-        const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at)));
-        const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at + 8 * DP * 2)));  // (row + 8: the same exchange)
-        const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-        const u32x4 a = {w0.x, w0.y, w1.x, w1.y};
+      for (int f = 0; f < 2 * NKB * NCB; ++f) {
+        const u32x4 a = vf[f % AH];
+        if (f + AH < 2 * NKB * NCB) vf[f % AH] = v_frag(f + AH);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt][cb] = mfma32<BF>(a, pa[mt][ks], acc[mt][cb]);
+        for (int mt = 0; mt < MT; ++mt) acc[mt][f % NCB] = mfma32<BF>(a, pa[mt][f / NCB], acc[mt][f % NCB]);
+        __builtin_amdgcn_sched_barrier(SCHEDB);
       }
     }
   }
 
   // ---- lane (n, h): row n, channels 32 cb + 8 q + 4 h .. + 3 ----
-  const bool part = it.splits > 1;
+  const bool part = !(k.first && k.last);
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const float lt = l[mt] + __shfl_xor(l[mt], 32, 64);
     const int r = r0 + 32 * mt + n32;
     if (r >= all) continue;
     if (part) {
-      const int64_t pr = static_cast<int64_t>(blockIdx.x) * M + 32 * (MT * wave + mt) + n32;
+      const int64_t pr = (static_cast<int64_t>(blockIdx.x) * 2 + (k.first ? 1 : 0)) * M + 32 * (MT * wave + mt) + n32;
       if (h == 0) p.part_ml[pr] = make_float2(m[mt] * sl2, lt);
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb)
@@ -690,7 +852,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
     } else {
       const int qi = r / p.G;
       const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;  // no visible key: zeros
-      uint16_t* dst = p.out + static_cast<int64_t>(it.q0 + qi) * p.o_st + static_cast<int64_t>(kvh * p.G + r - qi * p.G) * p.o_sh;
+      uint16_t* dst = p.out + static_cast<int64_t>(w.q0 + qi) * p.o_st + static_cast<int64_t>(kvh * p.G + r - qi * p.G) * p.o_sh;
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
@@ -703,70 +865,114 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
         }
     }
   }
+  }
+  finish(p, k, true);
 }
 
-// The splits of a tile's rows joined in split order: D / 4 threads per row.
-template <int M, bool BF>
-__global__ __launch_bounds__(kThreads) void paged_merge_kernel(Params p) {
-  const int kvh = blockIdx.x % p.Hkv;
-  Item it;
-  if (!find_item<M, true>(p, blockIdx.x / p.Hkv, it) || it.splits < 2) return;
-  const int tpr = p.D / 4, rpb = kThreads / tpr;
-  const int row = blockIdx.y * rpb + threadIdx.x / tpr, c = 4 * (threadIdx.x % tpr);
-  const int rows = it.n * p.G - it.tile * M < M ? it.n * p.G - it.tile * M : M;
-  if (threadIdx.x >= static_cast<unsigned>(rpb * tpr) || row >= rows) return;
-  const int64_t item = it.first + static_cast<int64_t>(it.tiles - 1 - it.tile) * it.splits;
-  if (item + it.splits > p.items) return;  // (counts that contradict each other)
-  auto at = [&](int s) { return ((item + s) * p.Hkv + kvh) * M + row; };
-  float mx = -INFINITY;
+// Tiles that a piece's border cuts, their parts joined in the order of the keys:
+// the beginning in piece `index` of the kv head, ends in the pieces after it.
+// D / 4 threads per matrix row; of a tile of many parts the threads left over take
+// a share each, whose sums are added up through LDS in a fixed order.
+template <bool BF>
+__device__ __forceinline__ void merge_tile(const Params& p, int block, int row0, int row_step) {
+  const int4 cut = p.cuts[block];
+  const int parts = cut.w;
+  if (parts < 2) return;
+  const int kvh = block % p.Hkv, M = 1 << p.lm;
+  const int rows = cut.z - cut.y < M ? cut.z - cut.y : M;
+  const int tpr = p.D / 4, groups = kThreads / tpr;
+  const int grp = threadIdx.x / tpr, c = 4 * (threadIdx.x % tpr);
+  const int per_row = parts >= 8 ? (groups < 8 ? groups : 8) : 1;  // threads' groups per row
+  const int rows_at_once = groups / per_row, sub = grp % per_row;
+  const bool in = grp < rows_at_once * per_row;
+  __shared__ f32x4 so[kThreads];
+  __shared__ float2 sml[kThreads];
+  auto at = [&](int i, int row) { return ((static_cast<int64_t>(block) + static_cast<int64_t>(i) * p.Hkv) * 2 + (i == 0 ? 1 : 0)) * M + row; };
+  for (int rb = row0 * rows_at_once; rb < rows; rb += row_step * rows_at_once) {
+    const int row = rb + grp / per_row;
+    const bool mine = in && row < rows;
+    float mx = -INFINITY, sum = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine) {
+      // a running maximum, as in the kernels: the parts' loads do not wait for it
 #pragma unroll 4
-  for (int s = 0; s < it.splits; ++s) mx = fmaxf(mx, p.part_ml[at(s)].x);
-  const float ms = mx == -INFINITY ? 0.0f : mx;
-  float sum = 0.0f;
-  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int s = 0; s < it.splits; ++s) {
-    const float2 w = p.part_ml[at(s)];
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p.part_o + at(s) * p.D + c);
-    const float f = __builtin_amdgcn_exp2f(w.x - ms);
-    sum += w.y * f;
-    o += a * f;
+      for (int i = sub; i < parts; i += per_row) {
+        const float2 ml = p.part_ml[at(i, row)];
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p.part_o + at(i, row) * p.D + c);
+        const float mn = fmaxf(mx, ml.x), ms = mn == -INFINITY ? 0.0f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(mx - ms), f1 = __builtin_amdgcn_exp2f(ml.x - ms);
+        mx = mn;
+        sum = sum * f0 + ml.y * f1;
+        o = o * f0 + a * f1;
+      }
+    }
+    if (per_row > 1) {
+      __syncthreads();
+      so[threadIdx.x] = o;
+      sml[threadIdx.x] = make_float2(mx, sum);
+      __syncthreads();
+      if (mine && sub == 0) {
+        float mm = mx;
+        for (int i = 1; i < per_row; ++i) mm = fmaxf(mm, sml[threadIdx.x + i * tpr].x);
+        const float ms = mm == -INFINITY ? 0.0f : mm;
+        sum = 0.0f;
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < per_row; ++i) {
+          const float2 ml = sml[threadIdx.x + i * tpr];
+          const float f = __builtin_amdgcn_exp2f(ml.x - ms);
+          sum += ml.y * f;
+          o += so[threadIdx.x + i * tpr] * f;
+        }
+      }
+    }
+    if (mine && sub == 0) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const int r = cut.y + row, qi = r / p.G;
+      uint16_t* dst = p.out + static_cast<int64_t>(cut.x + qi) * p.o_st + static_cast<int64_t>(kvh * p.G + r - qi * p.G) * p.o_sh + c;
+      *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<BF>(o[0] * inv, o[1] * inv), pack2<BF>(o[2] * inv, o[3] * inv)};
+    }
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int r = it.tile * M + row, qi = r / p.G;
-  uint16_t* dst = p.out + static_cast<int64_t>(it.q0 + qi) * p.o_st + static_cast<int64_t>(kvh * p.G + r - qi * p.G) * p.o_sh + c;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) dst[i] = f2w<BF>(o[i] * inv);
+}
+
+// Four blocks per piece of the few-row kernel, then eight per piece of the wide one.
+constexpr int kFewShares = 4, kWideShares = 8;
+template <bool BF>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(Params a, Params b, int first_blocks) {
+  const int i = blockIdx.x, j = i - first_blocks;
+  if (j < 0) merge_tile<BF>(a, i / kFewShares, i % kFewShares, kFewShares);
+  else merge_tile<BF>(b, j / kWideShares, j % kWideShares, kWideShares);
 }
 
 bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
 
-// How one kernel's work of a call is cut, from the sizes the host knows.
-struct Plan {
-  int M = 0;              // matrix rows of a tile; 0: not launched
-  int rows_of = kAll;
-  int target = 0, least = 0;
-  int64_t tiles = 0, items = 0;  // bounds: tiles of rows, items (per kv head)
-};
-struct Plans {
-  Plan few, wide;
-};
-
 template <int DP>
-struct Wide {  // waves and blocks of 32 rows per wave
-  static constexpr int NW = DP > 128 ? 4 : 8, MT = 1, M = 32 * NW * MT;
+struct Wide {  // waves, blocks of 32 rows per wave, keys per step
+  static constexpr int NW = WIDE_NW, MT = 1, M = 32 * NW * MT, KT = DP > 128 ? 32 : 64, NST = DP > 128 ? WIDE_ST256 : WIDE_ST;
 };
-int wide_rows(int D) { return D > 128 ? Wide<256>::M : Wide<128>::M; }
+constexpr int kWideLog = WIDE_NW == 8 ? 8 : 7;
 
-void bound_items(const Params& p, Plan& pl, int64_t tiles, int64_t pieces, int least) {
-  pl.tiles = tiles;
-  pl.target = static_cast<int>(cdiv(pieces, p.Hkv));
-  pl.least = least;
-  if (p.ppr * kPage <= least) pl.target = 0;
-  pl.items = pl.tiles + pl.target;
+// The two kernels' cuts of a call.
+struct Plan {
+  Params few, wide;
+  bool both;  // the wide kernel runs too
+};
+
+void set_cut(Params& p, int rows_of, int lm, int start_cost, int64_t workgroups, int least) {
+  p.rows_of = rows_of;
+  p.lm = lm;
+  p.per_tile = static_cast<int>(cdiv(1 << lm, p.G));
+  p.start_cost = start_cost;
+  p.least = least;
+  // pieces: no more than the longest line that the tensors allow has of the least size
+  const int64_t tiles = p.T * p.G / (1 << lm) + (p.B < p.T ? p.B : p.T);
+  const int64_t line = tiles * (p.ppr * kPage + p.start_cost + p.per_tile);
+  int64_t n = workgroups / p.Hkv;
+  if (n > cdiv(line, least)) n = cdiv(line, least);
+  p.pieces = static_cast<int>(n < 1 ? 1 : n);
+  p.per_piece = 1.00002f / static_cast<float>(p.pieces);
 }
 
-int plan_of(const fade_paged_attn_args* a, Params& p, Plans& pl) {
+int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   const char* what = "fade_paged_attn";
   if (a == nullptr) return einval("%s: null args", what);
   if (a->D < 8 || a->D > 256 || a->D % 8)
@@ -787,7 +993,7 @@ int plan_of(const fade_paged_attn_args* a, Params& p, Plans& pl) {
   if (a->mask_mode != FADE_MASK_BOTTOM_RIGHT && a->mask_mode != FADE_MASK_NONE)
     return einval("%s: mask_mode must be FADE_MASK_BOTTOM_RIGHT or FADE_MASK_NONE, got %d", what, a->mask_mode);
   if (!(a->sm_scale > 0.0f) || !(a->sm_scale < INFINITY)) return einval("%s: sm_scale must be positive and finite", what);
-  p = Params{};
+  Params p{};
   p.B = a->B;
   p.T = a->T;
   p.ppr = a->pages_per_row;
@@ -813,69 +1019,47 @@ int plan_of(const fade_paged_attn_args* a, Params& p, Plans& pl) {
   // Rows whose matrix rows fit one tile of 16 go to the few-row kernel, the others
   // to the wide one; a call of at most 16 matrix rows per row on average is taken to
   // be a decoding step, all of it the few-row kernel's.
-  const int64_t rows = p.T * p.G, live = p.B < p.T ? p.B : p.T;
-  const bool step = rows <= kRows * p.B;
-  pl.few.M = kRows;
-  pl.few.rows_of = step ? kAll : kFew;
-  // sum_b ceil(n_b G / M) <= T G / M + (rows with new tokens); two workgroups' worth of work per CU, in pieces of 256 keys or more
-  bound_items(p, pl.few, step ? rows / kRows + live : live, 2 * num_cus(), 256);
-  if (!step) {
-    pl.wide.M = wide_rows(p.D);
-    pl.wide.rows_of = kMany;
-    const int64_t tiles = rows / pl.wide.M + live;
-    // no splits where whole tiles fill the chip several times over
-    bound_items(p, pl.wide, tiles, rows / pl.wide.M * p.Hkv >= 8 * num_cus() ? 0 : 2 * num_cus(), 512);
-  }
-  for (const Plan* k : {&pl.few, &pl.wide})
-    if (k->items * p.Hkv >= (1ll << 24)) return einval("%s: shape too large (%lld items of work)", what, (long long)(k->items * p.Hkv));
+  const bool step = p.T * p.G <= kRows * p.B;
+  pl.both = !step;
+  const int per_cu = p.D <= 64 ? 2 * FEW_PER_CU : (p.D <= 128 ? FEW_PER_CU : (FEW_PER_CU + 1) / 2);
+  pl.few = pl.wide = p;
+  set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), FEW_LEAST);
+  set_cut(pl.wide, kMany, kWideLog, WIDE_START, WIDE_PER_CU * num_cus(), 256);
+  pl.wide.zero_tail = 0;
   return FADE_OK;
 }
 
-int64_t part_rows(const Params& p, const Plan& pl) { return pl.target == 0 ? 0 : pl.items * p.Hkv * pl.M; }
-// (the kernels run one after the other: their sums lie in the same memory)
-int64_t part_rows(const Params& p, const Plans& pl) {
-  const int64_t a = part_rows(p, pl.few), b = part_rows(p, pl.wide);
-  return a > b ? a : b;
-}
-int64_t part_bytes(const Params& p, const Plans& pl) { return part_rows(p, pl) * (p.D * 4 + static_cast<int64_t>(sizeof(float2))); }
-
-void apply(Params& p, const Plan& pl) {
-  p.rows_of = pl.rows_of;
-  p.target = pl.target;
-  p.least = pl.least;
-  p.per_item = pl.target > 0 ? 1.00002f / static_cast<float>(pl.target) : 0.0f;
-  p.items = static_cast<uint32_t>(pl.items);
-}
-
-template <int M, bool BF>
-int merge(const Params& p, const Plan& pl, hipStream_t st) {
-  if (pl.target == 0) return FADE_OK;
-  const dim3 grid(static_cast<unsigned>(p.Hkv * pl.tiles), static_cast<unsigned>(cdiv(M, kThreads / (p.D / 4))));
-  hipLaunchKernelGGL((paged_merge_kernel<M, BF>), grid, dim3(kThreads), 0, st, p);
-  return check_launch("fade_paged_attn (merge)");
+int64_t part_rows(const Params& p) { return p.pieces < 2 ? 0 : static_cast<int64_t>(p.pieces) * p.Hkv * 2 << p.lm; }
+int64_t part_rows(const Plan& pl) { return part_rows(pl.few) + (pl.both ? part_rows(pl.wide) : 0); }
+int64_t cut_bytes(const Params& p) { return static_cast<int64_t>(p.pieces) * p.Hkv * static_cast<int64_t>(sizeof(int4)); }
+int64_t part_bytes(const Plan& pl) {
+  const int64_t n = part_rows(pl);
+  return n == 0 ? 0 : cut_bytes(pl.few) + cut_bytes(pl.wide) + n * (pl.few.D * 4 + static_cast<int64_t>(sizeof(float2)));
 }
 
 template <int DP, bool BF>
-int launch(Params& p, const Plans& pl, hipStream_t st) {
-  apply(p, pl.few);
-  hipLaunchKernelGGL((paged_few_kernel<DP, BF>), dim3(static_cast<unsigned>(p.Hkv * pl.few.items)), dim3(64 * Few<DP>::kWaves), 0, st, p);
-  int rc = check_launch("fade_paged_attn");
-  if (!rc) rc = merge<kRows, BF>(p, pl.few, st);
-  if (rc || pl.wide.M == 0) return rc;
-  typedef Wide<DP> W;
-  apply(p, pl.wide);
-  p.zero_tail = 0;
-  hipLaunchKernelGGL((paged_wide_kernel<DP, W::NW, W::MT, BF>), dim3(static_cast<unsigned>(p.Hkv * pl.wide.items)), dim3(64 * W::NW), 0, st, p);
-  rc = check_launch("fade_paged_attn");
-  return rc ? rc : merge<W::M, BF>(p, pl.wide, st);
+int launch(const Plan& pl, hipStream_t st) {
+  if (pl.both) {
+    typedef Wide<DP> W;
+    hipLaunchKernelGGL((paged_wide_kernel<DP, W::NW, W::MT, W::KT, W::NST, BF>), dim3(static_cast<unsigned>(pl.wide.Hkv * pl.wide.pieces)), dim3(64 * W::NW), 0, st, pl.wide);
+    const int rc = check_launch("fade_paged_attn");
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL((paged_few_kernel<DP, BF>), dim3(static_cast<unsigned>(pl.few.Hkv * pl.few.pieces)), dim3(64), 0, st, pl.few);
+  const int rc = check_launch("fade_paged_attn");
+  // (the last piece's tiles end in it)
+  const int first = pl.few.Hkv * (pl.few.pieces - 1) * kFewShares, second = pl.both ? pl.wide.Hkv * (pl.wide.pieces - 1) * kWideShares : 0;
+  if (rc || first + second == 0) return rc;
+  hipLaunchKernelGGL((paged_merge_kernel<BF>), dim3(static_cast<unsigned>(first + second)), dim3(kThreads), 0, st, pl.few, pl.wide, first);
+  return check_launch("fade_paged_attn (merge)");
 }
 
 template <bool BF>
-int launch_any(Params& p, const Plans& pl, void* stream) {
+int launch_any(const Plan& pl, void* stream) {
   hipStream_t st = as_stream(stream);
-  if (p.D <= 64) return launch<64, BF>(p, pl, st);
-  if (p.D <= 128) return launch<128, BF>(p, pl, st);
-  return launch<256, BF>(p, pl, st);
+  if (pl.few.D <= 64) return launch<64, BF>(pl, st);
+  if (pl.few.D <= 128) return launch<128, BF>(pl, st);
+  return launch<256, BF>(pl, st);
 }
 
 }  // namespace
@@ -887,26 +1071,29 @@ using namespace fade::paged;
 
 FADE_API int fade_paged_attn_workspace_bytes(const fade_paged_attn_args* a, int64_t* bytes) {
   if (bytes == nullptr) return einval("fade_paged_attn_workspace_bytes: null output");
-  Params p;
-  Plans pl;
-  const int rc = plan_of(a, p, pl);
+  Plan pl;
+  const int rc = plan_of(a, pl);
   if (rc) return rc;
-  *bytes = part_bytes(p, pl);
+  *bytes = part_bytes(pl);
   return FADE_OK;
 }
 
 FADE_API int fade_paged_attn(const fade_paged_attn_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
-  Params p;
-  Plans pl;
-  const int rc = plan_of(a, p, pl);
+  Plan pl;
+  const int rc = plan_of(a, pl);
   if (rc) return rc;
-  if (p.T == 0) return FADE_OK;
-  const int64_t need = part_bytes(p, pl);
+  if (a->T == 0) return FADE_OK;
+  const int64_t need = part_bytes(pl);
   if (need > 0) {
     if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
       return einval("fade_paged_attn: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
-    p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + part_rows(p, pl) * p.D);
+    const int64_t all = part_rows(pl), few = part_rows(pl.few);
+    pl.few.cuts = static_cast<int4*>(workspace);
+    pl.wide.cuts = pl.few.cuts + cut_bytes(pl.few) / sizeof(int4);
+    pl.few.part_o = reinterpret_cast<float*>(pl.wide.cuts + cut_bytes(pl.wide) / sizeof(int4));
+    pl.few.part_ml = reinterpret_cast<float2*>(pl.few.part_o + all * pl.few.D);
+    pl.wide.part_o = pl.few.part_o + few * pl.few.D;
+    pl.wide.part_ml = pl.few.part_ml + few;
   }
-  return a->dtype == FADE_DTYPE_BF16 ? launch_any<true>(p, pl, stream) : launch_any<false>(p, pl, stream);
+  return a->dtype == FADE_DTYPE_BF16 ? launch_any<true>(pl, stream) : launch_any<false>(pl, stream);
 }
