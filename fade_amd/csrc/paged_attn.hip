@@ -810,7 +810,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         for (int j = 0; j < 4; ++j) {
           const uint32_t pw = pa[mt][st][j];  // (a bit cast of a vector's element itself takes element 0)
           if constexpr (BF)
-            ps = __builtin_amdgcn_fdot2c_f32_bf16(__builtin_bit_cast(bf16x2, pw), (bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}), ps, false);
+            ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw), (bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}), ps, false);
           else
             ps = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pw), (f16x2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}), ps, false);
         }
