@@ -170,6 +170,7 @@ SLOTS_STATUS = {1: "more pages needed than are free", 2: "a row would pass its t
                 4: "more new tokens than n_tokens", 8: "a negative or impossible count"}
 
 ROPE_MAX_FREQS = 128
+ROPE_MAX_AXES = 4
 
 
 class RopeRows(ctypes.Structure):
@@ -182,10 +183,10 @@ class RopeArgs(ctypes.Structure):
 
     _fields_ = [
         ("B", _i64), ("S", _i64), ("D", _i64), ("Hq", _i64), ("Hkv", _i64), ("n_freqs", _i64),
-        ("dtype", _i32), ("inverse", _i32), ("pos64", _i32), ("reserved", _i32),
+        ("dtype", _i32), ("inverse", _i32), ("pos64", _i32), ("n_axes", _i32),
         ("positions", _p), ("pos_sa", _i64), ("pos_sb", _i64), ("pos_ss", _i64),
         ("q", RopeRows), ("k", RopeRows), ("v", RopeRows), ("slots", _p), ("n_pages", _i64),
-        ("turn", ctypes.c_uint64 * ROPE_MAX_FREQS), ("axis", ctypes.c_uint8 * ROPE_MAX_FREQS),
+        ("turn", _p), ("axis", _p),
     ]
 
 
@@ -305,22 +306,26 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
+_GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
     """An entry point of one argument struct, on the current stream of ``device`` (made the
     current device: the default stream's handle is the current device's)."""
-    fn = getattr(load(), name)
-    if device.index == torch.cuda.current_device():
-        check(fn(ctypes.byref(args), current_stream_handle(device)), name)
+    if device.index == _GET_DEVICE():
+        rc = getattr(_lib or load(), name)(ctypes.byref(args), current_stream_handle(device))
+        if rc:
+            check(rc, name)
         return
     with torch.cuda.device(device):
-        check(fn(ctypes.byref(args), current_stream_handle(device)), name)
+        check(getattr(load(), name)(ctypes.byref(args), current_stream_handle(device)), name)
 
 
 def no_gradient(op: str, *tensors: torch.Tensor | None) -> None:
     """Refuse a call that would have to record a gradient: the op has no backward pass."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            if torch.is_grad_enabled():
                 raise ValueError(f"{op}: has no backward pass (call it under torch.no_grad())")
 
 

@@ -26,6 +26,7 @@ constexpr int kThreads = 256;
 
 struct SlotParams {
   int B, ppr, n_tokens, cap;
+  int wide;  // table rows are whole aligned groups of four entries
   const int32_t* lens;
   const int32_t* fresh;
   const uint8_t* reset;
@@ -141,9 +142,8 @@ __global__ __launch_bounds__(kThreads) void page_slots_kernel(SlotParams p) {
 
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
-  const int64_t entries = static_cast<int64_t>(p.B) * p.ppr;
   if (fail) {  // nothing changes
-    for (int64_t e = first; e < entries; e += stride) p.table_out[e] = p.table[e];
+    for (int64_t e = first; e < static_cast<int64_t>(p.B) * p.ppr; e += stride) p.table_out[e] = p.table[e];
     for (int64_t t = first; t < p.n_tokens; t += stride) {
       p.slots[t] = -1;
       p.positions[t] = 0;
@@ -160,20 +160,37 @@ __global__ __launch_bounds__(kThreads) void page_slots_kernel(SlotParams p) {
   // free page number j from the head, place j behind the tail (sums below 2^32)
   const uint32_t cap = static_cast<uint32_t>(p.cap);
   auto taken = [&](int j) { return p.free_pages[(static_cast<uint32_t>(head) + static_cast<uint32_t>(j)) % cap]; };
-  for (int64_t e = first; e < entries; e += stride) {
-    const int b = static_cast<int>(e / p.ppr), j = static_cast<int>(e - static_cast<int64_t>(b) * p.ppr);
+  // The table: a workgroup takes a row's next 1024 (256) entries, four (one) a thread.
+  auto entry = [&](int j, int old, int have, int mine, int need0, int back0, bool again, int was) {
+    if (again && j < old) p.free_pages[(static_cast<uint64_t>(head) + count + back0 + j) % cap] = was;
+    return j >= have && j < have + mine ? taken(need0 + j - have) : (j < have ? was : 0);
+  };
+  const int span = p.wide ? 4 * kThreads : kThreads;
+  const int spans = (p.ppr + span - 1) / span;
+  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(p.B) * spans; item += gridDim.x) {
+    const int b = spans == 1 ? static_cast<int>(item) : static_cast<int>(item / spans);
+    const int j0 = (static_cast<int>(item) - b * spans) * span;
     const int raw = s_lens[b], old = pages_of(raw < 0 ? ~raw : raw), have = raw < 0 ? 0 : old;
-    const int mine = s_need[b + 1] - s_need[b];
-    int id = 0;
-    if (j < old) {
-      id = p.table[e];
-      if (raw < 0) {
-        p.free_pages[(static_cast<uint64_t>(head) + count + s_back[b] + j) % cap] = id;
-        id = 0;
+    const int need0 = s_need[b], mine = s_need[b + 1] - need0, back0 = s_back[b];
+    const int64_t at = static_cast<int64_t>(b) * p.ppr;
+    if (p.wide) {
+      const int j = j0 + 4 * tid;
+      if (j >= p.ppr) continue;
+      int4 was = make_int4(0, 0, 0, 0);
+      if (j < old) was = *reinterpret_cast<const int4*>(p.table + at + j);
+      int4 id = make_int4(0, 0, 0, 0);
+      if (j < old || j < have + mine) {
+        id.x = entry(j, old, have, mine, need0, back0, raw < 0, was.x);
+        id.y = entry(j + 1, old, have, mine, need0, back0, raw < 0, was.y);
+        id.z = entry(j + 2, old, have, mine, need0, back0, raw < 0, was.z);
+        id.w = entry(j + 3, old, have, mine, need0, back0, raw < 0, was.w);
       }
+      *reinterpret_cast<int4*>(p.table_out + at + j) = id;
+    } else {
+      const int j = j0 + tid;
+      if (j >= p.ppr) continue;
+      p.table_out[at + j] = entry(j, old, have, mine, need0, back0, raw < 0, j < old ? p.table[at + j] : 0);
     }
-    if (j >= have && j < have + mine) id = taken(s_need[b] + j - have);
-    p.table_out[e] = id;
   }
   for (int64_t t = first; t < p.n_tokens; t += stride) {
     int slot = -1, pos = 0;
@@ -243,11 +260,14 @@ FADE_API int fade_page_slots(const fade_page_slots_args* a, void* stream) {
   p.positions = a->positions;
   p.ring_out = a->ring_out;
   p.status = a->status;
-  const int64_t most = a->B * a->pages_per_row > a->n_tokens ? a->B * a->pages_per_row : a->n_tokens;
-  int64_t blocks = cdiv(most, kThreads);
+  p.wide = p.ppr % 4 == 0 && ((reinterpret_cast<uintptr_t>(a->table) | reinterpret_cast<uintptr_t>(a->table_out)) & 15) == 0;
+  const int64_t items = a->B * cdiv(p.ppr, p.wide ? 4 * kThreads : kThreads);
+  int64_t blocks = items > cdiv(a->n_tokens, kThreads) ? items : cdiv(a->n_tokens, kThreads);
   if (blocks > 2 * num_cus()) blocks = 2 * num_cus();
   const dim3 grid(static_cast<unsigned>(blocks));
+  // (the fewer rows an instance has, the less LDS it takes and the shorter its sums are)
   if (a->B <= 256) hipLaunchKernelGGL(page_slots_kernel<256>, grid, dim3(kThreads), 0, as_stream(stream), p);
+  else if (a->B <= 1024) hipLaunchKernelGGL(page_slots_kernel<1024>, grid, dim3(kThreads), 0, as_stream(stream), p);
   else hipLaunchKernelGGL(page_slots_kernel<FADE_SLOTS_MAX_ROWS>, grid, dim3(kThreads), 0, as_stream(stream), p);
   return check_launch("fade_page_slots");
 }

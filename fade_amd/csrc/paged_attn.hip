@@ -218,12 +218,14 @@ struct Walk {
   uint64_t x, end, piece;
   Place from;
   Row lane_row;     // the lane's row of rows 0 .. 63
+  int tokens;       // new tokens of all rows (p.zero_tail)
   Tile w;
   int lo, hi;       // the keys of the tile in this piece: lo to hi (of steps of `grain` keys)
   bool first, last; // the piece holds the tile's beginning, its end
 };
 __device__ __forceinline__ bool walk_start(const Params& p, int piece_index, Walk& k) {
   uint64_t all, piece;
+  k.tokens = p.zero_tail ? p.starts[p.B] : 0;
   line_of(p, all, piece, k.lane_row);
   k.x = piece * static_cast<uint64_t>(piece_index);
   k.end = k.x + piece < all ? k.x + piece : all;
@@ -253,8 +255,7 @@ __device__ __forceinline__ bool walk_next(const Params& p, int grain, Walk& k) {
 }
 
 // Rows of q past the last sequence: zeros, where the caller asked for them.
-__device__ __forceinline__ void zero_tail(const Params& p, int64_t block, int64_t blocks, int kvh) {
-  int end = p.starts[p.B];
+__device__ __forceinline__ void zero_tail(const Params& p, int end, int64_t block, int64_t blocks, int kvh) {
   end = end < 0 ? 0 : end;
   const int G = p.G;
   for (int64_t t = end + block; t < p.T; t += blocks)
@@ -265,16 +266,19 @@ __device__ __forceinline__ void zero_tail(const Params& p, int64_t block, int64_
 // The end of a workgroup.  What the second launch has to join: the piece's last
 // tile, if it begins here and ends elsewhere.
 __device__ __forceinline__ void finish(const Params& p, const Walk& k, bool any) {
-  if (p.zero_tail) zero_tail(p, blockIdx.x / p.Hkv, gridDim.x / p.Hkv, blockIdx.x % p.Hkv);
+  if (p.zero_tail) zero_tail(p, k.tokens, blockIdx.x / p.Hkv, gridDim.x / p.Hkv, blockIdx.x % p.Hkv);
   if (p.pieces < 2 || threadIdx.x != 0) return;
   int parts = 0;
   if (any && k.first && !k.last) {
     const uint64_t rest = k.w.at + k.w.cost - k.end;  // > 0: in the next pieces
-    parts = 1;
-    for (uint64_t at = 0; at < rest && parts < p.pieces; at += k.piece) ++parts;
+    parts = static_cast<int>(static_cast<double>(rest) / static_cast<double>(k.piece));  // (a whole number or two off)
+    if (parts > 0) --parts;
+    while (k.piece * static_cast<uint64_t>(parts) < rest && parts < p.pieces) ++parts;
+    ++parts;
   }
   p.cuts[blockIdx.x] = make_int4(k.w.q0, k.w.tile << p.lm, k.w.n * p.G, parts);
 }
+
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (BF)
@@ -306,36 +310,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // 16-byte unit u of LDS row r lies at unit u ^ (2 (r & 7)) (mod the row), which the
 // loads' source addresses bring about: without it the 16 rows that a transposing
 // read touches would share their banks.
-#ifndef FEW_STAGES
-#define FEW_STAGES 2
-#endif
-#ifndef FEW_PER_CU
-#define FEW_PER_CU 4
-#endif
-#ifndef AHEAD256
-#define AHEAD256 2
-#endif
-#ifndef SCHEDB
-#define SCHEDB 0x6
-#endif
-#ifndef WIDE_ST
-#define WIDE_ST 3
-#endif
-#ifndef WIDE_ST256
-#define WIDE_ST256 4
-#endif
-#ifndef FEW_LEAST
-#define FEW_LEAST 64
-#endif
-#ifndef WIDE_NW
-#define WIDE_NW 8
-#endif
-#ifndef WIDE_START
-#define WIDE_START 192
-#endif
-#ifndef WIDE_PER_CU
-#define WIDE_PER_CU 1
-#endif
 template <int DP>
 struct Few {
   static constexpr int kKeys = 32;                 // keys per step
@@ -343,7 +317,7 @@ struct Few {
   static constexpr int kTensor = kKeys * DP * 2;   // bytes of a step's K or V
   static constexpr int kStage = 2 * kTensor;
   static constexpr int kLoads = kStage / 1024;     // direct loads per step
-  static constexpr int kStages = FEW_STAGES;
+  static constexpr int kStages = 2;
   static constexpr int kQBytes = kRows * DP * 2;
   static constexpr int kLds = kStages * kStage + kQBytes;
   static constexpr int kSwizzle = kUnits - 1;
@@ -731,7 +705,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (ahead < k.hi) issue_next(buf == 0 ? NST - 1 : buf - 1);
     if (key >= whi) continue;  // (to flip())
     // fragments are read AH ahead of their products
-    constexpr int AH = DP > 128 ? AHEAD256 : 4;
+    constexpr int AH = DP > 128 ? 2 : 4;
+    constexpr int kCompute = 0x6;  // (vector and scalar arithmetic may pass, reads and products keep their order)
     auto k_frag = [&](int f) { return lds_read16((kat ^ (32 * (f % NKS % KA))) + 32 * (f / NKS) * DP * 2 + 256 * (f % NKS / KA)); };
     auto v_frag = [&](int f) {
       const uint32_t at = (vat ^ (64 * (f % NCB % VA))) + 16 * (f / NCB) * DP * 2 + 256 * (f % NCB / VA);
@@ -743,7 +718,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       u32x4 kf[AH];
 #pragma unroll
       for (int f = 0; f < AH; ++f) kf[f] = k_frag(f);
-      __builtin_amdgcn_sched_barrier(SCHEDB);
+      __builtin_amdgcn_sched_barrier(kCompute);
 #pragma unroll
       for (int f = 0; f < NKS * NKB; ++f) {
         const u32x4 a = kf[f % AH];
@@ -756,7 +731,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
           }
           s[mt][f / NKS] = mfma32<BF>(a, qf[mt][f % NKS], s[mt][f / NKS]);
         }
-        __builtin_amdgcn_sched_barrier(SCHEDB);
+        __builtin_amdgcn_sched_barrier(kCompute);
       }
     }
     u32x4 pa[MT][2 * NKB];
@@ -820,14 +795,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       u32x4 vf[AH];
 #pragma unroll
       for (int f = 0; f < AH; ++f) vf[f] = v_frag(f);
-      __builtin_amdgcn_sched_barrier(SCHEDB);
+      __builtin_amdgcn_sched_barrier(kCompute);
 #pragma unroll
       for (int f = 0; f < 2 * NKB * NCB; ++f) {
         const u32x4 a = vf[f % AH];
         if (f + AH < 2 * NKB * NCB) vf[f % AH] = v_frag(f + AH);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) acc[mt][f % NCB] = mfma32<BF>(a, pa[mt][f / NCB], acc[mt][f % NCB]);
-        __builtin_amdgcn_sched_barrier(SCHEDB);
+        __builtin_amdgcn_sched_barrier(kCompute);
       }
     }
   }
@@ -871,32 +846,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
 // Tiles that a piece's border cuts, their parts joined in the order of the keys:
 // the beginning in piece `index` of the kv head, ends in the pieces after it.
-// D / 4 threads per matrix row; of a tile of many parts the threads left over take
-// a share each, whose sums are added up through LDS in a fixed order.
-template <bool BF>
-__device__ __forceinline__ void merge_tile(const Params& p, int block, int row0, int row_step) {
-  const int4 cut = p.cuts[block];
+// D / 4 threads per matrix row; of a tile of four parts or more four times as many,
+// each with a share of the parts, whose sums are added up through LDS in a fixed order.
+template <bool BF, int SHARES>
+__device__ __forceinline__ void merge_rows(const Params& p, int block, const int4 cut, int row0, int row_step, f32x4* so, float2* sml) {
   const int parts = cut.w;
-  if (parts < 2) return;
   const int kvh = block % p.Hkv, M = 1 << p.lm;
   const int rows = cut.z - cut.y < M ? cut.z - cut.y : M;
-  const int tpr = p.D / 4, groups = kThreads / tpr;
-  const int grp = threadIdx.x / tpr, c = 4 * (threadIdx.x % tpr);
-  const int per_row = parts >= 8 ? (groups < 8 ? groups : 8) : 1;  // threads' groups per row
-  const int rows_at_once = groups / per_row, sub = grp % per_row;
-  const bool in = grp < rows_at_once * per_row;
-  __shared__ f32x4 so[kThreads];
-  __shared__ float2 sml[kThreads];
+  const int tpr = p.D / 4, rows_at_once = kThreads / tpr / SHARES;
+  const int grp = threadIdx.x / tpr, c = 4 * (threadIdx.x % tpr), sub = grp % SHARES;
   auto at = [&](int i, int row) { return ((static_cast<int64_t>(block) + static_cast<int64_t>(i) * p.Hkv) * 2 + (i == 0 ? 1 : 0)) * M + row; };
   for (int rb = row0 * rows_at_once; rb < rows; rb += row_step * rows_at_once) {
-    const int row = rb + grp / per_row;
-    const bool mine = in && row < rows;
+    const int row = rb + grp / SHARES;
+    const bool mine = grp < rows_at_once * SHARES && row < rows;
     float mx = -INFINITY, sum = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     if (mine) {
       // a running maximum, as in the kernels: the parts' loads do not wait for it
 #pragma unroll 4
-      for (int i = sub; i < parts; i += per_row) {
+      for (int i = sub; i < parts; i += SHARES) {
         const float2 ml = p.part_ml[at(i, row)];
         const f32x4 a = *reinterpret_cast<const f32x4*>(p.part_o + at(i, row) * p.D + c);
         const float mn = fmaxf(mx, ml.x), ms = mn == -INFINITY ? 0.0f : mn;
@@ -906,22 +874,28 @@ __device__ __forceinline__ void merge_tile(const Params& p, int block, int row0,
         o = o * f0 + a * f1;
       }
     }
-    if (per_row > 1) {
+    if constexpr (SHARES > 1) {
       __syncthreads();
       so[threadIdx.x] = o;
       sml[threadIdx.x] = make_float2(mx, sum);
       __syncthreads();
       if (mine && sub == 0) {
-        float mm = mx;
-        for (int i = 1; i < per_row; ++i) mm = fmaxf(mm, sml[threadIdx.x + i * tpr].x);
-        const float ms = mm == -INFINITY ? 0.0f : mm;
+        float2 ml[SHARES];
+        f32x4 a[SHARES];
+#pragma unroll
+        for (int i = 0; i < SHARES; ++i) {
+          ml[i] = sml[threadIdx.x + i * tpr];
+          a[i] = so[threadIdx.x + i * tpr];
+          mx = fmaxf(mx, ml[i].x);
+        }
+        const float ms = mx == -INFINITY ? 0.0f : mx;
         sum = 0.0f;
         o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < per_row; ++i) {
-          const float2 ml = sml[threadIdx.x + i * tpr];
-          const float f = __builtin_amdgcn_exp2f(ml.x - ms);
-          sum += ml.y * f;
-          o += so[threadIdx.x + i * tpr] * f;
+#pragma unroll
+        for (int i = 0; i < SHARES; ++i) {
+          const float f = __builtin_amdgcn_exp2f(ml[i].x - ms);
+          sum += ml[i].y * f;
+          o += a[i] * f;
         }
       }
     }
@@ -933,23 +907,32 @@ __device__ __forceinline__ void merge_tile(const Params& p, int block, int row0,
     }
   }
 }
+template <bool BF>
+__device__ __forceinline__ void merge_tile(const Params& p, int block, int row0, int row_step) {
+  const int4 cut = p.cuts[block];
+  if (cut.w < 2) return;
+  __shared__ f32x4 so[kThreads];
+  __shared__ float2 sml[kThreads];
+  if (cut.w < 4) merge_rows<BF, 1>(p, block, cut, row0, row_step, so, sml);
+  else merge_rows<BF, 4>(p, block, cut, row0, row_step, so, sml);  // (D / 4 threads four times fit a block)
+}
 
-// Four blocks per piece of the few-row kernel, then eight per piece of the wide one.
-constexpr int kFewShares = 4, kWideShares = 8;
+// Eight blocks per piece of the few-row kernel, then eight per piece of the wide one.
+constexpr int kFewBlocks = 8, kWideBlocks = 8;
 template <bool BF>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(Params a, Params b, int first_blocks) {
   const int i = blockIdx.x, j = i - first_blocks;
-  if (j < 0) merge_tile<BF>(a, i / kFewShares, i % kFewShares, kFewShares);
-  else merge_tile<BF>(b, j / kWideShares, j % kWideShares, kWideShares);
+  if (j < 0) merge_tile<BF>(a, i / kFewBlocks, i % kFewBlocks, kFewBlocks);
+  else merge_tile<BF>(b, j / kWideBlocks, j % kWideBlocks, kWideBlocks);
 }
 
 bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
 
 template <int DP>
 struct Wide {  // waves, blocks of 32 rows per wave, keys per step
-  static constexpr int NW = WIDE_NW, MT = 1, M = 32 * NW * MT, KT = DP > 128 ? 32 : 64, NST = DP > 128 ? WIDE_ST256 : WIDE_ST;
+  static constexpr int NW = 8, MT = 1, M = 32 * NW * MT, KT = DP > 128 ? 32 : 64, NST = DP > 128 ? 4 : 3;
 };
-constexpr int kWideLog = WIDE_NW == 8 ? 8 : 7;
+constexpr int kWideLog = 8;
 
 // The two kernels' cuts of a call.
 struct Plan {
@@ -980,7 +963,7 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   if (a->B < 1 || a->T < 0 || a->Hq < 1 || a->Hkv < 1 || a->n_pages < 1 || a->pages_per_row < 1)
     return einval("%s: B, Hq, Hkv, n_pages and pages_per_row must be positive, T not negative", what);
   if (a->Hq % a->Hkv) return einval("%s: needs Hq %% Hkv == 0 (got %lld/%lld)", what, (long long)a->Hq, (long long)a->Hkv);
-  if (a->B > (1 << 20) || a->T > (1 << 24) || a->Hq > 65535 || a->T * (a->Hq / a->Hkv) >= (1ll << 31) ||
+  if (a->B > (1 << 20) || a->T > (1 << 24) || a->Hq > 65535 || a->T * (a->Hq / a->Hkv) >= (1ll << 30) ||
       a->pages_per_row > (1 << 24) || a->n_pages >= (1ll << 31))
     return einval("%s: shape too large", what);
   if (a->T > 0 && (!a->q || !a->out)) return einval("%s: null q or out", what);
@@ -1021,10 +1004,10 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   // be a decoding step, all of it the few-row kernel's.
   const bool step = p.T * p.G <= kRows * p.B;
   pl.both = !step;
-  const int per_cu = p.D <= 64 ? 2 * FEW_PER_CU : (p.D <= 128 ? FEW_PER_CU : (FEW_PER_CU + 1) / 2);
+  const int per_cu = p.D <= 64 ? 8 : (p.D <= 128 ? 4 : 2);
   pl.few = pl.wide = p;
-  set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), FEW_LEAST);
-  set_cut(pl.wide, kMany, kWideLog, WIDE_START, WIDE_PER_CU * num_cus(), 256);
+  set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), 64);
+  set_cut(pl.wide, kMany, kWideLog, 192, num_cus(), 256);
   pl.wide.zero_tail = 0;
   return FADE_OK;
 }
@@ -1048,7 +1031,7 @@ int launch(const Plan& pl, hipStream_t st) {
   hipLaunchKernelGGL((paged_few_kernel<DP, BF>), dim3(static_cast<unsigned>(pl.few.Hkv * pl.few.pieces)), dim3(64), 0, st, pl.few);
   const int rc = check_launch("fade_paged_attn");
   // (the last piece's tiles end in it)
-  const int first = pl.few.Hkv * (pl.few.pieces - 1) * kFewShares, second = pl.both ? pl.wide.Hkv * (pl.wide.pieces - 1) * kWideShares : 0;
+  const int first = pl.few.Hkv * (pl.few.pieces - 1) * kFewBlocks, second = pl.both ? pl.wide.Hkv * (pl.wide.pieces - 1) * kWideBlocks : 0;
   if (rc || first + second == 0) return rc;
   hipLaunchKernelGGL((paged_merge_kernel<BF>), dim3(static_cast<unsigned>(first + second)), dim3(kThreads), 0, st, pl.few, pl.wide, first);
   return check_launch("fade_paged_attn (merge)");

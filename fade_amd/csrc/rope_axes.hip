@@ -16,8 +16,10 @@
 //
 // Bound by HBM: every row is read and written once.  A thread keeps one token's
 // V = 16 bytes' worth of frequencies (their sines and cosines in registers) and
-// walks the heads with them, so the trigonometry is paid once per workgroup's
-// heads and a wave's access covers whole 128-byte runs of the rows.
+// walks the heads of its workgroup's tensor with them, so the trigonometry is paid
+// once per workgroup's heads and a wave's access covers whole 128-byte runs of the
+// rows.  Calls of few tokens are bound by latency: no load waits for another one
+// but for its address in the arguments.
 #include "fade_common.h"
 
 namespace fade {
@@ -37,17 +39,18 @@ struct Rows {
 struct RopeParams {
   int64_t tokens, S;  // B * S of them
   int D, half;        // channels of a row, rotated pairs
-  int Hq, Hkv, Hv;    // heads of q, k, v (v only in an append)
+  int heads[3];       // of q, k, v (v only in an append)
+  int first_group[3]; // of each tensor's heads in the grid's second dimension
   int heads_per_block;
   int inverse, append;
   const void* pos;    // axis a of token (b, s) at a * pos_sa + b * pos_sb + s * pos_ss
   int64_t pos_sa, pos_sb, pos_ss;
-  int pos64;
-  Rows q, k, v;       // append: k.dst, v.dst are pages [n_pages][Hkv][64][D]
+  int pos64, axes;
+  Rows rows[3];       // append: k's and v's dst are pages [n_pages][Hkv][64][D]
   const int32_t* slots;
   int64_t n_pages;
-  uint64_t turn[FADE_ROPE_MAX_FREQS];
-  uint8_t axis[FADE_ROPE_MAX_FREQS];
+  const uint64_t* turn;  // [half], in device memory: as arguments they cost 1 to 2 us a launch (1187 tokens 8.9 us, now 6.7)
+  const uint8_t* axis;
 };
 
 // sine and cosine of an angle in turns
@@ -72,62 +75,92 @@ struct alignas(V * sizeof(T)) Vec {
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
   typedef Vec<T, V> Vt;
-  const int units = p.D / (2 * V);
-  const int per_block = kThreads / units;
-  const int u = threadIdx.x % units;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * per_block + threadIdx.x / units;
-  if (threadIdx.x >= per_block * units || t >= p.tokens) return;
-  const int64_t b = t / p.S, s = t - b * p.S;
+  // a workgroup has heads of one tensor
+  const int which = blockIdx.y >= static_cast<unsigned>(p.first_group[2]) ? 2 : (blockIdx.y >= static_cast<unsigned>(p.first_group[1]) ? 1 : 0);
+  const Rows& r = p.rows[which];
+  const unsigned units = static_cast<unsigned>(p.D) / (2 * V);
+  const unsigned per_block = kThreads / units, lrow = threadIdx.x / units;
+  const int u = static_cast<int>(threadIdx.x - lrow * units);
+  const uint32_t t = blockIdx.x * per_block + lrow;  // (tokens < 2^31)
+  if (lrow >= per_block || t >= static_cast<uint32_t>(p.tokens)) return;
+  const uint32_t b = t / static_cast<uint32_t>(p.S), s = t - b * static_cast<uint32_t>(p.S);
   const int rot_units = p.half / V;
   const bool rot = u < rot_units;
   const int c0 = rot ? V * u : 2 * p.half + 2 * V * (u - rot_units);  // the unit's first channel
   const int c1 = rot ? c0 + p.half : c0 + V;                          // and the first of its other V
 
+  const int h0 = (static_cast<int>(blockIdx.y) - p.first_group[which]) * p.heads_per_block;
+  const int h1 = h0 + p.heads_per_block < p.heads[which] ? h0 + p.heads_per_block : p.heads[which];
+  const bool paged = p.append && which > 0;
+  const T* src = static_cast<const T*>(r.src) + b * r.s_sb + h0 * r.s_sh + s * r.s_ss;
+  // the loads do not wait for one another: the first head's row, the slot, positions on every axis, the frequencies
+  Vt x = *reinterpret_cast<const Vt*>(src + c0), y = *reinterpret_cast<const Vt*>(src + c1);
+  int32_t slot = 0;
+  if (paged) slot = p.slots[t];
   float sn[V], cs[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     sn[i] = 0.0f;
     cs[i] = 1.0f;
-    if (rot && p.pos != nullptr) {
-      const int f = c0 + i;
-      const int64_t at = p.axis[f] * p.pos_sa + b * p.pos_sb + s * p.pos_ss;
-      const int64_t ps = p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : static_cast<const int32_t*>(p.pos)[at];
-      const uint64_t a = static_cast<uint64_t>(ps) * p.turn[f];
+  }
+  if (p.pos != nullptr && which < 2) {
+    const int64_t at = b * p.pos_sb + s * p.pos_ss;
+    int64_t pos[FADE_ROPE_MAX_AXES];
+    if (p.pos64) {
+#pragma unroll
+      for (int k = 0; k < FADE_ROPE_MAX_AXES; ++k) pos[k] = static_cast<const int64_t*>(p.pos)[at + (k < p.axes ? k : 0) * p.pos_sa];
+    } else {
+#pragma unroll
+      for (int k = 0; k < FADE_ROPE_MAX_AXES; ++k) pos[k] = static_cast<const int32_t*>(p.pos)[at + (k < p.axes ? k : 0) * p.pos_sa];
+    }
+    const int f0 = rot ? c0 : 0;
+    uint64_t turn[V];
+    uint32_t ax[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      turn[i] = p.turn[f0 + i];
+      ax[i] = p.axis[f0 + i];
+    }
+    const float sign = p.inverse ? -1.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      int64_t ps = pos[0];
+#pragma unroll
+      for (int k = 1; k < FADE_ROPE_MAX_AXES; ++k) ps = ax[i] == k ? pos[k] : ps;
+      const uint64_t a = static_cast<uint64_t>(ps) * turn[i];
       sincos_turns<T>(static_cast<float>(static_cast<int32_t>(a >> 32)) * 0x1p-32f, sn[i], cs[i]);
-      if (p.inverse) sn[i] = -sn[i];
+      sn[i] *= sign;
     }
   }
-  int64_t page = 0, off = 0;
-  bool store = true;
-  if (p.append) {
-    const int32_t slot = p.slots[t];
-    page = slot / kPage;
-    off = slot % kPage;
-    store = slot >= kPage && page < p.n_pages;  // page 0 holds no tokens
+  T* dst = static_cast<T*>(r.dst);
+  int64_t d_sh = r.d_sh;
+  if (paged) {
+    const int32_t page = slot / kPage, off = slot % kPage;
+    if (slot < kPage || page >= p.n_pages) return;  // no place (page 0 holds no tokens)
+    d_sh = static_cast<int64_t>(kPage) * p.D;
+    dst += (static_cast<int64_t>(page) * p.heads[which] + h0) * d_sh + off * p.D;
+  } else {
+    dst += b * r.d_sb + h0 * d_sh + s * r.d_ss;
   }
-  const int h0 = blockIdx.y * p.heads_per_block, all = p.Hq + p.Hkv + p.Hv;
-  const int h1 = h0 + p.heads_per_block < all ? h0 + p.heads_per_block : all;
-#pragma unroll 4
   for (int hh = h0; hh < h1; ++hh) {
-    const bool is_q = hh < p.Hq, is_k = !is_q && hh < p.Hq + p.Hkv;
-    const Rows& r = is_q ? p.q : (is_k ? p.k : p.v);
-    const int h = is_q ? hh : (is_k ? hh - p.Hq : hh - p.Hq - p.Hkv);
-    const bool paged = p.append && !is_q;
-    if (paged && !store) continue;
-    const T* src = static_cast<const T*>(r.src) + b * r.s_sb + h * r.s_sh + s * r.s_ss;
-    T* dst = static_cast<T*>(r.dst) + (paged ? ((page * p.Hkv + h) * kPage + off) * p.D : b * r.d_sb + h * r.d_sh + s * r.d_ss);
-    const Vt x = *reinterpret_cast<const Vt*>(src + c0), y = *reinterpret_cast<const Vt*>(src + c1);
     Vt a = x, c = y;
-    if (rot && (is_q || is_k)) {
+    if (hh + 1 < h1) {  // the next head's row
+      src += r.s_sh;
+      x = *reinterpret_cast<const Vt*>(src + c0);
+      y = *reinterpret_cast<const Vt*>(src + c1);
+    }
+    if (rot && which < 2) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xf = to_f32(x.e[i]), yf = to_f32(y.e[i]);
-        a.e[i] = from_f32<T>(xf * cs[i] - yf * sn[i]);
-        c.e[i] = from_f32<T>(yf * cs[i] + xf * sn[i]);
+      for (int e = 0; e < V; ++e) {
+        const float xf = to_f32(a.e[e]), yf = to_f32(c.e[e]);
+        // (as they stand: the same operations in every instance)
+        a.e[e] = from_f32<T>(__fmaf_rn(xf, cs[e], -__fmul_rn(yf, sn[e])));
+        c.e[e] = from_f32<T>(__fmaf_rn(yf, cs[e], __fmul_rn(xf, sn[e])));
       }
     }
     *reinterpret_cast<Vt*>(dst + c0) = a;
     *reinterpret_cast<Vt*>(dst + c1) = c;
+    dst += d_sh;
   }
 }
 
@@ -136,13 +169,18 @@ int rope_launch(RopeParams& p, bool wide, void* stream) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   const int units = p.D / (2 * (wide ? V : 1));
   const int64_t bx = cdiv(p.tokens, kThreads / units);
-  const int all = p.Hq + p.Hkv + p.Hv;
-  // heads are spread over workgroups while there are fewer than four per CU
+  const int all = p.heads[0] + p.heads[1] + p.heads[2];
+  // heads are spread over workgroups while there are fewer than two per CU (16384 tokens x 40 heads, one, two, four
+  // per CU: 67.8, 66.5, 73.9 us; 1187 x 32: 9.5, 8.9, 10.0)
   int split = 1;
-  while (bx * split < 4 * num_cus() && split < all) split *= 2;
-  if (split > all) split = all;
+  while (bx * split < 2 * num_cus() && split < all) split *= 2;
   p.heads_per_block = static_cast<int>(cdiv(all, split));
-  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(cdiv(all, p.heads_per_block)));
+  int groups = 0;
+  for (int i = 0; i < 3; ++i) {
+    p.first_group[i] = groups;
+    groups += static_cast<int>(cdiv(p.heads[i], p.heads_per_block));
+  }
+  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(groups));
   if (wide) hipLaunchKernelGGL((rope_kernel<T, V>), grid, dim3(kThreads), 0, as_stream(stream), p);
   else hipLaunchKernelGGL((rope_kernel<T, 1>), grid, dim3(kThreads), 0, as_stream(stream), p);
   return check_launch("fade_rope_axes");
@@ -153,10 +191,11 @@ int rope_any(const fade_rope_args* a, bool append, const char* what, void* strea
   if (a->dtype != FADE_DTYPE_F16 && a->dtype != FADE_DTYPE_BF16 && (append || a->dtype != FADE_DTYPE_F32))
     return einval("%s: unknown dtype %d", what, a->dtype);
   if (a->D < 2 || a->D > 2 * FADE_ROPE_MAX_FREQS || a->D % 2) return einval("%s: head_dim must be even, 2 to 256, got %lld", what, (long long)a->D);
+  if (a->n_axes < 1 || a->n_axes > FADE_ROPE_MAX_AXES) return einval("%s: 1 to %d axes, got %d", what, FADE_ROPE_MAX_AXES, a->n_axes);
   if (a->n_freqs < 0 || 2 * a->n_freqs > a->D) return einval("%s: %lld frequencies for head_dim %lld", what, (long long)a->n_freqs, (long long)a->D);
   if (a->B < 0 || a->S < 0 || a->Hq < 0 || a->Hkv < 0 || a->Hq > 65535 || a->Hkv > 65535) return einval("%s: bad shape", what);
   if (append && a->B > 1) return einval("%s: tokens come as one row", what);
-  if (a->S != 0 && a->B > (1ll << 31) / a->S) return einval("%s: shape too large", what);
+  if (a->S != 0 && a->B >= (1ll << 31) / a->S) return einval("%s: shape too large", what);
   const int64_t tokens = a->B * a->S;
   if (tokens == 0 || a->Hq + a->Hkv == 0) return FADE_OK;
   if ((a->Hq > 0 && (!a->q.src || !a->q.dst)) || (a->Hkv > 0 && (!a->k.src || !a->k.dst))) return einval("%s: null q or k", what);
@@ -168,22 +207,22 @@ int rope_any(const fade_rope_args* a, bool append, const char* what, void* strea
   p.S = a->S;
   p.D = static_cast<int>(a->D);
   p.half = static_cast<int>(a->n_freqs);
-  p.Hq = static_cast<int>(a->Hq);
-  p.Hkv = static_cast<int>(a->Hkv);
-  p.Hv = append ? p.Hkv : 0;
+  p.heads[0] = static_cast<int>(a->Hq);
+  p.heads[1] = static_cast<int>(a->Hkv);
+  p.heads[2] = append ? p.heads[1] : 0;
   p.inverse = a->inverse;
   p.append = append;
-  p.pos = a->positions;
+  p.pos = p.half > 0 ? a->positions : nullptr;
   p.pos_sa = a->pos_sa;
   p.pos_sb = a->pos_sb;
   p.pos_ss = a->pos_ss;
   p.pos64 = a->pos64;
+  p.axes = a->n_axes;
   p.slots = a->slots;
   p.n_pages = a->n_pages;
-  for (int i = 0; i < p.half; ++i) {
-    p.turn[i] = a->turn[i];
-    p.axis[i] = a->axis[i];
-  }
+  if (p.half > 0 && p.pos != nullptr && (!a->turn || !a->axis)) return einval("%s: null turn or axis", what);
+  p.turn = a->turn;
+  p.axis = a->axis;
   // 16-byte accesses: whole units of both halves and aligned rows
   const int V = a->dtype == FADE_DTYPE_F32 ? 4 : 8, size = 16 / V;
   bool wide = p.D % (2 * V) == 0 && p.half % V == 0;
@@ -195,9 +234,9 @@ int rope_any(const fade_rope_args* a, bool append, const char* what, void* strea
     if (m % 16) wide = false;
     return r;
   };
-  if (p.Hq) p.q = rows(a->q, false);
-  if (p.Hkv) p.k = rows(a->k, append);
-  if (p.Hv) p.v = rows(a->v, append);
+  if (p.heads[0]) p.rows[0] = rows(a->q, false);
+  if (p.heads[1]) p.rows[1] = rows(a->k, append);
+  if (p.heads[2]) p.rows[2] = rows(a->v, append);
   if (a->dtype == FADE_DTYPE_F16) return rope_launch<uint16_t>(p, wide, stream);
   if (a->dtype == FADE_DTYPE_BF16) return rope_launch<Bf16>(p, wide, stream);
   return rope_launch<float>(p, wide, stream);

@@ -73,33 +73,35 @@ def paged_append(
         raise ValueError(f"{op}: q_out must be like q with a contiguous head_dim axis")
     if scheme is None:
         a = _lib.RopeArgs()
+        a.n_axes = 1
     else:
-        a = rope_args(scheme, D, op)
+        a = rope_args(scheme, D, k.device, op)
         if positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{op}: positions must be int32 or int64, got {positions.dtype}")
-        if positions.dim() not in (1, 2) or positions.shape[-1] != T or (positions.dim() == 2 and positions.shape[0] not in (1, scheme.n_axes)):
+        if positions.dim() not in (1, 2) or positions.shape[-1] != T or (positions.dim() == 2 and positions.shape[0] not in (1, a.n_axes)):
             raise ValueError(f"{op}: positions must be [{T}] or [{scheme.n_axes}, {T}], got {tuple(positions.shape)}")
         a.positions, a.pos64, a.pos_ss = positions.data_ptr(), int(positions.dtype == torch.int64), positions.stride(-1)
         a.pos_sa = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
     a.B, a.S, a.D, a.Hkv, a.dtype = 1, T, D, Hkv, dtc
     a.slots, a.n_pages = slots.data_ptr(), n_pages
     keep = []
+
+    def rows(t: Tensor, dst: int, sh: int = 0, ss: int = 0):
+        st = t.stride()
+        if st[2] != 1 or t.is_neg():
+            t = t.resolve_neg().contiguous()
+            st = t.stride()
+            keep.append(t)
+        return _lib.RopeRows(t.data_ptr(), dst, 0, st[1], st[0], 0, sh, ss)
+
     if q is not None:
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         else:
             _lib.written(op, q_out)
-        a.Hq = q.shape[1]
-        a.q.dst, a.q.dst_sh, a.q.dst_ss = q_out.data_ptr(), q_out.stride(1), q_out.stride(0)
-    for r, t in ((a.q, q), (a.k, k), (a.v, v)):
-        if t is None:
-            continue
-        if t.is_neg() or t.stride(2) != 1:
-            t = t.resolve_neg().contiguous()
-            keep.append(t)
-        r.src, r.src_sh, r.src_ss = t.data_ptr(), t.stride(1), t.stride(0)
+        a.Hq, a.q = q.shape[1], rows(q, q_out.data_ptr(), q_out.stride(1), q_out.stride(0))
+    a.k, a.v = rows(k, k_pages.data_ptr()), rows(v, v_pages.data_ptr())
     _lib.written(op, k_pages, v_pages)
-    a.k.dst, a.v.dst = k_pages.data_ptr(), v_pages.data_ptr()
     _lib.launch("fade_paged_append", a, k.device)
     return q_out
 

@@ -220,34 +220,35 @@ def page_slots(
     _lib.require_gpu(lens, new, table, free, ring, reset, op=op)
     if table.dim() != 2:
         raise ValueError(f"{op}: table must be [B, pages_per_row], got {tuple(table.shape)}")
-    B, ppr = (int(x) for x in table.shape)
-    n = int(n_tokens)
+    B, ppr = table.shape
+    n, n_free, i32 = int(n_tokens), free.numel(), torch.int32
     if n < 0:
         raise ValueError(f"{op}: n_tokens must be >= 0, got {n}")
-    for name, t, shape in (("lens", lens, (B,)), ("new", new, (B,)), ("table", table, (B, ppr)), ("free", free, (free.numel(),)),
-                           ("ring", ring, (2,))):
-        if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} {list(t.shape)}")
-    if reset is not None and (reset.dtype not in (torch.bool, torch.uint8) or tuple(reset.shape) != (B,) or not reset.is_contiguous()):
+    for name, t, size in (("lens", lens, B), ("new", new, B), ("table", table, B * ppr), ("free", free, n_free), ("ring", ring, 2)):
+        if t.dtype is not i32 or t.numel() != size or not t.is_contiguous() or (t.dim() != 1 and t is not table):
+            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of {size} elements, got {t.dtype} {list(t.shape)}")
+    if reset is not None and (reset.dtype not in (torch.bool, torch.uint8) or reset.shape != (B,) or not reset.is_contiguous()):
         raise ValueError(f"{op}: reset must be a contiguous bool or uint8 [B={B}], got {reset.dtype} {list(reset.shape)}")
-    sizes = [B * ppr, B, B + 1, n, n, 2, 1]
-    if out is None:
-        parts = torch.empty(sum(sizes), dtype=torch.int32, device=table.device).split(sizes)
+    sizes = (B * ppr, B, B + 1, n, n, 2, 1)
+    if out is None:  # (one allocation: the table first, on its alignment)
+        buf = torch.empty(sum(sizes), dtype=i32, device=table.device)
+        parts = buf.split_with_sizes(sizes)
         out = PageSlots(parts[0].view(B, ppr), *parts[1:])
+        at = buf.data_ptr()
+        ptrs = [at]
+        for size in sizes[:-1]:
+            at += 4 * size
+            ptrs.append(at)
     else:
-        for name, size in zip(("table", "lens", "starts", "slots", "positions", "ring", "status"), sizes):
-            t = getattr(out, name)
-            if t.dtype != torch.int32 or t.numel() != size or not t.is_contiguous() or t.device != table.device:
+        res = (out.table, out.lens, out.starts, out.slots, out.positions, out.ring, out.status)
+        for name, t, size in zip(("table", "lens", "starts", "slots", "positions", "ring", "status"), res, sizes):
+            if t.dtype is not i32 or t.numel() != size or not t.is_contiguous() or t.device != table.device:
                 raise ValueError(f"{op}: out.{name} must be contiguous int32 of {size} elements on {table.device}")
-        _lib.written(op, out.table, out.lens, out.starts, out.slots, out.positions, out.ring, out.status)
+        _lib.written(op, *res)
+        ptrs = [t.data_ptr() for t in res]
     _lib.written(op, free)
-    a = _lib.PageSlotsArgs()
-    a.B, a.pages_per_row, a.n_tokens, a.n_free = B, ppr, n, free.numel()
-    a.lens, a.new_tokens, a.reset = lens.data_ptr(), new.data_ptr(), _lib.ptr(reset)
-    a.table, a.free_pages, a.ring = table.data_ptr(), free.data_ptr(), ring.data_ptr()
-    a.table_out, a.lens_out, a.starts = out.table.data_ptr(), out.lens.data_ptr(), out.starts.data_ptr()
-    a.slots, a.positions = out.slots.data_ptr(), out.positions.data_ptr()
-    a.ring_out, a.status = out.ring.data_ptr(), out.status.data_ptr()
+    a = _lib.PageSlotsArgs(B, ppr, n, n_free, lens.data_ptr(), new.data_ptr(), _lib.ptr(reset), table.data_ptr(), free.data_ptr(),
+                           ring.data_ptr(), *ptrs)
     _lib.launch("fade_page_slots", a, table.device)
     return out
 

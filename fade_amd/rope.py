@@ -13,15 +13,15 @@ so that ``create_tiered_cache`` resolves the same scheme from an HF config.
 
 from __future__ import annotations
 
-import ctypes
 import math
 import struct
 import warnings
 from dataclasses import dataclass, field
-from fractions import Fraction
 
 import torch
 from torch import Tensor
+
+from . import _lib
 
 DEFAULT_ROPE_THETA: float = 10000.0
 DEFAULT_FACTOR: float = 1.0
@@ -32,7 +32,11 @@ DEFAULT_YARN_BETA_FAST: float = 32.0
 DEFAULT_YARN_BETA_SLOW: float = 1.0
 
 _HOST = torch.device("cpu")
-_PI = Fraction("3.14159265358979323846264338327950288419716939937511")
+# 2^192 / (2 pi), from pi to 75 digits
+_TURNS_192 = 10**74 * 2**191 // 314159265358979323846264338327950288419716939937510582097494459230781640628
+
+# device frequencies of the rotary kernels: (fractions, axes, device) -> (uint8 tensor, addresses of both)
+_TURN_TABLES: dict = {}
 
 
 def _vanilla_inv_freq(head_dim: int, theta: float, device=_HOST) -> Tensor:
@@ -93,16 +97,20 @@ class RopeScheme:
         """The axis whose position turns each frequency."""
         return [0] * int(self.inv_freq().shape[0])
 
-    def _turn_fractions(self) -> list[Fraction]:
-        """Full turns per position of each frequency, from its fp32 inverse frequency."""
-        return [Fraction(f) / (2 * _PI) for f in self.inv_freq().tolist()]
+    def _position_divisor(self) -> float:
+        return 1.0
 
     def turns(self) -> tuple[bytes, bytes]:
         """``fade_rope_args``' frequencies: each one's turns per position as a 64-bit fraction
         (so that position * fraction modulo 2^64 is the angle, exactly reduced) in 8 bytes, and
         its axis in one."""
         if self._turn_cache is None:
-            frac = [round(f * 2**64) % 2**64 for f in self._turn_fractions()]
+            da, db = float(self._position_divisor()).as_integer_ratio()
+            frac = []
+            for f in self.inv_freq().tolist():  # the fp32 inverse frequency / (2 pi), exactly, to the nearest 2^-64
+                num, den = f.as_integer_ratio()
+                num, den = num * db * _TURNS_192, den * da << 128
+                frac.append((2 * num + den) // (2 * den) % 2**64)
             self._turn_cache = (struct.pack(f"={len(frac)}Q", *frac), bytes(self.freq_axes()))
         return self._turn_cache
 
@@ -121,8 +129,8 @@ class LinearScaled(RopeScheme):
     def _positions(self, positions: Tensor) -> Tensor:
         return positions.to(_HOST).float() / self.factor
 
-    def _turn_fractions(self) -> list[Fraction]:
-        return [f / Fraction(self.factor) for f in super()._turn_fractions()]
+    def _position_divisor(self) -> float:
+        return self.factor
 
     def host_cos_sin(self, positions, model_dtype=torch.float16):
         # The reference always rounds through model_dtype for this scheme.
@@ -428,19 +436,23 @@ def rerope_gather(
     return k_out, v_out
 
 
-def rope_args(scheme: RopeScheme, head_dim: int, op: str):
-    """``fade_rope_args`` with a scheme's frequencies; the scheme keeps them."""
-    from . import _lib
-
+def rope_args(scheme: RopeScheme, head_dim: int, device: torch.device, op: str):
+    """``fade_rope_args`` with a scheme's frequencies, which stay on the device (as weights do)."""
     turn, axis = scheme.turns()
-    if 2 * len(axis) > head_dim or head_dim > 2 * _lib.ROPE_MAX_FREQS:
-        raise ValueError(f"{op}: the scheme rotates {2 * len(axis)} channels, the rows have {head_dim} (at most "
-                         f"{2 * _lib.ROPE_MAX_FREQS})")
+    tab = _TURN_TABLES.get((turn, axis, device))
+    if tab is None:
+        if scheme.n_axes > _lib.ROPE_MAX_AXES or head_dim > 2 * _lib.ROPE_MAX_FREQS:
+            raise ValueError(f"{op}: at most {_lib.ROPE_MAX_AXES} axes and head_dim {2 * _lib.ROPE_MAX_FREQS}, got {scheme.n_axes} "
+                             f"and {head_dim}")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{op}: the scheme's frequencies would be uploaded during HIP-graph capture; run the same call "
+                               "once before capturing")
+        t = torch.frombuffer(bytearray(turn + axis or b"\0"), dtype=torch.uint8).to(device)  # (waits: any stream may read it)
+        tab = _TURN_TABLES[(turn, axis, device)] = (t, t.data_ptr(), t.data_ptr() + len(turn))
+    if 2 * len(axis) > head_dim:
+        raise ValueError(f"{op}: the scheme rotates {2 * len(axis)} channels, the rows have {head_dim}")
     a = _lib.RopeArgs()
-    at = ctypes.addressof(a)
-    ctypes.memmove(at + _lib.RopeArgs.turn.offset, turn, len(turn))
-    ctypes.memmove(at + _lib.RopeArgs.axis.offset, axis, len(axis))
-    a.n_freqs = len(axis)
+    a.turn, a.axis, a.n_freqs, a.n_axes = tab[1], tab[2], len(axis), scheme.n_axes
     return a
 
 
@@ -464,32 +476,29 @@ def rope_axes(
     in fp32, one rounding to the dtype.  Returns new tensors (contiguous), or ``out``
     = (q_out, k_out), which may be the inputs themselves.
     """
-    from . import _lib
-
     op = "rope_axes"
-    tensors = [t for t in (q, k) if t is not None]
-    if not tensors:
+    ref = q if q is not None else k
+    if ref is None:
         raise ValueError(f"{op}: q or k is needed")
-    _lib.require_gpu(*tensors, positions, op=op)
+    _lib.require_gpu(q, k, positions, op=op)
     _lib.no_gradient(op, q, k)
-    ref = tensors[0]
-    if ref.dim() != 4 or tensors[-1].dim() != 4:
-        raise ValueError(f"{op}: q and k must be [B, H, S, D], got {[tuple(t.shape) for t in tensors]}")
+    if ref.dim() != 4:
+        raise ValueError(f"{op}: q and k must be [B, H, S, D], got {tuple(ref.shape)}")
     B, _, S, D = ref.shape
-    for t in tensors:
-        if (t.shape[0], t.shape[2], t.shape[3]) != (B, S, D) or t.dtype != ref.dtype:
-            raise ValueError(f"{op}: q and k differ in batch, length, head_dim or dtype: {tuple(q.shape)} {q.dtype}, "
-                             f"{tuple(k.shape)} {k.dtype}")
-    if ref.dtype not in _lib.DTYPE_CODES:
+    if k is not None and (k.dim() != 4 or k.shape[0] != B or k.shape[2] != S or k.shape[3] != D or k.dtype != ref.dtype):
+        raise ValueError(f"{op}: q and k differ in batch, length, head_dim or dtype: {tuple(ref.shape)} {ref.dtype}, "
+                         f"{tuple(k.shape)} {k.dtype}")
+    code = _lib.DTYPE_CODES.get(ref.dtype)
+    if code is None:
         raise ValueError(f"{op}: expected a float16, bfloat16 or float32 tensor, got {ref.dtype}")
-    a = rope_args(scheme, D, op)
-    a.B, a.S, a.D, a.dtype, a.inverse = B, S, D, _lib.DTYPE_CODES[ref.dtype], int(bool(inverse))
+    a = rope_args(scheme, D, ref.device, op)
+    a.B, a.S, a.D, a.dtype, a.inverse = B, S, D, code, int(bool(inverse))
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{op}: positions must be int32 or int64, got {positions.dtype}")
-    shape, axes = tuple(positions.shape), scheme.n_axes
+    shape, axes = positions.shape, a.n_axes
     if positions.dim() not in (1, 2, 3) or shape[-1] != S or (len(shape) > 1 and shape[-2] not in (1, B)) \
             or (len(shape) == 3 and shape[0] not in (1, axes)):
-        raise ValueError(f"{op}: positions must be [S], [B, S] or [{axes}, B, S] with B={B}, S={S}, got {shape}")
+        raise ValueError(f"{op}: positions must be [S], [B, S] or [{axes}, B, S] with B={B}, S={S}, got {tuple(shape)}")
     st = positions.stride()
     a.positions, a.pos64, a.pos_ss = positions.data_ptr(), int(positions.dtype == torch.int64), st[-1]
     a.pos_sb = st[-2] if len(shape) > 1 and shape[-2] > 1 else 0
@@ -510,13 +519,12 @@ def rope_axes(
                 raise ValueError(f"{op}: out must be like the input with a contiguous head_dim axis, got {o.dtype} {tuple(o.shape)}")
             _lib.no_gradient(op, o)
             _lib.written(op, o)
-        r = a.q if name == "q" else a.k
-        r.src, r.src_sb, r.src_sh, r.src_ss = t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
-        r.dst, r.dst_sb, r.dst_sh, r.dst_ss = o.data_ptr(), o.stride(0), o.stride(1), o.stride(2)
+        st, so = t.stride(), o.stride()
+        rows = _lib.RopeRows(t.data_ptr(), o.data_ptr(), st[0], st[1], st[2], so[0], so[1], so[2])
         if name == "q":
-            a.Hq = t.shape[1]
+            a.Hq, a.q = t.shape[1], rows
         else:
-            a.Hkv = t.shape[1]
+            a.Hkv, a.k = t.shape[1], rows
         res.append(o)
     _lib.launch("fade_rope_axes", a, ref.device)
     return res[0], res[1]

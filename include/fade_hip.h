@@ -499,6 +499,7 @@ int fade_page_slots(const fade_page_slots_args* args, void* stream);
  * the position read from axis axis[i]; channels from 2 * n_freqs on stay as they
  * are.  Products in fp32, rounded once to dtype. */
 #define FADE_ROPE_MAX_FREQS 128
+#define FADE_ROPE_MAX_AXES 4
 typedef struct fade_rope_rows { /* [B, heads, S, D], element strides, unit stride along D */
   const void* src;
   void* dst; /* may be src */
@@ -511,15 +512,15 @@ typedef struct fade_rope_args {
   int32_t dtype;            /* FADE_DTYPE_* (fade_paged_append: F16 or BF16) */
   int32_t inverse;          /* nonzero: turn back */
   int32_t pos64;            /* positions are int64, else int32 */
-  int32_t reserved;
+  int32_t n_axes;           /* 1 to FADE_ROPE_MAX_AXES */
   const void* positions;    /* axis a of token (b, s) at a * pos_sa + b * pos_sb + s * pos_ss */
   int64_t pos_sa, pos_sb, pos_ss;
   fade_rope_rows q, k;
   fade_rope_rows v;         /* fade_paged_append */
   const int32_t* slots;     /* fade_paged_append: [S] */
   int64_t n_pages;          /* fade_paged_append */
-  uint64_t turn[FADE_ROPE_MAX_FREQS];
-  uint8_t axis[FADE_ROPE_MAX_FREQS];
+  const uint64_t* turn;     /* device [n_freqs] */
+  const uint8_t* axis;      /* device [n_freqs], below n_axes */
 } fade_rope_args;
 int fade_rope_axes(const fade_rope_args* args, void* stream);
 /* The same for one row of S new tokens (B = 1), whose rotated k and whose v go to

@@ -39,7 +39,7 @@ def test_attention_arguments():
                 dict(q=None), dict(q=(1 << 20) + 8), dict(q_st=1020), dict(o_sh=126), dict(out=(1 << 20) + 4), dict(k_pages=None),
                 dict(v_pages=(1 << 20) + 2), dict(table=None), dict(lens=None), dict(starts=None), dict(sm_scale=0.0), dict(sm_scale=-1.0),
                 dict(sm_scale=math.nan), dict(sm_scale=math.inf), dict(mask_mode=1), dict(mask_mode=9), dict(dtype=2), dict(T=1 << 25),
-                dict(T=1 << 24, Hq=512, Hkv=512, q_st=1 << 16, o_st=1 << 16)):
+                dict(T=1 << 24, Hq=512, q_st=1 << 16, o_st=1 << 16)):
         a = _attn(**bad)
         assert _call("fade_paged_attn_workspace_bytes", a, nb) == _lib.FADE_EINVAL, bad
         assert _lib.load().fade_hip_last_error()
@@ -67,14 +67,15 @@ def test_slots_and_rope_arguments():
 
     def rope(**kw):
         a = _lib.RopeArgs()
-        for name, x in {**dict(B=1, S=4, D=64, Hq=2, Hkv=0, n_freqs=32, positions=1 << 20), **kw}.items():
+        for name, x in {**dict(B=1, S=4, D=64, Hq=2, Hkv=0, n_freqs=32, n_axes=1, positions=1 << 20), **kw}.items():
             setattr(a, name, x)
         a.q.src = a.q.dst = 1 << 20
+        a.turn = a.axis = 1 << 20
         return a
 
     for bad in (dict(dtype=3), dict(dtype=-1)):
         assert _call("fade_rope_axes", rope(**bad), None) == _lib.FADE_EINVAL
-    for name, x in (("D", 63), ("D", 258), ("n_freqs", 33), ("n_freqs", -1), ("positions", None), ("B", -1), ("B", 1 << 31), ("Hkv", 1)):
+    for name, x in (("D", 63), ("D", 258), ("n_freqs", 33), ("n_freqs", -1), ("positions", None), ("B", -1), ("B", 1 << 31), ("Hkv", 1), ("n_axes", 0), ("n_axes", 5), ("turn", None), ("axis", None)):
         a = rope()
         setattr(a, name, x)
         assert _call("fade_rope_axes", a, None) == _lib.FADE_EINVAL, name
@@ -87,35 +88,87 @@ def test_slots_and_rope_arguments():
     assert _call("fade_rope_axes", a, None) == 0
 
 
-def test_work_is_cut_into_the_bound():
-    """The device's cut (find_item of paged_attn.hip), with its fp32 sums: the items stay inside
-    the workspace and the grid, and a row's splits cover its keys."""
-    rng = random.Random(0)
+def _cut(lens, new, G, M, causal, start_cost, pieces, least, grain):
+    """What every piece of the line does (walk_start, walk_next and finish of paged_attn.hip), in
+    its precision: [(piece, row, tile, first key, last key, first, last)], the cuts {piece: parts}."""
     f = np.float32
-    for _ in range(300):
-        B, G, M = rng.choice((1, 2, 63, 64, 65, 200)), rng.choice((1, 4, 7, 20)), rng.choice((16, 64, 128, 256))
-        ppr = rng.choice((5, 100, 4000))
-        new = [rng.choice((0, 1, 1, rng.randint(0, 3000))) for _ in range(B)]
-        lens = [rng.randint(0, ppr * 64) if rng.random() < 0.7 else rng.randint(0, 90) for _ in range(B)]
-        T = sum(new) + rng.choice((0, 5))
-        target = rng.choice((3, 64, 129, 512))
-        tiles = [-(-n * G // M) for n in new]
-        bound = T * G // M + min(B, T) + target
-        work = f(0)
-        lanes = [f(0)] * 64
-        for b in range(B):
-            lanes[b % 64] = f(float(lanes[b % 64]) + float(f(tiles[b])) * float(f(lens[b])))
-        for x in lanes:
-            work = f(work + x)
-        work = f(work * f(f(1.00002) / f(target)))
-        chunk = max(256, -(-(int(work) + 1) // 64) * 64)
-        assert chunk * target >= sum(t * n for t, n in zip(tiles, lens))
-        splits = [max(1, -(-n // chunk)) for n in lens]
-        assert sum(t * s for t, s in zip(tiles, splits)) <= bound
-        assert all(s * chunk >= n > (s - 1) * chunk or s == 1 for n, s in zip(lens, splits))
+    step = -(-M // G) if causal else 0
+    base = [max(0, n - k) if causal else n for n, k in zip(lens, new)]
+    tiles = [-(-k * G // M) for k in new]
+
+    def cost(b, t):
+        return t * (base[b] + start_cost) + step * (t * (t + 1) // 2)
+
+    rows_at = [0]
+    for b in range(len(lens)):
+        rows_at.append(rows_at[-1] + cost(b, tiles[b]))
+    line = rows_at[-1]
+    piece = max(least, int(f(f(line) * f(f(1.00002) / f(pieces)))) + 1)
+    assert piece * pieces >= line
+    done, cuts = [], {}
+    for w in range(pieces):
+        x, end = w * piece, min(w * piece + piece, line)
+        tail = None
+        while x < end:
+            b = next(i for i in range(len(lens)) if rows_at[i] <= x < rows_at[i + 1])
+            off = x - rows_at[b]
+            a = base[b] + start_cost + 0.5 * step
+            t = int(2.0 * off / (a + math.sqrt(a * a + 2.0 * step * off)) if step else off / a)
+            t = min(max(t, 0), tiles[b] - 1)
+            while t > 0 and cost(b, t) > off:
+                t -= 1
+            while t + 1 < tiles[b] and cost(b, t + 1) <= off:
+                t += 1
+            at, c = rows_at[b] + cost(b, t), cost(b, t + 1) - cost(b, t)
+            assert at <= x < at + c
+            last_row = min((t + 1) * M, new[b] * G) - 1
+            seen = max(0, lens[b] - new[b] + last_row // G + 1 if causal else lens[b])
+            first, last = x == at, at + c <= end
+            lo = min((x - at) // grain * grain, seen)
+            hi = seen if last else min((end - at) // grain * grain, seen)
+            done.append((w, b, t, lo, hi, first, last))
+            tail = (at, c, first, last)
+            x = at + c
+        if tail and tail[2] and not tail[3]:
+            rest = tail[0] + tail[1] - end
+            parts = max(int(rest / piece) - 1, 0)
+            while piece * parts < rest and parts < pieces:
+                parts += 1
+            cuts[w] = parts + 1
+    return tiles, done, cuts
 
 
-def _fractions(scheme):
+def test_work_is_cut_into_equal_pieces():
+    """Every tile's keys are walked once and in order, whole or in a beginning and ends of
+    consecutive pieces, which is what the second launch joins."""
+    rng = random.Random(0)
+    for _ in range(400):
+        B, G = rng.choice((1, 2, 5, 64, 65, 150)), rng.choice((1, 2, 4, 7, 20, 71))
+        M, grain, start, least = rng.choice(((16, 32, 32, 64), (256, 64, 192, 256), (256, 32, 192, 256)))
+        cap = rng.choice((5, 100, 4000)) * 64
+        lens = [rng.randint(0, cap) if rng.random() < 0.7 else rng.randint(0, min(cap, 90)) for _ in range(B)]
+        new = [rng.choice((0, 1, 1, rng.randint(0, 3000 // G), n)) if n < 20000 else rng.choice((0, 1, 700)) for n in lens]
+        pieces, causal = rng.choice((1, 3, 32, 127, 512)), rng.random() < 0.7
+        tiles, done, cuts = _cut(lens, new, G, M, causal, start, pieces, least, grain)
+        by_tile, slots = {}, set()
+        for w, b, t, lo, hi, first, last in done:
+            by_tile.setdefault((b, t), []).append((w, lo, hi, first, last))
+            if not (first and last):
+                assert (w, first) not in slots  # a beginning and an end at most in each piece
+                slots.add((w, first))
+        assert sorted(by_tile) == [(b, t) for b in range(B) for t in range(tiles[b])]
+        for (b, t), parts in by_tile.items():
+            last_row = min((t + 1) * M, new[b] * G) - 1
+            seen = max(0, lens[b] - new[b] + last_row // G + 1 if causal else lens[b])
+            assert parts[0][1] == 0 and parts[0][3] and parts[-1][4] and parts[-1][2] == seen
+            assert [p[0] for p in parts] == list(range(parts[0][0], parts[0][0] + len(parts)))
+            assert all(p[2] == q[1] for p, q in zip(parts, parts[1:])) and not any(p[3] for p in parts[1:])
+            if len(parts) > 1:
+                assert cuts.pop(parts[0][0]) == len(parts)
+        assert not cuts
+
+
+def _fractions(scheme):  # (of a turn, in 2^-64)
     turn, axis = scheme.turns()
     return [int.from_bytes(turn[8 * i : 8 * i + 8], "little") for i in range(len(axis))], list(axis)
 
