@@ -292,6 +292,39 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
 }
 
+// Values that are no numbers.  A probability of zero does not hide an infinity or a
+// NaN from a product, so one of a token that a row does not see would reach it.  A
+// tile whose sums hold a NaN at the end of a piece is therefore walked once more:
+// each step's values are looked through, the rows add what is no number of the keys
+// that they see by themselves, and the products find zeros in their places.
+template <bool BF>
+struct Odd {
+  static constexpr uint32_t kExp = BF ? 0x7F80 : 0x7C00;
+  // whether one of the N KB at `at` (LDS) is an infinity or a NaN
+  template <int N>
+  static __device__ __forceinline__ bool any(const uint8_t* at, int lane) {
+    u16x8 top = {};
+#pragma unroll 2
+    for (int i = 0; i < N; ++i)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8, *reinterpret_cast<const u32x4*>(at + 1024 * i + 16 * lane) & 0x7FFF7FFFu));
+    const auto t2 = __builtin_elementwise_max(__builtin_elementwise_max(top.s01, top.s23), __builtin_elementwise_max(top.s45, top.s67));
+    return __builtin_amdgcn_ballot_w64(t2.x >= kExp || t2.y >= kExp) != 0;
+  }
+  static __device__ __forceinline__ uint32_t finite(uint32_t v) {
+    if ((v & kExp) == kExp) v &= 0xFFFF0000u;
+    if ((v >> 16 & kExp) == kExp) v &= 0xFFFFu;
+    return v;
+  }
+  // zeros in their places, in the BYTES bytes at `at` (LDS), by THREADS threads
+  template <int BYTES, int THREADS>
+  static __device__ __forceinline__ void clear(uint8_t* at) {
+#pragma unroll 1
+    for (int i = 4 * threadIdx.x; i < BYTES; i += 4 * THREADS) *reinterpret_cast<uint32_t*>(at + i) = finite(*reinterpret_cast<const uint32_t*>(at + i));
+  }
+  // x += what of v is no number
+  static __device__ __forceinline__ float added(float x, uint32_t v) { return (v & kExp) == kExp ? x + w2f<BF>(static_cast<uint16_t>(v)) : x; }
+};
+
 // ---- few rows: tiles of 16 matrix rows, one wave per workgroup ----
 //
 // The wave walks its piece in steps of 32 keys.  K and V rows go from the page
@@ -384,103 +417,133 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
       if (DP == D || 8 * u < D)
         lds_dma16(p.q + static_cast<int64_t>(w.q0 + rq) * p.q_st + static_cast<int64_t>(kvh * p.G + ri - rq * p.G) * p.q_sh + 8 * u, qlds + 1024 * i);
     }
-    int key = k.lo, ahead = k.lo, next = 0;  // ahead: the first key not asked for
-#pragma unroll
-    for (int i = 0; i < F::kStages - 1; ++i)
-      if (ahead < k.hi) {
-        issue(ahead, __builtin_amdgcn_readfirstlane(trow[ahead / kPage]), i);
-        ahead += F::kKeys;
-      }
-    if (ahead < k.hi) next = trow[ahead / kPage];
-    u32x4 qf[NKS];
-    {
-      // the query's loads are done when no more than the steps' are in flight
-      const int steps = (ahead - key + F::kKeys - 1) / F::kKeys;
-      if (steps >= 2 && F::kStages > 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * F::kLoads));
-      else if (steps >= 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
-      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-      asm volatile("" ::: "memory");
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
-        const int c = 32 * ks + 8 * g;
-        const u32x4 x = *reinterpret_cast<const u32x4*>(lds + F::kStages * F::kStage + 2 * (n16 * DP + c));
-        qf[ks] = DP == D || c < D ? x : u32x4{0, 0, 0, 0};
-      }
-    }
     f32x4 acc[NCB];
+    float m, l;  // of row n16 (l: over this lane's keys)
+    for (bool again = false;; again = true) {
+      int key = k.lo, ahead = k.lo, next = 0;  // ahead: the first key not asked for
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) acc[cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;  // of row n16 (l: over this lane's keys)
-    for (int t = 0; key < k.hi; key += F::kKeys, t = t + 1 == F::kStages ? 0 : t + 1) {
-      if (ahead < k.hi) {
-        issue(ahead, __builtin_amdgcn_readfirstlane(next), t == 0 ? F::kStages - 1 : t - 1);
-        ahead += F::kKeys;
-        if (ahead < k.hi) next = trow[ahead / kPage];
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm((F::kStages - 1) * F::kLoads));
-      } else if (F::kStages > 2 && key + F::kKeys < k.hi) {
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
-      } else {
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-      }
-      asm volatile("" ::: "memory");
-      uint8_t* const kt = lds + t * F::kStage;
-      uint8_t* const vt = kt + F::kTensor;
-      const int cnt = w.len - key;  // rows from here on hold no token of the row: whatever stands there must not count
-      if (cnt < F::kKeys) {
-        for (int i = lane; i < (F::kKeys - cnt) * F::kUnits; i += 64)
-          *reinterpret_cast<u32x4*>(vt + 16 * (cnt * F::kUnits + i)) = u32x4{0, 0, 0, 0};
-      }
-      f32x4 s[2];
-#pragma unroll
-      for (int kt16 = 0; kt16 < 2; ++kt16) {
-        s[kt16] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int row = 16 * kt16 + n16;
+      for (int i = 0; i < F::kStages - 1; ++i)
+        if (ahead < k.hi) {
+          issue(ahead, __builtin_amdgcn_readfirstlane(trow[ahead / kPage]), i);
+          ahead += F::kKeys;
+        }
+      if (ahead < k.hi) next = trow[ahead / kPage];
+      u32x4 qf[NKS];
+      {
+        // the query's loads are done when no more than the steps' are in flight
+        const int steps = (ahead - key + F::kKeys - 1) / F::kKeys;
+        if (steps >= 2 && F::kStages > 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * F::kLoads));
+        else if (steps >= 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
+        else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * DP * 2 + 16 * few_unit<DP>(row, 4 * ks + g));
-          s[kt16] = mfma16<BF>(a, qf[ks], s[kt16]);
+          const int c = 32 * ks + 8 * g;
+          const u32x4 x = *reinterpret_cast<const u32x4*>(lds + F::kStages * F::kStage + 2 * (n16 * DP + c));
+          qf[ks] = DP == D || c < D ? x : u32x4{0, 0, 0, 0};
         }
       }
-      float x[8], tm = -INFINITY;
-      const bool whole = key + F::kKeys <= seen_by_all;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = s[i >> 2][i & 3] * p.scale_log2;
-        if (!whole && key + 16 * (i >> 2) + 4 * g + (i & 3) >= lim) x[i] = -INFINITY;
-        tm = fmaxf(tm, x[i]);
+      for (int cb = 0; cb < NCB; ++cb) acc[cb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      m = -INFINITY;
+      l = 0.0f;
+      for (int t = 0; key < k.hi; key += F::kKeys, t = t + 1 == F::kStages ? 0 : t + 1) {
+        if (ahead < k.hi) {
+          issue(ahead, __builtin_amdgcn_readfirstlane(next), t == 0 ? F::kStages - 1 : t - 1);
+          ahead += F::kKeys;
+          if (ahead < k.hi) next = trow[ahead / kPage];
+          __builtin_amdgcn_s_waitcnt(vmcnt_imm((F::kStages - 1) * F::kLoads));
+        } else if (F::kStages > 2 && key + F::kKeys < k.hi) {
+          __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
+        } else {
+          __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        }
+        asm volatile("" ::: "memory");
+        uint8_t* const kt = lds + t * F::kStage;
+        uint8_t* const vt = kt + F::kTensor;
+        const int cnt = w.len - key;  // rows from here on hold no token of the row: whatever stands there must not count
+        if (cnt < F::kKeys) {
+          for (int i = lane; i < (F::kKeys - cnt) * F::kUnits; i += 64)
+            *reinterpret_cast<u32x4*>(vt + 16 * (cnt * F::kUnits + i)) = u32x4{0, 0, 0, 0};
+        }
+        f32x4 s[2];
+#pragma unroll
+        for (int kt16 = 0; kt16 < 2; ++kt16) {
+          s[kt16] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          const int row = 16 * kt16 + n16;
+#pragma unroll
+          for (int ks = 0; ks < NKS; ++ks) {
+            const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * DP * 2 + 16 * few_unit<DP>(row, 4 * ks + g));
+            s[kt16] = mfma16<BF>(a, qf[ks], s[kt16]);
+          }
+        }
+        float x[8], tm = -INFINITY;
+        const bool whole = key + F::kKeys <= seen_by_all;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = s[i >> 2][i & 3] * p.scale_log2;
+          if (!whole && key + 16 * (i >> 2) + 4 * g + (i & 3) >= lim) x[i] = -INFINITY;
+          tm = fmaxf(tm, x[i]);
+        }
+        tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
+        tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+        const float mn = fmaxf(m, tm);
+        const float ms = mn == -INFINITY ? 0.0f : mn;
+        float alpha = __builtin_amdgcn_exp2f(m - ms);
+        m = mn;
+        float ps = 0.0f;
+        u32x4 ph, pl;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float a = __builtin_amdgcn_exp2f(x[i] - ms), b = __builtin_amdgcn_exp2f(x[i + 1] - ms);
+          ps += a + b;
+          const uint32_t h = pack2<BF>(a, b);
+          ph[i / 2] = h;
+          pl[i / 2] = pack2<BF>(a - w2f<BF>(static_cast<uint16_t>(h)), b - w2f<BF>(static_cast<uint16_t>(h >> 16)));
+        }
+        l = l * alpha + ps;
+        auto value_frag = [&](int cb) {
+          // lane (n, g) points at key 4 g + n / 4 (+ 16), channels 16 cb + 4 (n % 4) .. + 3
+          const int row = 4 * g + (n16 >> 2), u = 2 * cb + ((n16 >> 1) & 1);
+          const uint8_t* at = vt + row * DP * 2 + 16 * few_unit<DP>(row, u) + 8 * (n16 & 1);
+          const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at)));
+          const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at + 16 * DP * 2)));  // (row + 16: the same swizzle)
+          const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+          return u32x4{w0.x, w0.y, w1.x, w1.y};
+        };
+        if (again && Odd<BF>::template any<F::kTensor / 1024>(vt, lane)) {
+#pragma unroll
+          for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[cb][i] *= alpha;
+#pragma unroll 1
+          for (int j = 0; j < F::kKeys && key + j < lim; ++j)
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb) {  // channels 16 cb + 4 g .. + 3
+              const u32x2 v = *reinterpret_cast<const u32x2*>(vt + j * DP * 2 + 16 * few_unit<DP>(j, 2 * cb + (g >> 1)) + 8 * (g & 1));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[cb][i] = Odd<BF>::added(acc[cb][i], v[i >> 1] >> (16 * (i & 1)));
+            }
+          Odd<BF>::template clear<F::kTensor, 64>(vt);
+          asm volatile("" ::: "memory");
+          alpha = 1.0f;
+        }
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+          const u32x4 a = value_frag(cb);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[cb][i] *= alpha;
+          acc[cb] = mfma16<BF>(a, ph, acc[cb]);
+          acc[cb] = mfma16<BF>(a, pl, acc[cb]);
+        }
       }
-      tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
-      tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
-      const float mn = fmaxf(m, tm);
-      const float ms = mn == -INFINITY ? 0.0f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m - ms);
-      m = mn;
-      float ps = 0.0f;
-      u32x4 ph, pl;
+      bool nan = false;
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const float a = __builtin_amdgcn_exp2f(x[i] - ms), b = __builtin_amdgcn_exp2f(x[i + 1] - ms);
-        ps += a + b;
-        const uint32_t h = pack2<BF>(a, b);
-        ph[i / 2] = h;
-        pl[i / 2] = pack2<BF>(a - w2f<BF>(static_cast<uint16_t>(h)), b - w2f<BF>(static_cast<uint16_t>(h >> 16)));
-      }
-      l = l * alpha + ps;
+      for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
-      for (int cb = 0; cb < NCB; ++cb) {
-        // lane (n, g) points at key 4 g + n / 4 (+ 16), channels 16 cb + 4 (n % 4) .. + 3
-        const int row = 4 * g + (n16 >> 2), u = 2 * cb + ((n16 >> 1) & 1);
-        const uint8_t* at = vt + row * DP * 2 + 16 * few_unit<DP>(row, u) + 8 * (n16 & 1);
-        const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at)));
-        const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            reinterpret_cast<lds_i16x4*>((lds_u8*)const_cast<uint8_t*>(at + 16 * DP * 2)));  // (row + 16: the same swizzle)
-        const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-        const u32x4 a = {w0.x, w0.y, w1.x, w1.y};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[cb][i] *= alpha;
-        acc[cb] = mfma16<BF>(a, ph, acc[cb]);
-        acc[cb] = mfma16<BF>(a, pl, acc[cb]);
-      }
+        for (int i = 0; i < 4; ++i) nan |= acc[cb][i] != acc[cb][i];
+      if (again || __builtin_amdgcn_ballot_w64(nan) == 0) break;
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -508,9 +571,9 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
   finish(p, k, true);
 }
 
-// ---- many rows: tiles of 32 NW MT matrix rows, the keys shared through LDS ----
+// ---- many rows: tiles of 32 NW matrix rows, the keys shared through LDS ----
 //
-// NW waves of MT blocks of 32 matrix rows each walk the item's keys page by page.
+// NW waves of 32 matrix rows each walk the item's keys page by page.
 // A page's K and V go straight to LDS, two pages deep, every wave loading its
 // share; one barrier per page.
 //   S^T = K Q^T   32x32x16 MFMAs, A = 32 keys x 16 channels, B = Q^T (registers):
@@ -551,9 +614,9 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <int DP, int NW, int MT, int KT, int NST, bool BF>
+template <int DP, int NW, int KT, int NST, bool BF>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_wide_kernel(Params p) {
-  constexpr int M = 32 * NW * MT;
+  constexpr int M = 32 * NW;
   constexpr int NKS = DP / 16, NCB = DP / 32, UNITS = DP / 8;
   constexpr int TENSOR = KT * DP * 2, STAGE = 2 * TENSOR, NKB = KT / 32;
   constexpr int LPW = TENSOR / 1024 / NW;  // direct loads of K, and of V, per wave and page
@@ -570,6 +633,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int D = p.D;
 
   __shared__ __attribute__((aligned(256))) uint8_t lds[NST * STAGE];
+  __shared__ int any_nan;
   const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds)));
   if (D < DP) {  // units past the head_dim are never loaded: zeros
     for (int i = 16 * threadIdx.x; i < NST * STAGE; i += 1024 * NW) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0, 0, 0, 0};
@@ -610,236 +674,271 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   };
   const float sl2 = p.scale_log2;
   while (walk_next(p, KT, k)) {
-  const Tile& w = k.w;
-  const int all = w.n * p.G;  // the row's matrix rows
-  auto limit = [&](int i) {
-    const int x = p.causal ? w.len - w.n + i + 1 : w.len;
-    return x < 0 ? 0 : x;
-  };
-  // this wave's matrix rows, and the fewest and the most keys they see
-  const int r0 = w.tile * M + 32 * MT * wave;
-  const bool active = r0 < all;
-  const int rl = r0 + 32 * MT < all ? r0 + 32 * MT : all;
-  const int wlo = __builtin_amdgcn_readfirstlane(active ? limit(r0 / p.G) : 0);
-  const int whi = __builtin_amdgcn_readfirstlane(active ? limit((rl - 1) / p.G) : 0);
-  int lim[MT];
-  const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + w.b * p.ppr);  // (scalar loads: vmcnt counts the steps' alone)
-  auto issue = [&](int key, int id, int buf) {
-    id = id < 0 || id >= p.n_pages ? 0 : id;
-    const int64_t at = ((static_cast<int64_t>(id) * p.Hkv + kvh) * kPage + key % kPage) * D;
-    const uint32_t to = base + buf * STAGE + 1024 * LPW * wave;
-    if constexpr (kKeep) {
-#pragma unroll
-      for (int i = 0; i < LPW; ++i) {
-        if (kin[i]) lds_dma16(p.kp + at, ko[i], to + 1024 * i);
-        if (vin[i]) lds_dma16(p.vp + at, vo[i], to + TENSOR + 1024 * i);
-      }
-    } else {
-      int l = threadIdx.x & 63;
-      asm volatile("" : "+v"(l));  // (not computed ahead of the loop)
-#pragma unroll
-      for (int i = 0; i < LPW; ++i) {
-        uint32_t k_off, v_off;
-        bool k_in, v_in;
-        place(i, l, k_off, v_off, k_in, v_in);
-        if (k_in) lds_dma16(p.kp + at, k_off, to + 1024 * i);
-        if (v_in) lds_dma16(p.vp + at, v_off, to + TENSOR + 1024 * i);
-      }
-    }
-  };
-  __syncthreads();  // the LDS is done with
-  int ahead = k.lo, next = 0;  // ahead: the first key not asked for
-  auto issue_next = [&](int to) {
-    issue(ahead, __builtin_amdgcn_readfirstlane(next), to);
-    ahead += KT;
-    if (ahead < k.hi) next = trow[ahead / kPage];
-  };
-  if (ahead < k.hi) {
-    next = trow[ahead / kPage];
-    issue_next(buf);
-  }
-  u32x4 qf[MT][NKS];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = r0 + 32 * mt + n32;
-    const bool live = r < all;
-    const int qi = live ? r / p.G : 0;
-    lim[mt] = live ? limit(qi) : 0;
-    const uint16_t* qr = p.q + static_cast<int64_t>(w.q0 + qi) * p.q_st + static_cast<int64_t>(kvh * p.G + (live ? r - qi * p.G : 0)) * p.q_sh;
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      const int c = 16 * ks + 8 * h;
-      qf[mt][ks] = live && c < D ? *reinterpret_cast<const u32x4*>(qr + c) : u32x4{0, 0, 0, 0};
-    }
-  }
-  f32x16 acc[MT][NCB];
-  float m[MT], l[MT];  // of row n32: the running maximum (raw scores), the sum over this half's keys
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    m[mt] = kNegBig;
-    l[mt] = 0.0f;
-#pragma unroll
-    for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[mt][cb][i] = 0.0f;
-  }
-
-  // the query and the first step; in the loop only the direct loads are in flight, which the compiler does not count
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-#pragma unroll
-  for (int i = 1; i < NST - 1; ++i)
-    if (ahead < k.hi) issue_next(buf + i < NST ? buf + i : buf + i - NST);
-  for (int key = k.lo; key < k.hi; key += KT, flip()) {
-    // this wave's share of the step: later steps' may be in flight
-    const int later = ahead - key - KT;
-    if (NST > 3 && later > KT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(4 * LPW));
-    else if (NST > 2 && later > 0) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * LPW));
-    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-    __syncthreads();  // everyone's; and the step before is done with
-    uint8_t* const vt = lds + buf * STAGE + TENSOR;
-    const int cnt = w.len - key;
-    if (cnt < KT) {  // rows that hold no token: whatever stands there must not count
-      for (int i = threadIdx.x; i < (KT - cnt) * UNITS; i += 64 * NW) *reinterpret_cast<u32x4*>(vt + 16 * (cnt * UNITS + i)) = u32x4{0, 0, 0, 0};
-      __syncthreads();
-    }
-    if (ahead < k.hi) issue_next(buf == 0 ? NST - 1 : buf - 1);
-    if (key >= whi) continue;  // (to flip())
-    // fragments are read AH ahead of their products
-    constexpr int AH = DP > 128 ? 2 : 4;
-    constexpr int kCompute = 0x6;  // (vector and scalar arithmetic may pass, reads and products keep their order)
-    auto k_frag = [&](int f) { return lds_read16((kat ^ (32 * (f % NKS % KA))) + 32 * (f / NKS) * DP * 2 + 256 * (f % NKS / KA)); };
-    auto v_frag = [&](int f) {
-      const uint32_t at = (vat ^ (64 * (f % NCB % VA))) + 16 * (f / NCB) * DP * 2 + 256 * (f % NCB / VA);
-      const u32x2 w0 = lds_read_tr(at), w1 = lds_read_tr(at + 8 * DP * 2);  // (row + 8: the same exchange)
-      return u32x4{w0.x, w0.y, w1.x, w1.y};
+    const Tile& w = k.w;
+    const int all = w.n * p.G;  // the row's matrix rows
+    auto limit = [&](int i) {
+      const int x = p.causal ? w.len - w.n + i + 1 : w.len;
+      return x < 0 ? 0 : x;
     };
-    f32x16 s[MT][NKB];
-    {
-      u32x4 kf[AH];
+    // this wave's matrix rows, and the fewest and the most keys they see
+    const int r0 = w.tile * M + 32 * wave;
+    const bool active = r0 < all;
+    const int rl = r0 + 32 < all ? r0 + 32 : all;
+    const int wlo = __builtin_amdgcn_readfirstlane(active ? limit(r0 / p.G) : 0);
+    const int whi = __builtin_amdgcn_readfirstlane(active ? limit((rl - 1) / p.G) : 0);
+    const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + w.b * p.ppr);  // (scalar loads: vmcnt counts the steps' alone)
+    auto issue = [&](int key, int id, int buf) {
+      id = id < 0 || id >= p.n_pages ? 0 : id;
+      const int64_t at = ((static_cast<int64_t>(id) * p.Hkv + kvh) * kPage + key % kPage) * D;
+      const uint32_t to = base + buf * STAGE + 1024 * LPW * wave;
+      if constexpr (kKeep) {
 #pragma unroll
-      for (int f = 0; f < AH; ++f) kf[f] = k_frag(f);
-      __builtin_amdgcn_sched_barrier(kCompute);
-#pragma unroll
-      for (int f = 0; f < NKS * NKB; ++f) {
-        const u32x4 a = kf[f % AH];
-        if (f + AH < NKS * NKB) kf[f % AH] = k_frag(f + AH);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          if (f % NKS == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[mt][f / NKS][i] = 0.0f;
-          }
-          s[mt][f / NKS] = mfma32<BF>(a, qf[mt][f % NKS], s[mt][f / NKS]);
+        for (int i = 0; i < LPW; ++i) {
+          if (kin[i]) lds_dma16(p.kp + at, ko[i], to + 1024 * i);
+          if (vin[i]) lds_dma16(p.vp + at, vo[i], to + TENSOR + 1024 * i);
         }
-        __builtin_amdgcn_sched_barrier(kCompute);
+      } else {
+        int l = threadIdx.x & 63;
+        asm volatile("" : "+v"(l));  // (not computed ahead of the loop)
+#pragma unroll
+        for (int i = 0; i < LPW; ++i) {
+          uint32_t k_off, v_off;
+          bool k_in, v_in;
+          place(i, l, k_off, v_off, k_in, v_in);
+          if (k_in) lds_dma16(p.kp + at, k_off, to + 1024 * i);
+          if (v_in) lds_dma16(p.vp + at, v_off, to + TENSOR + 1024 * i);
+        }
       }
-    }
-    u32x4 pa[MT][2 * NKB];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if (key + KT > wlo) {
-        const int left = lim[mt] - key;
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * kb + 8 * (i >> 2) + 4 * h + (i & 3) >= left) s[mt][kb][i] = -INFINITY;
+    };
+    const bool live = r0 + n32 < all;
+    // this lane's query and head (not kept over the steps, which need every register)
+    auto row = [&](int& qi, int& hd) {
+      int r = threadIdx.x & 31;
+      asm volatile("" : "+v"(r));
+      r = live ? r0 + r : 0;
+      qi = r / p.G;
+      hd = kvh * p.G + r - qi * p.G;
+    };
+    int lim;
+    f32x16 acc[NCB];
+    float m, l;  // of row n32: the running maximum (raw scores), the sum over this half's keys
+    for (bool again = false;; again = true) {
+      __syncthreads();  // the LDS is done with
+      if (threadIdx.x == 0) any_nan = 0;
+      int ahead = k.lo, next = 0;  // ahead: the first key not asked for
+      auto issue_next = [&](int to) {
+        issue(ahead, __builtin_amdgcn_readfirstlane(next), to);
+        ahead += KT;
+        if (ahead < k.hi) next = trow[ahead / kPage];
+      };
+      if (ahead < k.hi) {
+        next = trow[ahead / kPage];
+        issue_next(buf);
       }
-      auto probs = [&]() {
-        const float nm = -m[mt] * sl2;
+      u32x4 qf[NKS];
+      {
+        int qi, hd;
+        row(qi, hd);
+        lim = live ? limit(qi) : 0;
+        const uint16_t* qr = p.q + static_cast<int64_t>(w.q0 + qi) * p.q_st + static_cast<int64_t>(hd) * p.q_sh;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+          const int c = 16 * ks + 8 * h;
+          qf[ks] = live && c < D ? *reinterpret_cast<const u32x4*>(qr + c) : u32x4{0, 0, 0, 0};
+        }
+      }
+      m = kNegBig;
+      l = 0.0f;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[cb][i] = 0.0f;
+
+      // the query and the first step; in the loop only the direct loads are in flight, which the compiler does not count
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+#pragma unroll
+      for (int i = 1; i < NST - 1; ++i)
+        if (ahead < k.hi) issue_next(buf + i < NST ? buf + i : buf + i - NST);
+      for (int key = k.lo; key < k.hi; key += KT, flip()) {
+        // this wave's share of the step: later steps' may be in flight
+        const int later = ahead - key - KT;
+        if (NST > 3 && later > KT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(4 * LPW));
+        else if (NST > 2 && later > 0) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * LPW));
+        else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        __syncthreads();  // everyone's; and the step before is done with
+        uint8_t* const vt = lds + buf * STAGE + TENSOR;
+        const int cnt = w.len - key;
+        if (cnt < KT) {  // rows that hold no token: whatever stands there must not count
+          for (int i = threadIdx.x; i < (KT - cnt) * UNITS; i += 64 * NW) *reinterpret_cast<u32x4*>(vt + 16 * (cnt * UNITS + i)) = u32x4{0, 0, 0, 0};
+          __syncthreads();
+        }
+        if (ahead < k.hi) issue_next(buf == 0 ? NST - 1 : buf - 1);
+        const bool odd = again && Odd<BF>::template any<TENSOR / 1024>(vt, lane);
+        if (key >= whi) {
+          if (odd) {  // (the barriers of the waves that compute)
+            __syncthreads();
+            Odd<BF>::template clear<TENSOR, 64 * NW>(vt);
+            __syncthreads();
+          }
+          continue;  // (to flip())
+        }
+        // fragments are read AH ahead of their products
+        constexpr int AH = DP > 128 ? 2 : 4;
+        constexpr int kCompute = 0x6;  // (vector and scalar arithmetic may pass, reads and products keep their order)
+        auto k_frag = [&](int f) {  // k-step f / NKB of key block f % NKB
+          const int ks = f / NKB;
+          return lds_read16((kat ^ (32 * (ks % KA))) + 32 * (f % NKB) * DP * 2 + 256 * (ks / KA));
+        };
+        auto v_frag = [&](int f) {
+          const uint32_t at = (vat ^ (64 * (f % NCB % VA))) + 16 * (f / NCB) * DP * 2 + 256 * (f % NCB / VA);
+          const u32x2 w0 = lds_read_tr(at), w1 = lds_read_tr(at + 8 * DP * 2);  // (row + 8: the same exchange)
+          return u32x4{w0.x, w0.y, w1.x, w1.y};
+        };
+        f32x16 s[NKB];
+        {
+          u32x4 kf[AH];
+#pragma unroll
+          for (int f = 0; f < AH; ++f) kf[f] = k_frag(f);
+          __builtin_amdgcn_sched_barrier(kCompute);
+#pragma unroll
+          for (int f = 0; f < NKS * NKB; ++f) {
+            const u32x4 a = kf[f % AH];
+            if (f + AH < NKS * NKB) kf[f % AH] = k_frag(f + AH);
+            if (f < NKB) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[f % NKB][i] = 0.0f;
+            }
+            s[f % NKB] = mfma32<BF>(a, qf[f / NKB], s[f % NKB]);
+            __builtin_amdgcn_sched_barrier(kCompute);
+          }
+        }
+        if (key + KT > wlo) {
+          const int left = lim - key - 4 * h;
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (left <= 32 * kb + 8 * (i >> 2) + (i & 3)) s[kb][i] = -INFINITY;
+        }
+        u32x4 pa[2 * NKB];
+        auto probs = [&]() {
+          const float nm = -m * sl2;
+#pragma unroll
+          for (int st = 0; st < 2 * NKB; ++st)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              pa[st][j] = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j], sl2, nm)),
+                                    __builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j + 1], sl2, nm)));
+        };
+        probs();
+        // 16-bit patterns of the non-negative probabilities order as their values do
+        u16x8 pm = __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[0]), __builtin_bit_cast(u16x8, pa[1]));
+        if constexpr (NKB == 2)
+          pm = __builtin_elementwise_max(pm, __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[2]), __builtin_bit_cast(u16x8, pa[3])));
+        const auto p2 = __builtin_elementwise_max(__builtin_elementwise_max(pm.s01, pm.s23), __builtin_elementwise_max(pm.s45, pm.s67));
+        constexpr uint16_t kOver = BF ? 0x4380 : 0x5C00;  // 2^8
+        const bool over = __builtin_amdgcn_ballot_w64(p2.x > kOver || p2.y > kOver) != 0;
+        if (over || odd) {  // (one branch for what is rare)
+          if (over) {
+            float mx = kNegBig;
+#pragma unroll
+            for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[kb][i], s[kb][i + 1]));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mn = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f((m - mn) * sl2);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[cb][i] *= alpha;
+            probs();
+          }
+          if (odd) {
+#pragma unroll 1
+            for (int j = 0; j < KT && key + j < lim; ++j)
+#pragma unroll
+              for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {  // channels 32 cb + 8 q + 4 h .. + 3
+                  const u32x2 v = *reinterpret_cast<const u32x2*>(vt + j * DP * 2 + 16 * wide_v_unit<DP>(j, 4 * cb + q) + 8 * h);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[cb][4 * q + i] = Odd<BF>::added(acc[cb][4 * q + i], v[i >> 1] >> (16 * (i & 1)));
+                }
+            __syncthreads();
+            Odd<BF>::template clear<TENSOR, 64 * NW>(vt);
+            __syncthreads();
+          }
+        }
+        float ps = 0.0f;
 #pragma unroll
         for (int st = 0; st < 2 * NKB; ++st)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            pa[mt][st][j] = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[mt][st >> 1][8 * (st & 1) + 2 * j], sl2, nm)),
-                                      __builtin_amdgcn_exp2f(fmaf(s[mt][st >> 1][8 * (st & 1) + 2 * j + 1], sl2, nm)));
-      };
-      probs();
-      // 16-bit patterns of the non-negative probabilities order as their values do
-      u16x8 pm = __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][0]), __builtin_bit_cast(u16x8, pa[mt][1]));
-      if constexpr (NKB == 2)
-        pm = __builtin_elementwise_max(pm, __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[mt][2]), __builtin_bit_cast(u16x8, pa[mt][3])));
-      const auto p2 = __builtin_elementwise_max(__builtin_elementwise_max(pm.s01, pm.s23), __builtin_elementwise_max(pm.s45, pm.s67));
-      constexpr uint16_t kOver = BF ? 0x4380 : 0x5C00;  // 2^8
-      if (__builtin_amdgcn_ballot_w64(p2.x > kOver || p2.y > kOver) != 0) {
-        float mx = kNegBig;
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t pw = pa[st][j];  // (a bit cast of a vector's element itself takes element 0)
+            if constexpr (BF)
+              ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw), (bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}), ps, false);
+            else
+              ps = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pw), (f16x2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}), ps, false);
+          }
+        l += ps;
+        {
+          u32x4 vf[AH];
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb)
+          for (int f = 0; f < AH; ++f) vf[f] = v_frag(f);
+          __builtin_amdgcn_sched_barrier(kCompute);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[mt][kb][i], s[mt][kb][i + 1]));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m[mt], mx);
-        const float alpha = __builtin_amdgcn_exp2f((m[mt] - mn) * sl2);
-        m[mt] = mn;
-        l[mt] *= alpha;
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[mt][cb][i] *= alpha;
-        probs();
-      }
-      float ps = 0.0f;
-#pragma unroll
-      for (int st = 0; st < 2 * NKB; ++st)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t pw = pa[mt][st][j];  // (a bit cast of a vector's element itself takes element 0)
-          if constexpr (BF)
-            ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pw), (bf16x2{static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)}), ps, false);
-          else
-            ps = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pw), (f16x2{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}), ps, false);
+          for (int f = 0; f < 2 * NKB * NCB; ++f) {
+            const u32x4 a = vf[f % AH];
+            if (f + AH < 2 * NKB * NCB) vf[f % AH] = v_frag(f + AH);
+            acc[f % NCB] = mfma32<BF>(a, pa[f / NCB], acc[f % NCB]);
+            __builtin_amdgcn_sched_barrier(kCompute);
+          }
         }
-      l[mt] += ps;
-    }
-    {
-      u32x4 vf[AH];
-#pragma unroll
-      for (int f = 0; f < AH; ++f) vf[f] = v_frag(f);
-      __builtin_amdgcn_sched_barrier(kCompute);
-#pragma unroll
-      for (int f = 0; f < 2 * NKB * NCB; ++f) {
-        const u32x4 a = vf[f % AH];
-        if (f + AH < 2 * NKB * NCB) vf[f % AH] = v_frag(f + AH);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt][f % NCB] = mfma32<BF>(a, pa[mt][f / NCB], acc[mt][f % NCB]);
-        __builtin_amdgcn_sched_barrier(kCompute);
       }
-    }
-  }
 
-  // ---- lane (n, h): row n, channels 32 cb + 8 q + 4 h .. + 3 ----
-  const bool part = !(k.first && k.last);
+      bool nan = false;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const float lt = l[mt] + __shfl_xor(l[mt], 32, 64);
-    const int r = r0 + 32 * mt + n32;
-    if (r >= all) continue;
-    if (part) {
-      const int64_t pr = (static_cast<int64_t>(blockIdx.x) * 2 + (k.first ? 1 : 0)) * M + 32 * (MT * wave + mt) + n32;
-      if (h == 0) p.part_ml[pr] = make_float2(m[mt] * sl2, lt);
+      for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) nan |= acc[cb][i] != acc[cb][i];
+      if (again) break;
+      if (nan) any_nan = 1;
+      __syncthreads();
+      if (__builtin_amdgcn_readfirstlane(any_nan) == 0) break;
+    }
+
+    // ---- lane (n, h): row n, channels 32 cb + 8 q + 4 h .. + 3 ----
+    const bool part = !(k.first && k.last);
+    const float lt = l + __shfl_xor(l, 32, 64);
+    if (live && part) {
+      const int64_t pr = (static_cast<int64_t>(blockIdx.x) * 2 + (k.first ? 1 : 0)) * M + 32 * wave + n32;
+      if (h == 0) p.part_ml[pr] = make_float2(m * sl2, lt);
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int c = 32 * cb + 8 * q + 4 * h;
-          if (c < D) *reinterpret_cast<f32x4*>(p.part_o + pr * D + c) = f32x4{acc[mt][cb][4 * q], acc[mt][cb][4 * q + 1], acc[mt][cb][4 * q + 2], acc[mt][cb][4 * q + 3]};
+          if (c < D) *reinterpret_cast<f32x4*>(p.part_o + pr * D + c) = f32x4{acc[cb][4 * q], acc[cb][4 * q + 1], acc[cb][4 * q + 2], acc[cb][4 * q + 3]};
         }
-    } else {
-      const int qi = r / p.G;
+    } else if (live) {
       const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;  // no visible key: zeros
-      uint16_t* dst = p.out + static_cast<int64_t>(w.q0 + qi) * p.o_st + static_cast<int64_t>(kvh * p.G + r - qi * p.G) * p.o_sh;
+      int qi, hd;
+      row(qi, hd);
+      uint16_t* dst = p.out + static_cast<int64_t>(w.q0 + qi) * p.o_st + static_cast<int64_t>(hd) * p.o_sh;
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int c = 32 * cb + 8 * q + 4 * h;
-          u32x2 w;
-          w.x = pack2<BF>(acc[mt][cb][4 * q] * inv, acc[mt][cb][4 * q + 1] * inv);
-          w.y = pack2<BF>(acc[mt][cb][4 * q + 2] * inv, acc[mt][cb][4 * q + 3] * inv);
-          if (c < D) *reinterpret_cast<u32x2*>(dst + c) = w;
+          u32x2 o;
+          o.x = pack2<BF>(acc[cb][4 * q] * inv, acc[cb][4 * q + 1] * inv);
+          o.y = pack2<BF>(acc[cb][4 * q + 2] * inv, acc[cb][4 * q + 3] * inv);
+          if (c < D) *reinterpret_cast<u32x2*>(dst + c) = o;
         }
     }
-  }
   }
   finish(p, k, true);
 }
@@ -930,7 +1029,7 @@ bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 
 
 template <int DP>
 struct Wide {  // waves, blocks of 32 rows per wave, keys per step
-  static constexpr int NW = 8, MT = 1, M = 32 * NW * MT, KT = DP > 128 ? 32 : 64, NST = DP > 128 ? 4 : 3;
+  static constexpr int NW = 8, M = 32 * NW, KT = DP > 128 ? 32 : 64, NST = DP > 128 ? 4 : 3;
 };
 constexpr int kWideLog = 8;
 
@@ -1024,7 +1123,7 @@ template <int DP, bool BF>
 int launch(const Plan& pl, hipStream_t st) {
   if (pl.both) {
     typedef Wide<DP> W;
-    hipLaunchKernelGGL((paged_wide_kernel<DP, W::NW, W::MT, W::KT, W::NST, BF>), dim3(static_cast<unsigned>(pl.wide.Hkv * pl.wide.pieces)), dim3(64 * W::NW), 0, st, pl.wide);
+    hipLaunchKernelGGL((paged_wide_kernel<DP, W::NW, W::KT, W::NST, BF>), dim3(static_cast<unsigned>(pl.wide.Hkv * pl.wide.pieces)), dim3(64 * W::NW), 0, st, pl.wide);
     const int rc = check_launch("fade_paged_attn");
     if (rc) return rc;
   }

@@ -497,6 +497,38 @@ def test_attention_extreme_scores(dev):
     assert bool(got[1:3].isnan().all()) and bool(got[-1].isnan().all()) and not bool(got[3:-1].isnan().any())
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (3, 3, 64), (4, 2, 256), (2, 1, 80)])
+@pytest.mark.parametrize("lens,new", [([70, 33, 200], [3, 4, 2]), ([64, 300], [64, 170]), ([130, 1, 700], [130, 1, 97])])
+def test_attention_values_that_are_no_numbers(dev, lens, new, Hq, Hkv, D, dtype):
+    """An infinity or a NaN in V reaches the queries that see its key, and no other."""
+    g = torch.Generator(device=dev).manual_seed(D)
+    k, v, table = _pages(g, dev, lens, Hkv, D, dtype, junk=math.nan)
+    q = torch.randn(sum(new), Hq, D, generator=g, device=dev).to(dtype)
+    starts = _starts(new)
+    args = (table, _i32(lens, dev), _i32(starts, dev))
+    odd = v.clone()
+    up, down = torch.zeros(2, len(lens), max(lens), Hkv, D, dtype=torch.bool, device=dev)
+    for b, (L, n) in enumerate(zip(lens, new)):
+        # the last token, one among the new ones, the last one before them
+        for j, (t, x) in enumerate(zip((L - 1, L - 1 - n // 2, max(L - n - 1, 0)), (math.nan, math.inf, -math.inf))):
+            at = (table[b, t // PAGE_TOKENS], (b + j) % Hkv, t % PAGE_TOKENS)
+            odd[(*at, slice(j, D, 5))] = x
+            v[(*at, slice(j, D, 5))] = 0.0
+            up[b, t, (b + j) % Hkv, j::5] |= not x < 0
+            down[b, t, (b + j) % Hkv, j::5] |= not x > 0
+    want = paged_attention(q, k, v, *args)
+    got = paged_attention(q, k, odd, *args)
+    for b, (L, n) in enumerate(zip(lens, new)):
+        for i in range(n):
+            for kind, sign in ((up, math.inf), (down, -math.inf)):
+                hit = kind[b, : L - n + i + 1].any(0).repeat_interleave(Hq // Hkv, 0)
+                want[starts[b] + i] = torch.where(hit, want[starts[b] + i] + sign, want[starts[b] + i])
+    wrong = ~((got == want) | (got.isnan() & want.isnan()))
+    at = wrong.nonzero()[:4].tolist()
+    assert not at, [(i, float(got[tuple(i)]), float(want[tuple(i)])) for i in at]
+
+
 def test_attention_device_data_out_of_range(dev):
     """Lengths past the table, page ids outside the pool, starts past q: kept inside the tensors."""
     H, D = 2, 64
