@@ -10,6 +10,7 @@ import random
 import pytest
 import torch
 
+from fade_amd import _lib
 from fade_amd.kernels import PagedAttentionPlan, paged_append, paged_attention, tiered_prefill_attention
 from fade_amd.pages import PAGE_TOKENS, MiddlePagePool, PageSlots, TokenPagePool, page_slots
 from fade_amd.quant import quant_k_int4, quant_v_int4
@@ -663,3 +664,160 @@ def test_attention_agrees_with_the_prefill(dev):
     got = paged_attention(q.reshape(B * n, Hq, D), k, v, table, _i32([L] * B, dev), _i32([0, n, 2 * n], dev)).reshape(B, n, Hq, D)
     bound = 4 * torch.finfo(F16).eps / 2 * float(v.abs().max())  # two outputs, a rounding of the probabilities and of the output each
     assert float((got.transpose(1, 2).double() - ref.double()).abs().max()) <= bound
+
+
+def _step_inputs(g, dev, T, Hq, Hkv, D, dtype):
+    return torch.randn(T, Hq + 2 * Hkv, D, generator=g, device=dev).to(dtype)
+
+
+def _step(pool, state, new, qkv, T, Hq, Hkv, scheme):
+    state = pool.step(state, new, T)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq : Hq + Hkv], qkv[:, Hq + Hkv :]
+    qr = paged_append(k, v, pool.k, pool.v, state.slots, q=q, positions=state.positions, scheme=scheme)
+    return state, paged_attention(qr, pool.k, pool.v, state.table, state.lens, state.starts)
+
+
+def test_steps_in_two_graphs(dev):
+    """A decoding step and one with a chunk, captured and replayed in turn over one pool, with eager steps of
+    another pool between them: every replay as the eager step."""
+    B, Hq, Hkv, D, dtype = 5, 8, 2, 64, BF16
+    scheme = Llama3(theta=5e5, head_dim=D)
+    eager, pool = (TokenPagePool(80, Hkv, D, dtype, dev) for _ in range(2))
+    g = torch.Generator(device=dev).manual_seed(11)
+    kinds = ([1] * B, [1, 150, 1, 0, 1])
+    a = eager.start(B, 12)
+    lens, table = (torch.zeros_like(x) for x in (a.lens, a.table))
+    ring = pool.ring.clone()
+    graphs = []
+    for new in kinds:
+        T = sum(new) + 3
+        x = dict(new=_i32(new, dev), qkv=torch.zeros(T, Hq + 2 * Hkv, D, dtype=dtype, device=dev), T=T)
+
+        def run(x=x):
+            st = PageSlots(table, lens, None, None, None, ring, None)
+            pool.ring = ring
+            st, out = _step(pool, st, x["new"], x["qkv"], x["T"], Hq, Hkv, scheme)
+            for dst, src in ((lens, st.lens), (table, st.table), (ring, st.ring)):
+                dst.copy_(src)
+            return st, out
+
+        keep = [t.clone() for t in (lens, table, ring, pool.free, pool.k, pool.v)]
+        run()
+        for t, old in zip((lens, table, ring, pool.free, pool.k, pool.v), keep):
+            t.copy_(old)
+        x["graph"] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(x["graph"]):
+            x["state"], x["out"] = run()
+        graphs.append(x)
+    for i in range(7):
+        x = graphs[i % 2]
+        qkv = _step_inputs(g, dev, x["T"], Hq, Hkv, D, dtype)
+        a, want = _step(eager, a, x["new"], qkv, x["T"], Hq, Hkv, scheme)
+        a.check()
+        x["qkv"].copy_(qkv)
+        x["graph"].replay()
+        assert int(x["state"].status) == 0 and torch.equal(x["out"], want), i
+        assert torch.equal(lens, a.lens) and torch.equal(table, a.table) and torch.equal(ring, a.ring)
+        torch.cuda.synchronize()
+
+
+def test_steps_on_another_stream(dev):
+    """A step on a side stream while the default stream works on another pool's."""
+    B, Hq, Hkv, D, dtype = 3, 4, 4, 128, F16
+    scheme = Vanilla(theta=1e4, head_dim=D)
+    g = torch.Generator(device=dev).manual_seed(12)
+    new = _i32([300, 1, 64], dev)
+    pools = [TokenPagePool(40, Hkv, D, dtype, dev) for _ in range(4)]
+    xs = [_step_inputs(g, dev, 365, Hq, Hkv, D, dtype) for _ in range(4)]
+    want = [_step(TokenPagePool(40, Hkv, D, dtype, dev), pools[0].start(B, 8), new, x, 365, Hq, Hkv, scheme)[1] for x in xs]
+    starts = [p.start(B, 8) for p in pools]
+    torch.cuda.synchronize()
+    sides = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = [None] * 4
+    for i in range(4):
+        with torch.cuda.stream(sides[i % 2] if i < 3 else torch.cuda.default_stream(dev)):
+            got[i] = _step(pools[i], starts[i], new, xs[i], 365, Hq, Hkv, scheme)[1]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_frequencies_are_not_uploaded_during_capture(dev):
+    scheme = Vanilla(theta=123457.0, head_dim=64)
+    q, pos = torch.randn(1, 2, 5, 64, device=dev).half(), torch.arange(5, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        buf = q * 2
+        with pytest.raises(RuntimeError, match="once before capturing"):
+            rope_axes(q, None, pos, scheme)
+    want = rope_axes(q, None, pos, scheme)[0].clone()
+    graph2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph2):
+        out = rope_axes(q, None, pos, scheme)[0]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        graph2.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(buf, q * 2)
+
+
+def test_off_the_current_device(dev, monkeypatch):
+    """Every entry point makes its tensors' GPU the current one for its launch (seen on one GPU by its guard)."""
+    B, Hq, Hkv, D = 2, 4, 2, 64
+    scheme = Vanilla(theta=1e4, head_dim=D)
+    g = torch.Generator(device=dev).manual_seed(13)
+    x, new = _step_inputs(g, dev, 70, Hq, Hkv, D, F16), _i32([64, 6], dev)
+    pools = [TokenPagePool(9, Hkv, D, F16, dev) for _ in range(2)]
+    states = [p.start(B, 2) for p in pools]
+    want = _step(pools[0], states[0], new, x, 70, Hq, Hkv, scheme)[1]
+    entered, current = [], [1]
+
+    class Guard:
+        def __init__(self, device):
+            entered.append(device)
+
+        def __enter__(self):
+            current[0] = dev.index or 0
+
+        def __exit__(self, *_):
+            current[0] = 1
+
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "_GET_DEVICE", lambda: current[0])
+        m.setattr(torch.cuda, "current_device", lambda: current[0])
+        m.setattr(torch.cuda, "device", Guard)
+        got = _step(pools[1], states[1], new, x, 70, Hq, Hkv, scheme)[1]
+    assert len(entered) == 3 and torch.equal(got, want)
+
+
+def test_offsets_past_32_bits(dev):
+    """Pages and rows whose offsets pass 2^32 elements."""
+    Hq, Hkv, D = 4, 8, 128
+    page = Hkv * PAGE_TOKENS * D
+    n_pages = 2**32 // page + 6
+    k_pages, v_pages = (torch.empty(n_pages, Hkv, PAGE_TOKENS, D, dtype=BF16, device=dev) for _ in range(2))
+    lens, new = [130, 1], [130, 1]
+    ids = [n_pages - 1, 2, n_pages - 4, 2**31 // page + 1]
+    table = _i32([[ids[0], ids[1], ids[2]], [ids[3], 0, 0]], dev)
+    slots = _i32([64 * ids[i // 64] + i % 64 for i in range(130)] + [64 * ids[3]], dev)
+    g = torch.Generator(device=dev).manual_seed(17)
+    k, v = (torch.randn(131, Hkv, D, generator=g, device=dev).to(BF16) for _ in range(2))
+    paged_append(k, v, k_pages, v_pages, slots)
+    assert torch.equal(k_pages[ids[0], :, :].transpose(0, 1), k[:64]) and torch.equal(v_pages[ids[3], :, 0], v[130])
+    # queries whose tokens lie 2^32 elements apart, in the pages' memory
+    spare = k_pages.view(-1)
+    q = torch.randn(131, Hkv * Hq, D, generator=g, device=dev).to(BF16)
+    starts = _i32([0, 130, 131], dev)
+    want = paged_attention(q, k_pages, v_pages, table, _i32(lens, dev), starts)
+    ref, tol = _reference(q, k_pages, v_pages, table, lens, [0, 130, 131], 1 / math.sqrt(D), "bottom_right")
+    _check(want, ref, tol)
+    far = spare[3 * page :].as_strided((1, 2, Hq, D), (0, 2**32, D, 1))
+    far.copy_(q[:2, :Hq][None])
+    got = paged_attention(far[0], k_pages[:3, :Hq].contiguous(), v_pages[:3, :Hq].contiguous(), _i32([[2], [2]], dev), _i32([64, 64], dev),
+                          _i32([0, 1, 2], dev))
+    near = paged_attention(q[:2, :Hq].contiguous(), k_pages[:3, :Hq].contiguous(), v_pages[:3, :Hq].contiguous(), _i32([[2], [2]], dev),
+                           _i32([64, 64], dev), _i32([0, 1, 2], dev))
+    assert torch.equal(got, near)
+    scheme, pos = Vanilla(theta=1e4, head_dim=D), _i32([5, 6], dev)
+    xs = far.transpose(1, 2)
+    assert torch.equal(rope_axes(xs, None, pos, scheme)[0], rope_axes(xs.contiguous(), None, pos, scheme)[0])
