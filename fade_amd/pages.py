@@ -231,7 +231,7 @@ def page_slots(
         raise ValueError(f"{op}: reset must be a contiguous bool or uint8 [B={B}], got {reset.dtype} {list(reset.shape)}")
     sizes = (B * ppr, B, B + 1, n, n, 2, 1)
     if out is None:  # (one allocation: the table first, on its alignment)
-        buf = torch.empty(sum(sizes), dtype=i32, device=table.device)
+        buf = table.new_empty(sum(sizes))
         parts = buf.split_with_sizes(sizes)
         out = PageSlots(parts[0].view(B, ppr), *parts[1:])
         at = buf.data_ptr()
