@@ -15,7 +15,8 @@
 // rows' token starts, page starts and returned-page starts) and then writes its
 // share of the outputs: entries of the table and slots of the new tokens.  What
 // bounds it is latency (the counts' loads, the sums' barriers, a token's search
-// and table read), not the bytes.
+// and table read), not the bytes: 16 rows of 512 pages 4.0 us, 1000 rows of 1024
+// pages with 16 chunks 7.5 (8 MB, 1.2 us at a large copy's rate).
 #include "fade_common.h"
 
 namespace fade {
@@ -160,7 +161,8 @@ __global__ __launch_bounds__(kThreads) void page_slots_kernel(SlotParams p) {
   // free page number j from the head, place j behind the tail (sums below 2^32)
   const uint32_t cap = static_cast<uint32_t>(p.cap);
   auto taken = [&](int j) { return p.free_pages[(static_cast<uint32_t>(head) + static_cast<uint32_t>(j)) % cap]; };
-  // The table: a workgroup takes a row's next 1024 (256) entries, four (one) a thread.
+  // The table: a workgroup takes a row's next 1024 (256) entries, four (one) a thread (1000 rows of 1024 entries 7.5 us,
+  // one a thread 8.9).
   auto entry = [&](int j, int old, int have, int mine, int need0, int back0, bool again, int was) {
     if (again && j < old) p.free_pages[(static_cast<uint64_t>(head) + count + back0 + j) % cap] = was;
     return j >= have && j < have + mine ? taken(need0 + j - have) : (j < have ? was : 0);
@@ -265,7 +267,8 @@ FADE_API int fade_page_slots(const fade_page_slots_args* a, void* stream) {
   int64_t blocks = items > cdiv(a->n_tokens, kThreads) ? items : cdiv(a->n_tokens, kThreads);
   if (blocks > 2 * num_cus()) blocks = 2 * num_cus();
   const dim3 grid(static_cast<unsigned>(blocks));
-  // (the fewer rows an instance has, the less LDS it takes and the shorter its sums are)
+  // The fewer rows an instance has, the less LDS it takes and the shorter its sums are (in the one of 4096 rows
+  // 16 rows take 7.5 us instead of 4.0, 1000 rows 11.3 instead of 7.5).
   if (a->B <= 256) hipLaunchKernelGGL(page_slots_kernel<256>, grid, dim3(kThreads), 0, as_stream(stream), p);
   else if (a->B <= 1024) hipLaunchKernelGGL(page_slots_kernel<1024>, grid, dim3(kThreads), 0, as_stream(stream), p);
   else hipLaunchKernelGGL(page_slots_kernel<FADE_SLOTS_MAX_ROWS>, grid, dim3(kThreads), 0, as_stream(stream), p);

@@ -329,9 +329,12 @@ struct Odd {
 //
 // The wave walks its piece in steps of 32 keys.  K and V rows go from the page
 // straight to LDS (no register holds them, no barrier is needed), two steps deep:
-// the next step's loads fly while this one is computed.  Five such waves per CU
-// (head_dim 128) keep 80 KB of loads in flight, and one's start or end runs beside
-// the others' loads.
+// the next step's loads fly while this one is computed.  Four such waves per CU
+// (head_dim 128) keep 64 KB of loads in flight, and one's start or end runs beside
+// the others' loads.  Bound by HBM: 16 rows over 8000 keys each (32 heads, 8 kv
+// heads of 128) 103 us, 5.2 TB/s, as a large copy has; 64 rows of 10 to 9000 keys
+// 149 us.  Eight waves per CU 111 us, sixteen 120; three steps deep no faster.  A
+// single row of few keys is bound by latency: 6.5 us and 3.5 for the join.
 //   S^T = K Q^T   16x16x32 MFMAs, A = 16 keys x 32 channels, B = Q^T (registers):
 //                 lane (n, g) holds query row n, keys 4 g + i of the 16
 //   O^T += V^T P^T  A = V^T by transposing LDS reads (4 keys x 16 channels each),
@@ -573,9 +576,9 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
 
 // ---- many rows: tiles of 32 NW matrix rows, the keys shared through LDS ----
 //
-// NW waves of 32 matrix rows each walk the item's keys page by page.
-// A page's K and V go straight to LDS, two pages deep, every wave loading its
-// share; one barrier per page.
+// NW waves of 32 matrix rows each walk the tile's keys in steps of KT.  A step's K
+// and V go straight to LDS, NST steps' buffers in a ring, every wave loading its
+// share; one barrier per step.
 //   S^T = K Q^T   32x32x16 MFMAs, A = 32 keys x 16 channels, B = Q^T (registers):
 //                 lane (n, h) holds matrix row n, register i key 8 (i / 4) + 4 h + i % 4
 //   O^T += V^T P^T  A = V^T by transposing LDS reads, B = P^T straight from S^T's
@@ -583,10 +586,20 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
 //                 16 s + 8 + 4 h + j - 4
 // so a row's maximum, sum and rescaling are lane-local.  The running maximum moves
 // only where a probability passes 2^8 (found on the 16-bit probabilities, two per
-// operation; the exact maximum is taken there alone), so most pages need neither a
+// operation; the exact maximum is taken there alone), so most steps need neither a
 // maximum of the scores nor an exchange between lanes nor a rescaling.  P is
 // rounded to 16 bits (as the output is; the sum takes the same rounded values): a
 // second product for its rest would cost half the matrix work again.
+//
+// Eight chunks of 128 to 2048 tokens over up to 11K keys (32 heads, 8 kv heads of
+// 128): 560 to 580 us, 1040 TFLOP/s of visible keys.  What bounds it is the power
+// that the card has: its matrix instructions alone reach 1370 TFLOP/s on random
+// numbers (2200 on constant ones), with this kernel's LDS reads and exponentials
+// beside them 1296, with its loads and barriers 1090.  Measured without gain: scores
+// of the next step beside this step's exponentials, a barrier per two steps, 2 to 4
+// buffers, 64 rows per wave.  256-row tiles: 128-row ones (4 waves, two workgroups a
+// CU) 700 us against 657 then; steps of 32 keys at head_dim over 128, where the
+// accumulators and the query leave registers for one block of scores.
 // LDS rows are DP channels, 16-byte units exchanged so that the eight (16) rows
 // that a read of K touches and the four that a transposing read of V touches lie
 // in different banks.
@@ -1101,10 +1114,17 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   p.causal = a->mask_mode == FADE_MASK_BOTTOM_RIGHT;
   p.zero_tail = a->zero_tail;
   // Rows whose matrix rows fit one tile of 16 go to the few-row kernel, the others
-  // to the wide one; a call of at most 16 matrix rows per row on average is taken to
-  // be a decoding step, all of it the few-row kernel's.
+  // to the wide one (16 rows over 8192 keys each, 32 matrix rows a row: 113 us, by the
+  // few-row kernel 124; 64: 114 and 204; 128: 131 and 389); a call of at most 16 matrix
+  // rows per row on average is taken to be a decoding step, all of it the few-row
+  // kernel's (the wide kernel's launch, empty, costs such a step 2.5 us).
   const bool step = p.T * p.G <= kRows * p.B;
   pl.both = !step;
+  // The few-row kernel has as many workgroups as find a place at once (16 rows over
+  // 8192 keys: 4 per CU 104.5 us, 8 110.6, 16 120), of 64 keys or more each (a row of
+  // 1000 keys: 32 and 64 alike, 128 2 us more, 256 4); the wide one a workgroup per CU (30 decoding
+  // rows with two 512-token chunks: 241 us, two 280, three 291), a tile's start and end
+  // counted as 192 keys (64 and 512: within 2 us).
   const int per_cu = p.D <= 64 ? 8 : (p.D <= 128 ? 4 : 2);
   pl.few = pl.wide = p;
   set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), 64);

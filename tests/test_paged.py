@@ -142,7 +142,7 @@ def test_work_is_cut_into_equal_pieces():
     """Every tile's keys are walked once and in order, whole or in a beginning and ends of
     consecutive pieces, which is what the second launch joins."""
     rng = random.Random(0)
-    for _ in range(400):
+    for _ in range(80):
         B, G = rng.choice((1, 2, 5, 64, 65, 150)), rng.choice((1, 2, 4, 7, 20, 71))
         M, grain, start, least = rng.choice(((16, 32, 32, 64), (256, 64, 192, 256), (256, 32, 192, 256)))
         cap = rng.choice((5, 100, 4000)) * 64
