@@ -124,8 +124,8 @@ class PagedAttentionPlan:
         starts: int32 [B + 1], the first of each row's tokens in q and their end; ``starts[0]`` is 0.
         mask: ``"bottom_right"`` (query i of a row's n sees keys 0 .. lens - n + i) or
             ``"none"`` (all lens of them, as a decoder's queries see an encoder's states).
-        out: like q, contiguous along D; rows at and past ``starts[B]`` are left as they
-            are.  Default: a new tensor, zeros there.
+        out: like q, contiguous along D, q itself or other memory; rows at and past ``starts[B]``
+            are left as they are.  Default: a new tensor, zeros there.
 
     A query that sees no key gets zeros; a NaN or an infinity in a value reaches the
     queries that see its key and no others.  Lengths, starts and pages are read on the
@@ -162,18 +162,21 @@ class PagedAttentionPlan:
         for name, t, shape in (("table", table, (B, ppr)), ("lens", lens, (B,)), ("starts", starts, (B + 1,))):
             if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} {list(t.shape)}")
-        if q.is_neg() or q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 8 or q.data_ptr() % 16:
-            raise ValueError(f"{op}: q needs a contiguous head_dim axis and 16-byte aligned rows (call .contiguous())")
+        # (the stride of an axis of one element is never used, whatever it says)
+        q_st, q_sh = q.stride(0) if T > 1 else 0, q.stride(1) if Hq > 1 else 0
+        if q.is_neg() or q.stride(2) != 1 or (q_st | q_sh) % 8 or q.data_ptr() % 16:
+            raise ValueError(f"{op}: q needs a contiguous head_dim axis and 16-byte aligned rows (make a copy)")
         self._fresh = out is None
         if out is None:
             out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.is_neg() or out.stride(2) != 1 or (out.stride(0) | out.stride(1)) % 4 \
+        o_st, o_sh = out.stride(0) if T > 1 else D, out.stride(1) if Hq > 1 else D
+        if out.shape != q.shape or out.dtype != q.dtype or out.is_neg() or out.stride(2) != 1 or (o_st | o_sh) % 4 or not o_st or not o_sh \
                 or out.data_ptr() % 8:
             raise ValueError(f"{op}: out must be {q.dtype} {tuple(q.shape)} with a contiguous head_dim axis and 8-byte aligned rows")
         a = _lib.PagedAttnArgs()
         a.B, a.T, a.Hq, a.Hkv, a.D, a.n_pages, a.pages_per_row = B, T, Hq, Hkv, D, n_pages, ppr
-        a.q, a.q_st, a.q_sh = q.data_ptr(), q.stride(0), q.stride(1)
-        a.out, a.o_st, a.o_sh = out.data_ptr(), out.stride(0), out.stride(1)
+        a.q, a.q_st, a.q_sh = q.data_ptr(), q_st, q_sh
+        a.out, a.o_st, a.o_sh = out.data_ptr(), o_st, o_sh
         a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
         a.table, a.lens, a.starts = table.data_ptr(), lens.data_ptr(), starts.data_ptr()
         a.sm_scale = float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale)

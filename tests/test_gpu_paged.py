@@ -471,6 +471,29 @@ def test_attention_strides_tail_and_scale(dev, new):
     assert bool((out[starts[-1] :] == 7.0).all())  # the caller's: left as they were
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (6, 3, 64)])
+def test_attention_into_its_queries(dev, Hq, Hkv, D):
+    """out = q, with tiles of both kernels, cut and whole, and one that is walked again; strides of one-element axes."""
+    lens, new = [2500, 300, 1, 40, 900], [1, 300, 1, 3, 130]
+    g = torch.Generator(device=dev).manual_seed(Hq)
+    k, v, table = _pages(g, dev, lens, Hkv, D, BF16)
+    v[table[4, 13], :, 60] = math.inf
+    starts = _starts(new)
+    q = torch.randn(starts[-1] + 2, Hq, D, generator=g, device=dev).to(BF16)
+    args = (k, v, table, _i32(lens, dev), _i32(starts, dev))
+    want, rest = paged_attention(q, *args), q[starts[-1] :].clone()
+    got = paged_attention(q, *args, out=q)
+    assert got is q
+    a, b = got[: starts[-1]], want[: starts[-1]]
+    assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num()) and torch.equal(got[starts[-1] :], rest)
+    x = torch.randn(Hq, D, generator=g, device=dev).to(BF16)
+    one = x.as_strided((1, Hq, D), (3, D, 1))
+    assert torch.equal(paged_attention(one, k, v, table[:1], _i32([70], dev), _i32([0, 1], dev)),
+                       paged_attention(x[None], k, v, table[:1], _i32([70], dev), _i32([0, 1], dev)))
+    with pytest.raises(ValueError, match="out must be"):
+        paged_attention(q, *args, out=q[:1].expand(starts[-1] + 2, Hq, D))
+
+
 def test_attention_extreme_scores(dev):
     """Scores of thousands, equal keys, infinite keys: as a softmax in 64 bits has them."""
     lens, new, H, D = [130, 70, 65], [1, 2, 65], 2, 64
