@@ -16,7 +16,8 @@
 // matrix rows of a (row b, kv head); its cost is the keys that it reads and a
 // constant for its start and end.  The tiles of all rows lie one after the other on
 // a line, and every workgroup of a kv head takes an equal piece of it, whatever the
-// rows' lengths are: the end of one tile, whole tiles, the beginning of another.  A
+// rows' lengths are: the end of one tile, whole tiles, the beginning of another (a
+// border close to a tile's own is moved there, where a cut costs more than that).  A
 // wave finds its place by a sum over the rows' costs (one load per lane for 64
 // rows).  Whole tiles are written out; a tile cut by a piece's border leaves
 // unnormalized fp32 sums, at most two per workgroup, which a second launch joins in
@@ -80,6 +81,7 @@ struct Params {
   int pieces;      // workgroups per kv head
   float per_piece; // a little over 1 / pieces
   int least;       // fewest keys of a piece
+  int snap;        // a border this near to a tile's is moved there
   float* part_o;   // [workgroup][2][M][D]: a tile's end (0), a tile's beginning (1)
   float2* part_ml; // [workgroup][2][M]: maximum (log2 units), sum
   int4* cuts;      // [workgroup]: the tile that begins in its piece and ends in another: first new token, its
@@ -215,7 +217,7 @@ __device__ __forceinline__ bool find_tile(const Params& p, uint64_t x, const Row
 
 // One workgroup's walk over its piece of the line.
 struct Walk {
-  uint64_t x, end, piece;
+  uint64_t x, end, piece, snap;
   Place from;
   Row lane_row;     // the lane's row of rows 0 .. 63
   int tokens;       // new tokens of all rows (p.zero_tail)
@@ -231,20 +233,39 @@ __device__ __forceinline__ bool walk_start(const Params& p, int piece_index, Wal
   k.end = k.x + piece < all ? k.x + piece : all;
   k.from = Place{0, 0};
   k.piece = piece;
+  k.snap = piece / 4 < static_cast<uint64_t>(p.snap) ? piece / 4 : p.snap;
   k.first = k.last = false;
   return k.x < k.end;
 }
+// Where the border x, inside the tile from `at` to `end`, comes to lie: at the
+// nearer end of the tile, if that is near.
+__device__ __forceinline__ uint64_t snapped(const Walk& k, uint64_t x, uint64_t at, uint64_t end) {
+  const uint64_t d0 = x - at, d1 = end - x;
+  if ((d0 < d1 ? d0 : d1) > k.snap) return x;
+  return d0 < d1 ? at : end;
+}
 // The next tile of the piece; `grain`: keys that are not divided.
 __device__ __forceinline__ bool walk_next(const Params& p, int grain, Walk& k) {
-  if (k.x >= k.end || !find_tile(p, k.x, k.lane_row, k.from, k.w)) return false;
+  Tile t;
+  uint64_t tile_end;
+  do {
+    if (k.x >= k.end || !find_tile(p, k.x, k.lane_row, k.from, t)) return false;
+    tile_end = t.at + t.cost;
+    if (tile_end <= k.x) return false;  // (counts that contradict each other)
+    if (k.x != t.at) k.x = snapped(k, k.x, t.at, tile_end);  // the piece's begin
+  } while (k.x == tile_end);
+  uint64_t end = k.end;
+  if (end < tile_end) {
+    end = snapped(k, end, t.at, tile_end);
+    if (end == t.at) return false;
+  }
+  k.w = t;
   const Tile& w = k.w;
-  const uint64_t tile_end = w.at + w.cost;
-  if (tile_end <= k.x) return false;  // (counts that contradict each other)
   const int rows = w.n * p.G, last_row = ((w.tile + 1) << p.lm) < rows ? ((w.tile + 1) << p.lm) : rows;
   int seen = p.causal ? w.len - w.n + (last_row - 1) / p.G + 1 : w.len;  // keys that the tile's last row sees
   seen = seen < 0 ? 0 : seen;
   k.first = k.x == w.at;
-  k.last = tile_end <= k.end;
+  k.last = tile_end <= end;
   const int a = static_cast<int>(k.x - w.at) / grain * grain, e = static_cast<int>(k.end - w.at) / grain * grain;
   k.lo = a < seen ? a : seen;
   k.hi = k.last || e > seen ? seen : e;
@@ -274,7 +295,8 @@ __device__ __forceinline__ void finish(const Params& p, const Walk& k, bool any)
     parts = static_cast<int>(static_cast<double>(rest) / static_cast<double>(k.piece));  // (a whole number or two off)
     if (parts > 0) --parts;
     while (k.piece * static_cast<uint64_t>(parts) < rest && parts < p.pieces) ++parts;
-    ++parts;
+    // (the last border in the tile may be the tile's own)
+    if (parts < 2 || rest - k.piece * static_cast<uint64_t>(parts - 1) > k.snap) ++parts;
   }
   p.cuts[blockIdx.x] = make_int4(k.w.q0, k.w.tile << p.lm, k.w.n * p.G, parts);
 }
@@ -1054,12 +1076,13 @@ struct Plan {
   bool both;  // the wide kernel runs too
 };
 
-void set_cut(Params& p, int rows_of, int lm, int start_cost, int64_t workgroups, int least) {
+void set_cut(Params& p, int rows_of, int lm, int start_cost, int64_t workgroups, int least, int snap) {
   p.rows_of = rows_of;
   p.lm = lm;
   p.per_tile = static_cast<int>(cdiv(1 << lm, p.G));
   p.start_cost = start_cost;
   p.least = least;
+  p.snap = snap;
   // pieces: no more than the longest line that the tensors allow has of the least size
   const int64_t tiles = p.T * p.G / (1 << lm) + (p.B < p.T ? p.B : p.T);
   const int64_t line = tiles * (p.ppr * kPage + p.start_cost + p.per_tile);
@@ -1124,11 +1147,14 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   // 8192 keys: 4 per CU 104.5 us, 8 110.6, 16 120), of 64 keys or more each (a row of
   // 1000 keys: 32 and 64 alike, 128 2 us more, 256 4); the wide one a workgroup per CU (30 decoding
   // rows with two 512-token chunks: 241 us, two 280, three 291), a tile's start and end
-  // counted as 192 keys (64 and 512: within 2 us).
+  // counted as 192 keys (64 and 512: within 2 us), and a border within 256 keys of a
+  // tile's, and a quarter of a piece, moved there: the fp32 sums of a cut tile cost as
+  // much (three prompts at head_dim 256 151 us, so 135; eight of 512 tokens 77 and 60; long
+  // chunks alike; 512 keys: two chunks beside decoding rows 218 instead of 216).
   const int per_cu = p.D <= 64 ? 8 : (p.D <= 128 ? 4 : 2);
   pl.few = pl.wide = p;
-  set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), 64);
-  set_cut(pl.wide, kMany, kWideLog, 192, num_cus(), 256);
+  set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), 64, 0);
+  set_cut(pl.wide, kMany, kWideLog, 192, num_cus(), 256, 256);
   pl.wide.zero_tail = 0;
   return FADE_OK;
 }

@@ -88,7 +88,7 @@ def test_slots_and_rope_arguments():
     assert _call("fade_rope_axes", a, None) == 0
 
 
-def _cut(lens, new, G, M, causal, start_cost, pieces, least, grain):
+def _cut(lens, new, G, M, causal, start_cost, pieces, least, grain, snap):
     """What every piece of the line does (walk_start, walk_next and finish of paged_attn.hip), in
     its precision: [(piece, row, tile, first key, last key, first, last)], the cuts {piece: parts}."""
     f = np.float32
@@ -106,6 +106,12 @@ def _cut(lens, new, G, M, causal, start_cost, pieces, least, grain):
     piece = max(least, int(f(f(line) * f(f(1.00002) / f(pieces)))) + 1)
     assert piece * pieces >= line
     done, cuts = [], {}
+    snap = min(snap, piece // 4)
+
+    def snapped(x, at, to):
+        near = at if x - at < to - x else to
+        return near if abs(near - x) <= snap else x
+
     for w in range(pieces):
         x, end = w * piece, min(w * piece + piece, line)
         tail = None
@@ -121,9 +127,15 @@ def _cut(lens, new, G, M, causal, start_cost, pieces, least, grain):
                 t += 1
             at, c = rows_at[b] + cost(b, t), cost(b, t + 1) - cost(b, t)
             assert at <= x < at + c
+            x = snapped(x, at, at + c) if x != at else x
+            if x == at + c:
+                continue
+            to = snapped(end, at, at + c) if end < at + c else end
+            if to == at:
+                break
             last_row = min((t + 1) * M, new[b] * G) - 1
             seen = max(0, lens[b] - new[b] + last_row // G + 1 if causal else lens[b])
-            first, last = x == at, at + c <= end
+            first, last = x == at, at + c <= to
             lo = min((x - at) // grain * grain, seen)
             hi = seen if last else min((end - at) // grain * grain, seen)
             done.append((w, b, t, lo, hi, first, last))
@@ -134,7 +146,7 @@ def _cut(lens, new, G, M, causal, start_cost, pieces, least, grain):
             parts = max(int(rest / piece) - 1, 0)
             while piece * parts < rest and parts < pieces:
                 parts += 1
-            cuts[w] = parts + 1
+            cuts[w] = parts + (parts < 2 or rest - piece * (parts - 1) > snap)
     return tiles, done, cuts
 
 
@@ -144,12 +156,12 @@ def test_work_is_cut_into_equal_pieces():
     rng = random.Random(0)
     for _ in range(80):
         B, G = rng.choice((1, 2, 5, 64, 65, 150)), rng.choice((1, 2, 4, 7, 20, 71))
-        M, grain, start, least = rng.choice(((16, 32, 32, 64), (256, 64, 192, 256), (256, 32, 192, 256)))
+        M, grain, start, least, snap = rng.choice(((16, 32, 32, 64, 0), (256, 64, 192, 256, 256), (256, 32, 192, 256, 256)))
         cap = rng.choice((5, 100, 4000)) * 64
         lens = [rng.randint(0, cap) if rng.random() < 0.7 else rng.randint(0, min(cap, 90)) for _ in range(B)]
         new = [rng.choice((0, 1, 1, rng.randint(0, 3000 // G), n)) if n < 20000 else rng.choice((0, 1, 700)) for n in lens]
         pieces, causal = rng.choice((1, 3, 32, 127, 512)), rng.random() < 0.7
-        tiles, done, cuts = _cut(lens, new, G, M, causal, start, pieces, least, grain)
+        tiles, done, cuts = _cut(lens, new, G, M, causal, start, pieces, least, grain, snap)
         by_tile, slots = {}, set()
         for w, b, t, lo, hi, first, last in done:
             by_tile.setdefault((b, t), []).append((w, lo, hi, first, last))
