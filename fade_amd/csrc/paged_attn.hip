@@ -233,7 +233,7 @@ __device__ __forceinline__ bool walk_start(const Params& p, int piece_index, Wal
   k.end = k.x + piece < all ? k.x + piece : all;
   k.from = Place{0, 0};
   k.piece = piece;
-  k.snap = piece / 4 < static_cast<uint64_t>(p.snap) ? piece / 4 : p.snap;
+  k.snap = piece / 3 < static_cast<uint64_t>(p.snap) ? piece / 3 : p.snap;
   k.first = k.last = false;
   return k.x < k.end;
 }
@@ -1147,14 +1147,15 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   // 8192 keys: 4 per CU 104.5 us, 8 110.6, 16 120), of 64 keys or more each (a row of
   // 1000 keys: 32 and 64 alike, 128 2 us more, 256 4); the wide one a workgroup per CU (30 decoding
   // rows with two 512-token chunks: 241 us, two 280, three 291), a tile's start and end
-  // counted as 192 keys (64 and 512: within 2 us), and a border within 256 keys of a
-  // tile's, and a quarter of a piece, moved there: the fp32 sums of a cut tile cost as
-  // much (three prompts at head_dim 256 151 us, so 135; eight of 512 tokens 77 and 60; long
-  // chunks alike; 512 keys: two chunks beside decoding rows 218 instead of 216).
+  // counted as 300 keys (a prompt of 4096 tokens 184 us, four of 1000 at head_dim 256
+  // 84; as 192: 200 and 97, as 500: 182 and 96, and eight of 512 74 instead of 61), and a
+  // border within 256 keys of a tile's, and a third of a piece, moved there: the fp32
+  // sums of a cut tile cost as much (three prompts at head_dim 256 134 us, unmoved 151;
+  // eight of 512 tokens 61 and 77; long chunks alike).
   const int per_cu = p.D <= 64 ? 8 : (p.D <= 128 ? 4 : 2);
   pl.few = pl.wide = p;
   set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), 64, 0);
-  set_cut(pl.wide, kMany, kWideLog, 192, num_cus(), 256, 256);
+  set_cut(pl.wide, kMany, kWideLog, 300, num_cus(), 256, 256);
   pl.wide.zero_tail = 0;
   return FADE_OK;
 }

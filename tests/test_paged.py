@@ -106,7 +106,7 @@ def _cut(lens, new, G, M, causal, start_cost, pieces, least, grain, snap):
     piece = max(least, int(f(f(line) * f(f(1.00002) / f(pieces)))) + 1)
     assert piece * pieces >= line
     done, cuts = [], {}
-    snap = min(snap, piece // 4)
+    snap = min(snap, piece // 3)
 
     def snapped(x, at, to):
         near = at if x - at < to - x else to
@@ -156,7 +156,7 @@ def test_work_is_cut_into_equal_pieces():
     rng = random.Random(0)
     for _ in range(80):
         B, G = rng.choice((1, 2, 5, 64, 65, 150)), rng.choice((1, 2, 4, 7, 20, 71))
-        M, grain, start, least, snap = rng.choice(((16, 32, 32, 64, 0), (256, 64, 192, 256, 256), (256, 32, 192, 256, 256)))
+        M, grain, start, least, snap = rng.choice(((16, 32, 32, 64, 0), (256, 64, 300, 256, 256), (256, 32, 300, 256, 256)))
         cap = rng.choice((5, 100, 4000)) * 64
         lens = [rng.randint(0, cap) if rng.random() < 0.7 else rng.randint(0, min(cap, 90)) for _ in range(B)]
         new = [rng.choice((0, 1, 1, rng.randint(0, 3000 // G), n)) if n < 20000 else rng.choice((0, 1, 700)) for n in lens]
