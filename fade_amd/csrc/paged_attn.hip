@@ -365,6 +365,9 @@ struct Odd {
 // so the running maximum, the sum and the rescaling are lane-local; P is multiplied
 // as a 16-bit head plus a 16-bit rest (P to 2^-16 or better): the matrix cores are
 // idle here, and rounding P alone would cost as much accuracy as rounding the output.
+// fp16 holds nothing finer than 2^-24, and where one key takes the weight (a sink)
+// the output is what many light ones add up to: P and its sum are held 2^15 times
+// larger there, P to 2^-40 of the largest.
 // 16-byte unit u of LDS row r lies at unit u ^ (2 (r & 7)) (mod the row), which the
 // loads' source addresses bring about: without it the 16 rows that a transposing
 // read touches would share their banks.
@@ -379,6 +382,7 @@ struct Few {
   static constexpr int kQBytes = kRows * DP * 2;
   static constexpr int kLds = kStages * kStage + kQBytes;
   static constexpr int kSwizzle = kUnits - 1;
+  static constexpr float kHeld = 15.0f;            // log2 of the factor on fp16 probabilities, which are 1 at most
 };
 
 template <int DP>
@@ -520,7 +524,12 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
         u32x4 ph, pl;
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-          const float a = __builtin_amdgcn_exp2f(x[i] - ms), b = __builtin_amdgcn_exp2f(x[i + 1] - ms);
+          float da = x[i] - ms, db = x[i + 1] - ms;
+          if constexpr (!BF) {  // (2^15 times, not added to ms: its rounding there would differ from step to step)
+            da += F::kHeld;
+            db += F::kHeld;
+          }
+          const float a = __builtin_amdgcn_exp2f(da), b = __builtin_amdgcn_exp2f(db);
           ps += a + b;
           const uint32_t h = pack2<BF>(a, b);
           ph[i / 2] = h;
