@@ -616,11 +616,15 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
 //                 registers: k slot (h, j) of step s is key 16 s + 4 h + j (j < 4),
 //                 16 s + 8 + 4 h + j - 4
 // so a row's maximum, sum and rescaling are lane-local.  The running maximum moves
-// only where a probability passes 2^8 (found on the 16-bit probabilities, two per
-// operation; the exact maximum is taken there alone), so most steps need neither a
-// maximum of the scores nor an exchange between lanes nor a rescaling.  P is
+// only where a probability passes 2^8 (fp16: 2^6; found on the 16-bit probabilities,
+// two per operation; the exact maximum is taken there alone), so most steps need
+// neither a maximum of the scores nor an exchange between lanes nor a rescaling.  P is
 // rounded to 16 bits (as the output is; the sum takes the same rounded values): a
-// second product for its rest would cost half the matrix work again.
+// second product for its rest would cost half the matrix work again.  fp16
+// probabilities are held 2^9 times larger, so that a key 2^23 times lighter than the
+// heaviest one still counts with all 11 bits (2^34 times lighter: not at all); eight
+// chunks of 128 to 2048 tokens 505 us, not held larger 501, 2^11 times 515, 2^12 times
+// 525 (they pass their bound, and are rescaled, more often).
 //
 // Eight chunks of 128 to 2048 tokens over up to 11K keys (32 heads, 8 kv heads of
 // 128): 560 to 580 us, 1040 TFLOP/s of visible keys.  What bounds it is the power
@@ -717,6 +721,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     buf = buf == NST - 1 ? 0 : buf + 1;
   };
   const float sl2 = p.scale_log2;
+  // what a probability's exponent adds to the score's: the maximum's, and log2 of the factor on fp16 probabilities
+  auto held = [&](float m) { return fmaf(-m, sl2, BF ? 0.0f : 9.0f); };
   while (walk_next(p, KT, k)) {
     const Tile& w = k.w;
     const int all = w.n * p.G;  // the row's matrix rows
@@ -866,7 +872,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         }
         u32x4 pa[2 * NKB];
         auto probs = [&]() {
-          const float nm = -m * sl2;
+          const float nm = held(m);
 #pragma unroll
           for (int st = 0; st < 2 * NKB; ++st)
 #pragma unroll
@@ -880,7 +886,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         if constexpr (NKB == 2)
           pm = __builtin_elementwise_max(pm, __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[2]), __builtin_bit_cast(u16x8, pa[3])));
         const auto p2 = __builtin_elementwise_max(__builtin_elementwise_max(pm.s01, pm.s23), __builtin_elementwise_max(pm.s45, pm.s67));
-        constexpr uint16_t kOver = BF ? 0x4380 : 0x5C00;  // 2^8
+        constexpr uint16_t kOver = BF ? 0x4380 : 0x7800;  // 2^8, 2^9 * 2^6
         const bool over = __builtin_amdgcn_ballot_w64(p2.x > kOver || p2.y > kOver) != 0;
         if (over || odd) {  // (one branch for what is rare)
           if (over) {
@@ -891,7 +897,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
               for (int i = 0; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[kb][i], s[kb][i + 1]));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const float mn = fmaxf(m, mx);
-            const float alpha = __builtin_amdgcn_exp2f((m - mn) * sl2);
+            const float alpha = __builtin_amdgcn_exp2f(held(mn) - held(m));
             m = mn;
             l *= alpha;
 #pragma unroll
@@ -959,7 +965,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const float lt = l + __shfl_xor(l, 32, 64);
     if (live && part) {
       const int64_t pr = (static_cast<int64_t>(blockIdx.x) * 2 + (k.first ? 1 : 0)) * M + 32 * wave + n32;
-      if (h == 0) p.part_ml[pr] = make_float2(m * sl2, lt);
+      if (h == 0) p.part_ml[pr] = make_float2(-held(m), lt);
 #pragma unroll
       for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll

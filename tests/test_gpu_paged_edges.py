@@ -22,7 +22,7 @@ def _rows(x, table, L):
 
 @pytest.mark.parametrize("gap", [10, 16, 20, 24, 28])
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("B,new", [(600, 1)])  # a tile of 16 matrix rows or more to a workgroup
+@pytest.mark.parametrize("B,new", [(600, 1), (150, 40)])  # tiles of 16 and of 256 matrix rows, one or more to a workgroup
 def test_attention_of_a_light_tail(dev, B, new, dtype, gap):
     """One key takes the weight and has no value (an attention sink): the output is what keys 2^gap times lighter add up to."""
     L, Hq, Hkv, D = 450, 4, 2, 64
@@ -49,5 +49,5 @@ def test_attention_of_a_light_tail(dev, B, new, dtype, gap):
     u, few = torch.finfo(dtype).eps / 2, new == 1
     tol = (u + 2.0**-15 + (0 if few else 2 * u)) * want.abs()
     if dtype == F16:  # what fp16 cannot hold of a probability, next to one of 1: 2^-25 of the factor that they are held with
-        tol += L * 384 * (2.0**-40 if few else 2.0**-36)
+        tol += L * 384 * (2.0**-40 if few else 2.0**-34)
     _check(got, want, tol, f"gap {gap}")
