@@ -49,7 +49,7 @@ typedef __attribute__((address_space(4))) int32_t const_i32;
 constexpr int kThreads = 256;
 constexpr int kPage = 64;
 constexpr int kRows = 16;  // matrix rows of an item of the few-row kernel
-constexpr float kNegBig = -1.0e30f;
+constexpr float kNegBig = -3.402823466e38f;  // no score is lower
 
 template <int V>
 struct Int {
@@ -721,8 +721,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     buf = buf == NST - 1 ? 0 : buf + 1;
   };
   const float sl2 = p.scale_log2;
-  // what a probability's exponent adds to the score's: the maximum's, and log2 of the factor on fp16 probabilities
-  auto held = [&](float m) { return fmaf(-m, sl2, BF ? 0.0f : 9.0f); };
+  // What a probability's exponent adds to the score's: the maximum's, and log2 of the factor on fp16 probabilities.
+  // Far from zero both products are rounded by more than 1: the sum is kept from falling short (2^-22 of its size
+  // covers three roundings), which would leave the maximum itself no weight, and where it exceeds by more than the
+  // bound on probabilities, the scores' differences are taken first.
+  constexpr float kHeld = BF ? 0.0f : 9.0f, kBound = BF ? 8.0f : 6.0f;
+  auto held = [&](float m) {
+    const float t = m * sl2;
+    return fminf(fmaf(fabsf(t), 0x1p-22f, kHeld - t), 3.0e38f);
+  };
   while (walk_next(p, KT, k)) {
     const Tile& w = k.w;
     const int all = w.n * p.G;  // the row's matrix rows
@@ -871,8 +878,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
               if (left <= 32 * kb + 8 * (i >> 2) + (i & 3)) s[kb][i] = -INFINITY;
         }
         u32x4 pa[2 * NKB];
-        auto probs = [&]() {
-          const float nm = held(m);
+        auto probs = [&](float nm) {
 #pragma unroll
           for (int st = 0; st < 2 * NKB; ++st)
 #pragma unroll
@@ -880,7 +886,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
               pa[st][j] = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j], sl2, nm)),
                                     __builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j + 1], sl2, nm)));
         };
-        probs();
+        probs(held(m));
         // 16-bit patterns of the non-negative probabilities order as their values do
         u16x8 pm = __builtin_elementwise_max(__builtin_bit_cast(u16x8, pa[0]), __builtin_bit_cast(u16x8, pa[1]));
         if constexpr (NKB == 2)
@@ -897,14 +903,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
               for (int i = 0; i < 16; i += 2) mx = fmaxf(mx, fmaxf(s[kb][i], s[kb][i + 1]));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const float mn = fmaxf(m, mx);
-            const float alpha = __builtin_amdgcn_exp2f(held(mn) - held(m));
+            float nm = held(mn);
+            const float alpha = __builtin_amdgcn_exp2f(fminf(nm - held(m), 0.0f));
             m = mn;
             l *= alpha;
 #pragma unroll
             for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
               for (int i = 0; i < 16; ++i) acc[cb][i] *= alpha;
-            probs();
+            const bool far = fmaf(m, sl2, nm) > kHeld + kBound + 0.25f;  // (0.25: a bound that rounding may have met is met here too)
+            if (__builtin_amdgcn_ballot_w64(far) != 0) {
+              const float less = far ? m : 0.0f;
+              nm = far ? kHeld : nm;
+#pragma unroll
+              for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][i] -= less;
+            }
+            probs(nm);
           }
           if (odd) {
 #pragma unroll 1

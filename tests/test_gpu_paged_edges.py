@@ -9,7 +9,7 @@ import torch
 
 from fade_amd.kernels import paged_attention
 from fade_amd.pages import PAGE_TOKENS
-from test_gpu_paged import BF16, F16, _check, _i32, _pages, _starts
+from test_gpu_paged import BF16, F16, _check, _i32, _pages, _reference, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,42 @@ def test_attention_of_a_light_tail(dev, B, new, dtype, gap):
     if dtype == F16:  # what fp16 cannot hold of a probability, next to one of 1: 2^-25 of the factor that they are held with
         tol += L * 384 * (2.0**-40 if few else 2.0**-34)
     _check(got, want, tol, f"gap {gap}")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scale", [1e3, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("lens,new", [([300, 1, 700], [1, 1, 1]), ([300, 64, 1000], [300, 33, 150]), ([2000], [700])])
+def test_attention_of_far_scores(dev, lens, new, scale, dtype):
+    """Whole scores times a large factor: the mean of the values whose scores are the largest."""
+    Hq, Hkv, D = 6, 3, 64
+    g = torch.Generator(device=dev).manual_seed(len(lens))
+    k, v, table = _pages(g, dev, lens, Hkv, D, dtype)
+    k.copy_(torch.randint(-4, 5, k.shape, generator=g, device=dev))
+    starts = _starts(new)
+    q = torch.randint(-4, 5, (starts[-1], Hq, D), generator=g, device=dev).to(dtype)
+    for mask in ("bottom_right", "none"):
+        got = paged_attention(q, k, v, table, _i32(lens, dev), _i32(starts, dev), sm_scale=scale, mask=mask)
+        # (differences of at least 1 are at least 1443 powers of two: nothing is left of any other key in 64 bits)
+        want, _ = _reference(q, k, v, table, lens, starts, scale, mask)
+        # equal keys have equal probabilities, which their sum takes as they are: the sums' roundings and the output's
+        tol = (torch.finfo(dtype).eps / 2 + 2.0**-17) * want.abs() + 2.0**-17 * float(v.abs().max())
+        _check(got, want, tol, mask)
+
+
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("scale", [2.0**-106, 1.0])
+def test_attention_of_far_negative_scores(dev, new, scale):
+    """Products of -2^106 and less: a query's keys are seen however low they all score."""
+    L, H, D = 500, 2, 64
+    g = torch.Generator(device=dev).manual_seed(new)
+    k, v, table = _pages(g, dev, [L], H, D, BF16)
+    q = torch.zeros(new, H, D, device=dev, dtype=BF16)
+    q[..., 0] = 2.0**53
+    k.zero_()
+    k[..., 0] = -(2.0**53) * torch.randint(1, 9, k.shape[:3], generator=g, device=dev).to(BF16)
+    got = paged_attention(q, k, v, table, _i32([L], dev), _i32([0, new], dev), sm_scale=scale)
+    want, _ = _reference(q, k, v, table, [L], [0, new], scale, "bottom_right")
+    # exact products; exponents of 12 at most that count: the roundings of the output, of each probability and of their sum,
+    # and 2^-17 for the exponents' and the sums' in fp32
+    u = torch.finfo(BF16).eps / 2
+    _check(got, want, (u + 2.0**-17) * want.abs() + (2 * u + 2.0**-17) * float(v.abs().max()))
