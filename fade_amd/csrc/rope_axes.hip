@@ -157,8 +157,10 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
       for (int e = 0; e < V; ++e) {
         const float xf = to_f32(a.e[e]), yf = to_f32(c.e[e]);
         // (as they stand: the same operations in every instance)
-        a.e[e] = from_f32<T>(__fmaf_rn(xf, cs[e], -__fmul_rn(yf, sn[e])));
-        c.e[e] = from_f32<T>(__fmaf_rn(yf, cs[e], __fmul_rn(xf, sn[e])));
+        float lo = __fmaf_rn(xf, cs[e], -__fmul_rn(yf, sn[e])), hi = __fmaf_rn(yf, cs[e], __fmul_rn(xf, sn[e]));
+        asm("" : "+v"(lo), "+v"(hi));  // (fp32 sums: the compiler joins some with their rounding to fp16, others not)
+        a.e[e] = from_f32<T>(lo);
+        c.e[e] = from_f32<T>(hi);
       }
     }
     *reinterpret_cast<Vt*>(dst + c0) = a;

@@ -1,4 +1,5 @@
-"""The paged attention where its numbers are hard, against softmaxes in 64 bits."""
+"""The paged attention where its numbers are hard, against softmaxes in 64 bits, and rotations that must
+not depend on how their rows lie in memory."""
 
 from __future__ import annotations
 
@@ -7,9 +8,10 @@ import math
 import pytest
 import torch
 
-from fade_amd.kernels import paged_attention
-from fade_amd.pages import PAGE_TOKENS
-from test_gpu_paged import BF16, F16, _check, _i32, _pages, _reference, _starts
+from fade_amd.kernels import paged_append, paged_attention
+from fade_amd.pages import PAGE_TOKENS, TokenPagePool
+from fade_amd.rope import MRope, Vanilla, rope_axes
+from test_gpu_paged import BF16, F16, F32, _check, _i32, _pages, _reference, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +92,29 @@ def test_attention_of_far_negative_scores(dev, new, scale):
     # and 2^-17 for the exponents' and the sums' in fp32
     u = torch.finfo(BF16).eps / 2
     _check(got, want, (u + 2.0**-17) * want.abs() + (2 * u + 2.0**-17) * float(v.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("scheme", [Vanilla(theta=1e6, head_dim=128), MRope(theta=1e6, head_dim=128, partial_rotary_factor=0.25)])
+def test_rotation_of_unaligned_rows(dev, scheme, dtype):
+    """Bit for bit that of aligned rows, and the two halves of a row alike: one fp32 sum, rounded to the type."""
+    B, H, S, D = 2, 16, 200, 128
+    g = torch.Generator(device=dev).manual_seed(7)
+    x = torch.randn(B, H, S, D, generator=g, device=dev).to(dtype)
+    pos = torch.randint(0, 5000, (B, S), generator=g, device=dev)
+    want, _ = rope_axes(x, None, pos, scheme)
+    buf = torch.zeros(B, H, S, D + 1, device=dev, dtype=dtype)
+    buf[..., 1:] = x
+    assert torch.equal(rope_axes(buf[..., 1:], None, pos, scheme)[0], want)
+    # (x, y) and (-y, x) turn into (a, b) and (-b, a)
+    h = len(scheme.freq_axes())
+    y = torch.cat([-x[..., h : 2 * h], x[..., :h], x[..., 2 * h :]], -1)
+    other, _ = rope_axes(y, None, pos, scheme)
+    assert torch.equal(other[..., h : 2 * h], want[..., :h]) and torch.equal(-other[..., :h], want[..., h : 2 * h])
+    if dtype != F32:
+        pool = TokenPagePool(-(-B * S // PAGE_TOKENS), H, D, dtype, dev)
+        k = torch.zeros(B * S, H, D + 1, device=dev, dtype=dtype)[..., 1:]
+        k.copy_(x.transpose(1, 2).reshape(B * S, H, D))
+        paged_append(k, k, pool.k, pool.v, torch.arange(B * S, device=dev).int() + PAGE_TOKENS, positions=pos.reshape(-1), scheme=scheme)
+        got = pool.k[1:].transpose(1, 2).reshape(-1, H, D)[: B * S]
+        assert torch.equal(got.view(B, S, H, D).transpose(1, 2), want)
