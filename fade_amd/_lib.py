@@ -322,11 +322,15 @@ def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
 
 
 def no_gradient(op: str, *tensors: torch.Tensor | None) -> None:
-    """Refuse a call that would have to record a gradient: the op has no backward pass."""
+    """Refuse a call that would have to record a gradient, or to carry a forward-mode tangent on: the op has neither."""
     for t in tensors:
         if t is not None and t.requires_grad:
             if torch.is_grad_enabled():
                 raise ValueError(f"{op}: has no backward pass (call it under torch.no_grad())")
+    if torch.autograd.forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and t.is_floating_point() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{op}: has no forward-mode derivative (take the primal of torch.autograd.forward_ad.unpack_dual)")
 
 
 def written(op: str, *tensors: torch.Tensor) -> None:

@@ -1,5 +1,5 @@
 """The paged attention where its numbers are hard, against softmaxes in 64 bits, and rotations that must
-not depend on how their rows lie in memory."""
+not depend on how their rows lie in memory; what the paged operators refuse."""
 
 from __future__ import annotations
 
@@ -7,6 +7,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from fade_amd.kernels import paged_append, paged_attention
 from fade_amd.pages import PAGE_TOKENS, TokenPagePool
@@ -118,3 +119,21 @@ def test_rotation_of_unaligned_rows(dev, scheme, dtype):
         paged_append(k, k, pool.k, pool.v, torch.arange(B * S, device=dev).int() + PAGE_TOKENS, positions=pos.reshape(-1), scheme=scheme)
         got = pool.k[1:].transpose(1, 2).reshape(-1, H, D)[: B * S]
         assert torch.equal(got.view(B, S, H, D).transpose(1, 2), want)
+
+
+def test_forward_mode_is_refused(dev):
+    """A tangent would be lost: the calls that would lose it raise, whichever tensor has it."""
+    D = 64
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, pages = (torch.randn(s, generator=g, device=dev).half() for s in ((5, 2, D), (3, 2, PAGE_TOKENS, D)))
+    ints = (_i32([[1, 2]], dev), _i32([70], dev), _i32([0, 5], dev))
+    scheme, pos = Vanilla(theta=1e4, head_dim=D), torch.arange(5, device=dev)
+    slots = pos.int() + PAGE_TOKENS
+    calls = [lambda x, p: paged_attention(x, p, p, *ints), lambda x, p: rope_axes(x[None], None, pos[:2], scheme),
+             lambda x, p: paged_append(x, x, p, p.clone(), slots, q=x, positions=pos, scheme=scheme)]
+    for call in calls:
+        call(q, pages.clone())
+        with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+            call(forward_ad.make_dual(q, torch.ones_like(q)), pages.clone())
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        calls[0](q, forward_ad.make_dual(pages, torch.ones_like(pages)))
