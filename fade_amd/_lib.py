@@ -9,6 +9,7 @@ when it is handed a CPU tensor.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -341,6 +342,23 @@ def written(op: str, *tensors: torch.Tensor) -> None:
                 raise RuntimeError(f"{op}: in-place write to an inference tensor outside inference mode")
         else:
             torch.autograd.graph.increment_version(t)
+
+
+@functools.lru_cache(maxsize=4096)
+def _places_differ(shape: tuple, stride: tuple) -> bool:
+    reach = 0
+    for st, n in sorted(zip(stride, shape)):
+        if n > 1:
+            if st <= reach:
+                return False
+            reach += st * (n - 1)
+    return True
+
+
+def each_once(t: torch.Tensor) -> bool:
+    """Whether every element of ``t`` has a place of its own (every stride passes what the smaller
+    ones reach): an output whose rows repeat would be written by several threads at once."""
+    return t.is_contiguous() or _places_differ(tuple(t.shape), t.stride())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -69,8 +69,9 @@ def paged_append(
         raise ValueError(f"{op}: a scheme needs positions, and positions a scheme")
     if scheme is None and q is not None:
         raise ValueError(f"{op}: q is taken to be rotated, which needs a scheme")
-    if q_out is not None and (q is None or q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1 or q_out.is_neg()):
-        raise ValueError(f"{op}: q_out must be like q with a contiguous head_dim axis")
+    if q_out is not None and (q is None or q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1 or q_out.is_neg()
+                              or not _lib.each_once(q_out)):
+        raise ValueError(f"{op}: q_out must be like q with a contiguous head_dim axis and no row twice")
     if scheme is None:
         a = _lib.RopeArgs()
         a.n_axes = 1
@@ -170,9 +171,9 @@ class PagedAttentionPlan:
         if out is None:
             out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
         o_st, o_sh = out.stride(0) if T > 1 else D, out.stride(1) if Hq > 1 else D
-        if out.shape != q.shape or out.dtype != q.dtype or out.is_neg() or out.stride(2) != 1 or (o_st | o_sh) % 4 or not o_st or not o_sh \
-                or out.data_ptr() % 8:
-            raise ValueError(f"{op}: out must be {q.dtype} {tuple(q.shape)} with a contiguous head_dim axis and 8-byte aligned rows")
+        if out.shape != q.shape or out.dtype != q.dtype or out.is_neg() or out.stride(2) != 1 or (o_st | o_sh) % 4 \
+                or not _lib.each_once(out) or out.data_ptr() % 8:
+            raise ValueError(f"{op}: out must be {q.dtype} {tuple(q.shape)} with a contiguous head_dim axis, 8-byte aligned rows and no row twice")
         a = _lib.PagedAttnArgs()
         a.B, a.T, a.Hq, a.Hkv, a.D, a.n_pages, a.pages_per_row = B, T, Hq, Hkv, D, n_pages, ppr
         a.q, a.q_st, a.q_sh = q.data_ptr(), q_st, q_sh

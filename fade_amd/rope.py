@@ -515,8 +515,9 @@ def rope_axes(
         if o is None:
             o = torch.empty_like(t, memory_format=torch.contiguous_format)  # (half the time of torch.empty)
         else:
-            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(3) != 1 or o.is_neg():
-                raise ValueError(f"{op}: out must be like the input with a contiguous head_dim axis, got {o.dtype} {tuple(o.shape)}")
+            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or o.stride(3) != 1 or o.is_neg() or not _lib.each_once(o):
+                raise ValueError(f"{op}: out must be like the input with a contiguous head_dim axis and no row twice, got {o.dtype} "
+                                 f"{tuple(o.shape)} with strides {o.stride()}")
             _lib.no_gradient(op, o)
             _lib.written(op, o)
         st, so = t.stride(), o.stride()

@@ -137,3 +137,24 @@ def test_forward_mode_is_refused(dev):
             call(forward_ad.make_dual(q, torch.ones_like(q)), pages.clone())
     with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
         calls[0](q, forward_ad.make_dual(pages, torch.ones_like(pages)))
+
+
+def test_outputs_of_repeated_rows_are_refused(dev):
+    D, T = 64, 6
+    g = torch.Generator(device=dev).manual_seed(2)
+    q = torch.randn(T, 4, D, generator=g, device=dev).half()
+    pages = torch.randn(3, 4, PAGE_TOKENS, D, generator=g, device=dev).half()
+    scheme, pos = Vanilla(theta=1e4, head_dim=D), torch.arange(T, device=dev)
+    room = torch.zeros(T * 4 * D + 8, device=dev).half()
+    for out in (q[:1].expand(T, 4, D), q[:, :1].expand(T, 4, D), room.as_strided((T, 4, D), (2 * D, D, 1)), room.as_strided((T, 4, D), (4 * D, D - 4, 1))):
+        with pytest.raises(ValueError, match="no row twice"):
+            rope_axes(q.transpose(0, 1)[None], None, pos, scheme, out=(out.transpose(0, 1)[None], None))
+        with pytest.raises(ValueError, match="no row twice"):
+            paged_append(q, q, pages, pages.clone(), pos.int() + PAGE_TOKENS, q=q, positions=pos, scheme=scheme, q_out=out)
+        with pytest.raises(ValueError, match="no row twice"):
+            paged_attention(q, pages, pages, _i32([[1]], dev), _i32([T], dev), _i32([0, T], dev), out=out)
+    assert not room.any()
+    other = room[: T * 4 * D].view(4, T, D).transpose(0, 1)  # rows in another order are fine
+    assert rope_axes(q.transpose(0, 1)[None], None, pos, scheme, out=(other.transpose(0, 1)[None], None))[0] is not None
+    paged_append(q, q, pages, pages.clone(), pos.int() + PAGE_TOKENS, q=q, positions=pos, scheme=scheme, q_out=other)
+    paged_attention(q, pages, pages, _i32([[1]], dev), _i32([T], dev), _i32([0, T], dev), out=other)
