@@ -361,6 +361,65 @@ def each_once(t: torch.Tensor) -> bool:
     return t.is_contiguous() or _places_differ(tuple(t.shape), t.stride())
 
 
+@functools.lru_cache(maxsize=4096)
+def _places_meet(na: tuple, sa: tuple, nb: tuple, sb: tuple, delta: int) -> bool:
+    """Whether sum(i * sa) = delta + sum(j * sb) for some i < na, j < nb (strides in the same units).
+    Few of the sums lie near delta where the strides are nested, as they are in views of one
+    tensor; after 4096 of them the answer is yes."""
+    reach: dict[int, list[int]] = {}
+    for n, s in zip(na, sa):
+        if n > 1 and s:
+            reach.setdefault(s, [0, 0])[1] += n - 1
+    for n, s in zip(nb, sb):
+        if n > 1 and s:
+            reach.setdefault(s, [0, 0])[0] -= n - 1
+    dims = sorted(reach.items(), reverse=True)
+    low, high = [0], [0]  # what the strides from there on reach
+    for s, (lo, hi) in reversed(dims):
+        low.append(low[-1] + lo * s)
+        high.append(high[-1] + hi * s)
+    left, todo = 4096, [(0, delta)]
+    while todo:
+        at, d = todo.pop()
+        if at == len(dims):
+            if d == 0:
+                return True
+            continue
+        s, (lo, hi) = dims[at]
+        below = len(dims) - at - 1
+        first, last = max(lo, -((high[below] - d) // s)), min(hi, (d - low[below]) // s)
+        left -= max(0, last - first + 1)
+        if left < 0:
+            return True
+        todo += [(at + 1, d - c * s) for c in range(first, last + 1)]
+    return False
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors have a place in common: exact for views of one tensor (parts of a
+    projection's output lie between one another without one), else at worst yes for no."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    pa, pb, ia, ib = a.data_ptr(), b.data_ptr(), a.element_size(), b.element_size()
+    na, nb, sa, sb = tuple(a.shape), tuple(b.shape), a.stride(), b.stride()
+    if pa + ia * (1 + sum((n - 1) * s for n, s in zip(na, sa))) <= pb or pb + ib * (1 + sum((n - 1) * s for n, s in zip(nb, sb))) <= pa:
+        return False
+    if ia == ib and (pb - pa) % ia == 0:
+        return _places_meet(na, sa, nb, sb, (pb - pa) // ia)
+    return _places_meet(na + (ia,), tuple(s * ia for s in sa) + (1,), nb + (ib,), tuple(s * ib for s in sb) + (1,), pb - pa)
+
+
+def apart(op: str, name: str, out: torch.Tensor, place_of: torch.Tensor | None, **others: torch.Tensor | None) -> None:
+    """Refuse an output that lies in memory which the kernel reads (or writes) for another element.
+    ``place_of``: the input that ``out`` may be, element for element."""
+    if place_of is not None and overlap(out, place_of):
+        if out.data_ptr() != place_of.data_ptr() or any(n > 1 and x != y for n, x, y in zip(out.shape, out.stride(), place_of.stride())):
+            raise ValueError(f"{op}: {name} overlaps its input (it may be the input itself, or other memory)")
+    for other, t in others.items():
+        if t is not None and overlap(out, t):
+            raise ValueError(f"{op}: {name} and {other} overlap in memory")
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

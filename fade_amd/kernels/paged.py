@@ -51,7 +51,8 @@ def paged_append(
     tokens whose slot is -1 (or in page 0, or past the pages) are not written.  With
     ``scheme`` K is rotated at ``positions`` (int [tokens] or [axes, tokens]) as
     ``rope_axes`` does, and so is ``q`` [tokens, Hq, D] where given: its rotation is returned
-    (``q_out``, which may be ``q``, or a new tensor), for every token.
+    (``q_out``, which may be ``q`` or other memory, or a new tensor), for every token.
+    ``k`` and ``v`` may be views of pages, as long as none of their tokens is written.
     """
     op = "paged_append"
     _lib.require_gpu(k, v, k_pages, v_pages, slots, q, positions, q_out, op=op)
@@ -85,15 +86,20 @@ def paged_append(
         a.pos_sa = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
     a.B, a.S, a.D, a.Hkv, a.dtype = 1, T, D, Hkv, dtc
     a.slots, a.n_pages = slots.data_ptr(), n_pages
-    keep = []
+    read = []
 
     def rows(t: Tensor, dst: int, sh: int = 0, ss: int = 0):
         st = t.stride()
         if st[2] != 1 or t.is_neg():
             t = t.resolve_neg().contiguous()
             st = t.stride()
-            keep.append(t)
+        read.append(t)
         return _lib.RopeRows(t.data_ptr(), dst, 0, st[1], st[0], 0, sh, ss)
+
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if abs(kp - vp) < k_pages.nbytes:
+        raise ValueError(f"{op}: k_pages and v_pages overlap in memory")
+    given = q_out is not None
 
     if q is not None:
         if q_out is None:
@@ -101,7 +107,9 @@ def paged_append(
         else:
             _lib.written(op, q_out)
         a.Hq, a.q = q.shape[1], rows(q, q_out.data_ptr(), q_out.stride(1), q_out.stride(0))
-    a.k, a.v = rows(k, k_pages.data_ptr()), rows(v, v_pages.data_ptr())
+    a.k, a.v = rows(k, kp), rows(v, vp)
+    if given:
+        _lib.apart(op, "q_out", q_out, read[0], k=read[1], v=read[2], slots=slots, positions=positions, k_pages=k_pages, v_pages=v_pages)
     _lib.written(op, k_pages, v_pages)
     _lib.launch("fade_paged_append", a, k.device)
     return q_out
@@ -174,6 +182,8 @@ class PagedAttentionPlan:
         if out.shape != q.shape or out.dtype != q.dtype or out.is_neg() or out.stride(2) != 1 or (o_st | o_sh) % 4 \
                 or not _lib.each_once(out) or out.data_ptr() % 8:
             raise ValueError(f"{op}: out must be {q.dtype} {tuple(q.shape)} with a contiguous head_dim axis, 8-byte aligned rows and no row twice")
+        if not self._fresh:
+            _lib.apart(op, "out", out, q, k_pages=k_pages, v_pages=v_pages, table=table, lens=lens, starts=starts)
         a = _lib.PagedAttnArgs()
         a.B, a.T, a.Hq, a.Hkv, a.D, a.n_pages, a.pages_per_row = B, T, Hq, Hkv, D, n_pages, ppr
         a.q, a.q_st, a.q_sh = q.data_ptr(), q_st, q_sh

@@ -474,7 +474,7 @@ def rope_axes(
     and i + rotated / 2; channels past the scheme's rotated ones are copied.
     ``inverse`` turns back.  Angles are reduced exactly whatever the position; products
     in fp32, one rounding to the dtype.  Returns new tensors (contiguous), or ``out``
-    = (q_out, k_out), which may be the inputs themselves.
+    = (q_out, k_out), which may be the inputs themselves (q_out q, k_out k), else other memory.
     """
     op = "rope_axes"
     ref = q if q is not None else k
@@ -504,14 +504,15 @@ def rope_axes(
     a.pos_sb = st[-2] if len(shape) > 1 and shape[-2] > 1 else 0
     a.pos_sa = st[0] if len(shape) == 3 and shape[0] > 1 else 0
     dst = [None, None] if out is None else list(out)
-    res, keep = [], []
+    res, read = [], []
     for name, t, o in (("q", q, dst[0]), ("k", k, dst[1])):
         if t is None:
             res.append(None)
+            read.append(None)
             continue
         if t.is_neg() or t.stride(3) != 1:
             t = t.resolve_neg().contiguous()
-            keep.append(t)
+        read.append(t)
         if o is None:
             o = torch.empty_like(t, memory_format=torch.contiguous_format)  # (half the time of torch.empty)
         else:
@@ -527,6 +528,11 @@ def rope_axes(
         else:
             a.Hkv, a.k = t.shape[1], rows
         res.append(o)
+    if out is not None:
+        if dst[0] is not None and q is not None:
+            _lib.apart(op, "out[0]", dst[0], read[0], k=read[1], positions=positions, **{"out[1]": res[1]})
+        if dst[1] is not None and k is not None:
+            _lib.apart(op, "out[1]", dst[1], read[1], q=read[0], positions=positions)
     _lib.launch("fade_rope_axes", a, ref.device)
     return res[0], res[1]
 

@@ -502,7 +502,7 @@ int fade_page_slots(const fade_page_slots_args* args, void* stream);
 #define FADE_ROPE_MAX_AXES 4
 typedef struct fade_rope_rows { /* [B, heads, S, D], element strides, unit stride along D */
   const void* src;
-  void* dst; /* may be src */
+  void* dst; /* may be src (with its strides), else memory that the call does not read; no element twice */
   int64_t src_sb, src_sh, src_ss;
   int64_t dst_sb, dst_sh, dst_ss;
 } fade_rope_rows;

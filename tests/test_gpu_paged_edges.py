@@ -158,3 +158,40 @@ def test_outputs_of_repeated_rows_are_refused(dev):
     assert rope_axes(q.transpose(0, 1)[None], None, pos, scheme, out=(other.transpose(0, 1)[None], None))[0] is not None
     paged_append(q, q, pages, pages.clone(), pos.int() + PAGE_TOKENS, q=q, positions=pos, scheme=scheme, q_out=other)
     paged_attention(q, pages, pages, _i32([[1]], dev), _i32([T], dev), _i32([0, T], dev), out=other)
+
+
+def test_outputs_over_inputs_are_refused(dev):
+    """An output may be its own input, or lie between the inputs' rows, and nothing else of the call's memory."""
+    D, T, H = 64, 6, 4
+    g = torch.Generator(device=dev).manual_seed(3)
+    qkv = torch.randn(T + 1, 3 * H, D, generator=g, device=dev).half()
+    q, k, v = qkv[:T, :H], qkv[:T, H : 2 * H], qkv[:T, 2 * H :]
+    pages = torch.randn(2, 3, H, PAGE_TOKENS, D, generator=g, device=dev).half()
+    scheme, pos = Vanilla(theta=1e4, head_dim=D), torch.arange(T, device=dev)
+    slots, ints = pos.int() + PAGE_TOKENS, (_i32([[1]], dev), _i32([T], dev), _i32([0, T], dev))
+    four = lambda x: x.transpose(0, 1)[None]  # noqa: E731
+    before, kept = qkv.clone(), pages.clone()
+    for out in (qkv[1:, :H], k, qkv[:T, 1 : H + 1], pages[0, 1].transpose(0, 1)[:T]):
+        if out.data_ptr() != pages[0, 1].data_ptr():
+            with pytest.raises(ValueError, match="overlap"):
+                rope_axes(four(q), four(k), pos, scheme, out=(four(out), None))
+        with pytest.raises(ValueError, match="overlap"):
+            paged_append(k, v, pages[0], pages[1], slots, q=q, positions=pos, scheme=scheme, q_out=out)
+        if out.data_ptr() != k.data_ptr():
+            with pytest.raises(ValueError, match="overlap"):
+                paged_attention(q, pages[0], pages[1], *ints, out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        rope_axes(four(q), four(k), pos, scheme, out=(four(q), four(q)))
+    with pytest.raises(ValueError, match="overlap"):
+        paged_append(k, v, pages[0], pages[0], slots)
+    assert torch.equal(qkv, before) and torch.equal(pages, kept)
+    want = rope_axes(four(q), four(k), pos, scheme)
+    rope_axes(four(q), four(k), pos, scheme, out=(four(q), four(k)))
+    assert torch.equal(four(q), want[0]) and torch.equal(four(k), want[1]) and torch.equal(v, before[:T, 2 * H :])
+    qkv.copy_(before)
+    paged_append(k, v, pages[0], pages[1], slots, q=q, positions=pos, scheme=scheme, q_out=q)
+    assert torch.equal(four(q), want[0]) and torch.equal(pages[0, 1].transpose(0, 1)[:T], want[1][0].transpose(0, 1))
+    # tokens of one page to another
+    paged_append(pages[0, 1].transpose(0, 1), pages[1, 1].transpose(0, 1), pages[0], pages[1], torch.arange(128, 192, device=dev).int())
+    assert torch.equal(pages[:, 2], pages[:, 1])
+    paged_attention(q, pages[0], pages[1], *ints, out=k)

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -29,3 +31,48 @@ def test_places_of_an_output():
         assert _lib.each_once(t), t.stride()
     for t in (x[:1].expand(4, 3, 8), x[:, :1].expand(4, 3, 8), rows.as_strided((3, 3, 8), (4, 12, 1)), rows.as_strided((2, 3, 8), (16, 8, 1))):
         assert not _lib.each_once(t), t.stride()
+
+
+def test_overlap_of_views():
+    """Against the bytes that both tensors hold."""
+    rng, room = random.Random(1), torch.zeros(4000, dtype=torch.int16)
+
+    def view():
+        while True:
+            shape = [rng.choice((1, 2, 3, 5)) for _ in range(rng.randint(1, 4))]
+            if rng.random() < 0.6:  # nested strides, in either order, with gaps
+                stride, reach = [], 1
+                for n in reversed(shape):
+                    stride.insert(0, reach)
+                    reach *= n + rng.choice((0, 0, 1))
+                if rng.random() < 0.5:
+                    stride.reverse()
+            else:
+                stride = [rng.choice((0, 1, 2, 3, 4, 7, 10, 30)) for _ in shape]
+            x = room if rng.random() < 0.8 else room.view(torch.int32)
+            at = rng.randint(0, 60)
+            if at + sum((n - 1) * s for n, s in zip(shape, stride)) < x.numel():
+                return x.as_strided(shape, stride, at)
+
+    def held(x):
+        at = torch.zeros(x.shape, dtype=torch.int64)
+        for d, (n, s) in enumerate(zip(x.shape, x.stride())):
+            at += (torch.arange(n) * s).view([-1 if e == d else 1 for e in range(x.dim())])
+        size = x.element_size()
+        return {(i + x.storage_offset()) * size + e for i in at.flatten().tolist() for e in range(size)}
+
+    seen = set()
+    for _ in range(3000):
+        a, b = view(), view()
+        want = bool(held(a) & held(b))
+        assert _lib.overlap(a, b) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+        seen.add(want)
+    assert len(seen) == 2
+    # parts of a projection's output lie between one another
+    qkv = torch.zeros(500, 48, 64, dtype=torch.float16)
+    q, k = qkv[:, :32], qkv[:, 32:40]
+    assert not _lib.overlap(q, k) and _lib.overlap(q, qkv[:, 31:]) and not _lib.overlap(q[:0], q)
+    _lib.apart("op", "out", q, q, k=k, none=None)
+    for bad, other in ((qkv[:, 1:33], {}), (q.transpose(0, 1)[:, :32].transpose(0, 1), {"k": qkv[:, 31:]})):
+        with pytest.raises(ValueError, match="op: out .*overlap"):
+            _lib.apart("op", "out", bad, q, **other)
