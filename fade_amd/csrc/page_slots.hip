@@ -240,10 +240,27 @@ FADE_API int fade_page_slots(const fade_page_slots_args* a, void* stream) {
   if (!a->lens || !a->new_tokens || !a->table || !a->free_pages || !a->ring || !a->table_out || !a->lens_out || !a->starts ||
       !a->ring_out || !a->status || (a->n_tokens > 0 && (!a->slots || !a->positions)))
     return einval("fade_page_slots: null pointer");
-  if (a->lens_out == a->lens || a->ring_out == a->ring || a->lens_out == a->new_tokens || a->starts == a->lens ||
-      a->starts == a->new_tokens)
-    return einval("fade_page_slots: lens_out, starts and ring_out must be other memory than the counts and the ring "
-                  "(every workgroup reads them)");
+  // what one workgroup writes, others read: every array of the call has memory of its own, but table_out may be table
+  // (a workgroup reads the entries that it writes, and those of a row's pages, which stay as they are)
+  struct Span {
+    const void* at;
+    int64_t bytes;
+    const char* name;
+  };
+  const Span spans[] = {{a->table_out, 4 * a->B * a->pages_per_row, "table_out"}, {a->lens_out, 4 * a->B, "lens_out"},
+                        {a->starts, 4 * a->B + 4, "starts"}, {a->slots, 4 * a->n_tokens, "slots"},
+                        {a->positions, 4 * a->n_tokens, "positions"}, {a->ring_out, 8, "ring_out"}, {a->status, 4, "status"},
+                        {a->free_pages, 4 * a->n_free, "free_pages"},  // (written so far)
+                        {a->lens, 4 * a->B, "lens"}, {a->new_tokens, 4 * a->B, "new_tokens"}, {a->reset, a->reset ? a->B : 0, "reset"},
+                        {a->ring, 8, "ring"}, {a->table, 4 * a->B * a->pages_per_row, "table"}};
+  for (int i = 0; i < 8; ++i)
+    for (int j = i + 1; j < 13; ++j) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(spans[i].at), y = reinterpret_cast<uintptr_t>(spans[j].at);
+      if ((i == 0 && j == 12 && x == y) || spans[i].bytes == 0 || spans[j].bytes == 0) continue;
+      if (x < y + spans[j].bytes && y < x + spans[i].bytes)
+        return einval("fade_page_slots: %s and %s overlap; what is written must be other memory than the rest of the call's (table_out may be table)",
+                      spans[i].name, spans[j].name);
+    }
   SlotParams p;
   p.B = static_cast<int>(a->B);
   p.ppr = static_cast<int>(a->pages_per_row);

@@ -209,7 +209,7 @@ def page_slots(
     int32 [n] the ring of free pages, written where pages are returned (those are handed out
     from the next call on), ``ring`` int32 [2] its first entry and count.  ``n_tokens``
     is the size of the slot map: at least the new tokens.  ``out`` takes the results
-    (its ``table`` may be ``table`` itself, its other tensors not the inputs).
+    (its ``table`` may be ``table`` itself; else memory of their own, which is checked).
 
     All or nothing: where pages run out, a row's table is too short, ``n_tokens`` is too
     small or a count is impossible, ``status`` says so, the table, the lengths and the

@@ -474,8 +474,9 @@ int fade_tiered_prefill_attn_ws(const fade_prefill_args* args, void* workspace, 
  * page returned by a call is handed out from the next one on).  Writes the
  * block table (table_out may be table), lens_out, starts [B + 1] (first new token
  * of each row), slots and positions of the new tokens [n_tokens] (-1 and 0 past
- * the last one), ring_out and status [1].  lens_out, starts and ring_out must be
- * other memory than the inputs.  The same inputs give the same outputs again. */
+ * the last one), ring_out and status [1].  What is written (free_pages too) must be
+ * other memory than the rest of the call's; overlaps are refused.  The same inputs
+ * give the same outputs again. */
 typedef struct fade_page_slots_args {
   int64_t B, pages_per_row, n_tokens, n_free;
   const int32_t* lens;

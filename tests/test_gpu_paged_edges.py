@@ -10,7 +10,7 @@ import torch
 from torch.autograd import forward_ad
 
 from fade_amd.kernels import paged_append, paged_attention
-from fade_amd.pages import PAGE_TOKENS, TokenPagePool
+from fade_amd.pages import PAGE_TOKENS, PageSlots, TokenPagePool, page_slots
 from fade_amd.rope import MRope, Vanilla, rope_axes
 from test_gpu_paged import BF16, F16, F32, _check, _i32, _pages, _reference, _starts
 
@@ -195,3 +195,20 @@ def test_outputs_over_inputs_are_refused(dev):
     paged_append(pages[0, 1].transpose(0, 1), pages[1, 1].transpose(0, 1), pages[0], pages[1], torch.arange(128, 192, device=dev).int())
     assert torch.equal(pages[:, 2], pages[:, 1])
     paged_attention(q, pages[0], pages[1], *ints, out=k)
+
+
+def test_slots_outputs_over_other_memory_are_refused(dev):
+    m = torch.zeros(64, dtype=torch.int32, device=dev)
+    lens, new, table, free, ring = m[:2], m[2:4], m[4:10].view(2, 3), m[10:14], m[14:16]
+    free.copy_(_i32([1, 2, 3, 4], dev))
+    ring[1], new[0] = 4, 3
+    fresh = m[20:]
+    names = ("table", "lens", "starts", "slots", "positions", "ring", "status")
+    for name, over in (("slots", lens), ("positions", new), ("status", ring[:1]), ("lens", free[:2]), ("starts", fresh[7:10]), ("table", m[5:11])):
+        parts = dict(zip(names, fresh.split([6, 2, 3, 2, 2, 2, 1, 26])))
+        parts[name] = over.view(2, 3) if name == "table" else over
+        with pytest.raises(ValueError, match="overlap"):
+            page_slots(lens, new, table, free, ring, 2, out=PageSlots(**parts))
+    parts = dict(zip(names, fresh.split([6, 2, 3, 4, 4, 2, 1, 22])), table=table)
+    got = page_slots(lens, new, table, free, ring, 4, out=PageSlots(**parts)).check()
+    assert got.slots.tolist() == [64, 65, 66, -1] and table.tolist() == [[1, 0, 0], [0, 0, 0]] and got.ring.tolist() == [1, 3]

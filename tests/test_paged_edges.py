@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import ctypes
 import random
 
 import pytest
@@ -76,3 +77,30 @@ def test_overlap_of_views():
     for bad, other in ((qkv[:, 1:33], {}), (q.transpose(0, 1)[:, :32].transpose(0, 1), {"k": qkv[:, 31:]})):
         with pytest.raises(ValueError, match="op: out .*overlap"):
             _lib.apart("op", "out", bad, q, **other)
+
+
+def test_slots_outputs_over_other_memory_are_refused():
+    """Every overlap of what is written with anything else of the call, by one byte at least; the entry
+    refuses before it launches anything."""
+    B, ppr, n, cap = 5, 3, 7, 11
+    sizes = dict(lens=4 * B, new_tokens=4 * B, reset=B, table=4 * B * ppr, free_pages=4 * cap, ring=8, table_out=4 * B * ppr, lens_out=4 * B,
+                 starts=4 * B + 4, slots=4 * n, positions=4 * n, ring_out=8, status=4)
+    written = ("free_pages", "table_out", "lens_out", "starts", "slots", "positions", "ring_out", "status")
+    place = {name: (1 << 20) + 4096 * i for i, name in enumerate(sizes)}
+
+    def refused(**at):
+        a = _lib.PageSlotsArgs(B, ppr, n, cap)
+        for name, x in {**place, **at}.items():
+            setattr(a, name, x)
+        lib = _lib.load()
+        return lib.fade_page_slots(ctypes.byref(a), None) == _lib.FADE_EINVAL and b"overlap" in lib.fade_hip_last_error()
+
+    for name in written:
+        for other in sizes:
+            if other == name:
+                continue
+            for at in (place[other], place[other] + sizes[other] - 1 & ~3, place[other] - sizes[name] + 4):
+                if (name, other, at) == ("table_out", "table", place["table"]):
+                    continue
+                assert refused(**{name: at}), (name, other, at - place[other])
+    assert refused(table_out=place["table"] + 4)
