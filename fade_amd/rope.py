@@ -100,19 +100,24 @@ class RopeScheme:
     def _position_divisor(self) -> float:
         return 1.0
 
+    def _turn_key(self) -> tuple:
+        """What the turns follow beside the inverse frequencies, which stay as first computed."""
+        return ()
+
     def turns(self) -> tuple[bytes, bytes]:
         """``fade_rope_args``' frequencies: each one's turns per position as a 64-bit fraction
         (so that position * fraction modulo 2^64 is the angle, exactly reduced) in 8 bytes, and
         its axis in one."""
-        if self._turn_cache is None:
+        key = self._turn_key()
+        if self._turn_cache is None or self._turn_cache[0] != key:
             da, db = float(self._position_divisor()).as_integer_ratio()
             frac = []
             for f in self.inv_freq().tolist():  # the fp32 inverse frequency / (2 pi), exactly, to the nearest 2^-64
                 num, den = f.as_integer_ratio()
                 num, den = num * db * _TURNS_192, den * da << 128
                 frac.append((2 * num + den) // (2 * den) % 2**64)
-            self._turn_cache = (struct.pack(f"={len(frac)}Q", *frac), bytes(self.freq_axes()))
-        return self._turn_cache
+            self._turn_cache = (key, (struct.pack(f"={len(frac)}Q", *frac), bytes(self.freq_axes())))
+        return self._turn_cache[1]
 
 
 @dataclass
@@ -131,6 +136,9 @@ class LinearScaled(RopeScheme):
 
     def _position_divisor(self) -> float:
         return self.factor
+
+    def _turn_key(self) -> tuple:
+        return (self.factor,)
 
     def host_cos_sin(self, positions, model_dtype=torch.float16):
         # The reference always rounds through model_dtype for this scheme.
@@ -230,6 +238,9 @@ class MRope(RopeScheme):
     @property
     def n_axes(self) -> int:
         return len(self.mrope_section) if self.mrope_section else 1
+
+    def _turn_key(self) -> tuple:
+        return (tuple(self.mrope_section or ()), self.interleaved)
 
     def freq_axes(self) -> list[int]:
         n, sec = int(self.inv_freq().shape[0]), self.mrope_section

@@ -10,6 +10,7 @@ import torch
 from torch.autograd import forward_ad
 
 from fade_amd import _lib
+from fade_amd.rope import LinearScaled, MRope
 
 
 def test_forward_mode_is_refused():
@@ -104,3 +105,23 @@ def test_slots_outputs_over_other_memory_are_refused():
                     continue
                 assert refused(**{name: at}), (name, other, at - place[other])
     assert refused(table_out=place["table"] + 4)
+
+
+def test_turns_follow_the_scheme():
+    """A scheme whose factor, sections or order are changed turns as a new one does (its tables did already)."""
+    s = LinearScaled(theta=1e4, head_dim=64, factor=2.0)
+    first = s.turns()
+    assert s.turns() is first
+    s.factor = 4.0
+    assert s.turns() == LinearScaled(theta=1e4, head_dim=64, factor=4.0).turns() != first
+    m = MRope(theta=1e6, head_dim=128, mrope_section=[24, 20, 20])
+    first = m.turns()
+    m.interleaved = True
+    assert m.turns() == MRope(theta=1e6, head_dim=128, mrope_section=[24, 20, 20], interleaved=True).turns() != first
+    m.mrope_section[:] = [22, 21, 21]
+    assert m.turns() == MRope(theta=1e6, head_dim=128, mrope_section=[22, 21, 21], interleaved=True).turns()
+    m.mrope_section = [1, 2, 3]
+    with pytest.raises(ValueError, match="share out"):
+        m.turns()
+    m.mrope_section = None
+    assert set(m.turns()[1]) == {0} and m.n_axes == 1
