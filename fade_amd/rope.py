@@ -459,7 +459,8 @@ def rope_args(scheme: RopeScheme, head_dim: int, device: torch.device, op: str):
             raise RuntimeError(f"{op}: the scheme's frequencies would be uploaded during HIP-graph capture; run the same call "
                                "once before capturing")
         t = torch.frombuffer(bytearray(turn + axis or b"\0"), dtype=torch.uint8).to(device)  # (waits: any stream may read it)
-        tab = _TURN_TABLES[(turn, axis, device)] = (t, t.data_ptr(), t.data_ptr() + len(turn))
+        # (two threads' first calls: both take the one that stays, the other is freed)
+        tab = _TURN_TABLES.setdefault((turn, axis, device), (t, t.data_ptr(), t.data_ptr() + len(turn)))
     if 2 * len(axis) > head_dim:
         raise ValueError(f"{op}: the scheme rotates {2 * len(axis)} channels, the rows have {head_dim}")
     a = _lib.RopeArgs()

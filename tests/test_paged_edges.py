@@ -9,8 +9,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from fade_amd import _lib
-from fade_amd.rope import LinearScaled, MRope
+from fade_amd import _lib, rope
+from fade_amd.rope import LinearScaled, MRope, Vanilla
 
 
 def test_forward_mode_is_refused():
@@ -125,3 +125,18 @@ def test_turns_follow_the_scheme():
         m.turns()
     m.mrope_section = None
     assert set(m.turns()[1]) == {0} and m.n_axes == 1
+
+
+def test_first_calls_of_two_threads_share_a_table(monkeypatch):
+    """Both launches read the frequencies that stay in memory, where both threads have found none and made some."""
+
+    class Tables(dict):
+        def get(self, key):
+            return None  # as for a thread that looked before the other stored its own
+
+    monkeypatch.setattr(rope, "_TURN_TABLES", Tables())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    scheme = Vanilla(theta=4321.0, head_dim=32)
+    a, b = (rope.rope_args(scheme, 32, torch.device("cpu"), "op") for _ in range(2))
+    (kept, turn, axis), = rope._TURN_TABLES.values()
+    assert a.turn == b.turn == turn == kept.data_ptr() and a.axis == b.axis == axis == turn + 8 * 16
