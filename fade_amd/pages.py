@@ -296,10 +296,13 @@ class TokenPagePool:
         B, ppr = (int(d) for d in table.shape)
         if length > ppr * PAGE_TOKENS:
             raise ValueError(f"length {length} exceeds the table's {ppr} pages per row")
-        pages = table[:, : -(-length // PAGE_TOKENS)].long()
+        if length < 0:
+            raise ValueError(f"length must be >= 0, got {length}")
+        n = -(-length // PAGE_TOKENS)
+        pages = table[:, :n].long()
 
         def one(x: Tensor) -> Tensor:
-            return x[pages].permute(0, 2, 1, 3, 4).reshape(B, self.n_kv_heads, -1, self.head_dim)[:, :, :length].contiguous()
+            return x[pages].permute(0, 2, 1, 3, 4).reshape(B, self.n_kv_heads, n * PAGE_TOKENS, self.head_dim)[:, :, :length].contiguous()
 
         return one(self.k), one(self.v)
 

@@ -10,6 +10,7 @@ import torch
 from torch.autograd import forward_ad
 
 from fade_amd import _lib, rope
+from fade_amd.pages import TokenPagePool
 from fade_amd.rope import LinearScaled, MRope, Vanilla
 
 
@@ -140,3 +141,13 @@ def test_first_calls_of_two_threads_share_a_table(monkeypatch):
     a, b = (rope.rope_args(scheme, 32, torch.device("cpu"), "op") for _ in range(2))
     (kept, turn, axis), = rope._TURN_TABLES.values()
     assert a.turn == b.turn == turn == kept.data_ptr() and a.axis == b.axis == axis == turn + 8 * 16
+
+
+def test_gather_of_no_tokens():
+    pool = TokenPagePool(5, 2, 16, torch.bfloat16, "cpu")
+    for B in (0, 2):
+        k, v = pool.gather(torch.zeros(B, 3, dtype=torch.int32), 0)  # rows that hold nothing yet
+        assert k.shape == v.shape == (B, 2, 0, 16)
+        assert pool.gather(torch.zeros(B, 3, dtype=torch.int32), 70)[0].shape == (B, 2, 70, 16)
+    with pytest.raises(ValueError, match=">= 0"):
+        pool.gather(torch.zeros(2, 3, dtype=torch.int32), -1)
