@@ -41,6 +41,7 @@ struct Rows {
 
 struct RopeParams {
   int64_t tokens, S;  // B * S of them
+  uint32_t first;     // this launch's first
   int D, half;        // channels of a row, rotated pairs
   int heads[3];       // of q, k, v (v only in an append)
   int first_group[3]; // of each tensor's heads in the grid's second dimension
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
   const unsigned units = static_cast<unsigned>(p.D) / (2 * V);
   const unsigned per_block = kThreads / units, lrow = threadIdx.x / units;
   const int u = static_cast<int>(threadIdx.x - lrow * units);
-  const uint32_t t = blockIdx.x * per_block + lrow;  // (tokens < 2^31)
+  const uint32_t t = p.first + blockIdx.x * per_block + lrow;  // (tokens < 2^31)
   if (lrow >= per_block || t >= static_cast<uint32_t>(p.tokens)) return;
   const uint32_t b = t / static_cast<uint32_t>(p.S), s = t - b * static_cast<uint32_t>(p.S);
   const int rot_units = p.half / V;
@@ -185,10 +186,17 @@ int rope_launch(RopeParams& p, bool wide, void* stream) {
     p.first_group[i] = groups;
     groups += static_cast<int>(cdiv(p.heads[i], p.heads_per_block));
   }
-  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(groups));
-  if (wide) hipLaunchKernelGGL((rope_kernel<T, V>), grid, dim3(kThreads), 0, as_stream(stream), p);
-  else hipLaunchKernelGGL((rope_kernel<T, 1>), grid, dim3(kThreads), 0, as_stream(stream), p);
-  return check_launch("fade_rope_axes");
+  // (a launch has fewer than 2^32 threads along x)
+  const int64_t most = ((1ll << 32) / kThreads) - 1;
+  for (int64_t b0 = 0; b0 < bx; b0 += most) {
+    p.first = static_cast<uint32_t>(b0 * (kThreads / units));
+    const dim3 grid(static_cast<unsigned>(bx - b0 < most ? bx - b0 : most), static_cast<unsigned>(groups));
+    if (wide) hipLaunchKernelGGL((rope_kernel<T, V>), grid, dim3(kThreads), 0, as_stream(stream), p);
+    else hipLaunchKernelGGL((rope_kernel<T, 1>), grid, dim3(kThreads), 0, as_stream(stream), p);
+    const int rc = check_launch("fade_rope_axes");
+    if (rc) return rc;
+  }
+  return FADE_OK;
 }
 
 int rope_any(const fade_rope_args* a, bool append, const char* what, void* stream) {

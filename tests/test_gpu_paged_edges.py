@@ -212,3 +212,17 @@ def test_slots_outputs_over_other_memory_are_refused(dev):
     parts = dict(zip(names, fresh.split([6, 2, 3, 4, 4, 2, 1, 22])), table=table)
     got = page_slots(lens, new, table, free, ring, 4, out=PageSlots(**parts)).check()
     assert got.slots.tolist() == [64, 65, 66, -1] and table.tolist() == [[1, 0, 0], [0, 0, 0]] and got.ring.tolist() == [1, 3]
+
+
+def test_rotation_of_more_workgroups_than_a_launch_has(dev):
+    """Rows that are not 16-byte aligned, four to a workgroup, past 2^32 threads: every row is turned, once."""
+    D, S = 128, 2**26 + 9
+    scheme = Vanilla(theta=1e4, head_dim=D)
+    buf = torch.ones(S * D + 1, dtype=BF16, device=dev)
+    x = buf[1:].view(1, 1, S, D)
+    pos = torch.full((1,), 3, device=dev).expand(S)
+    one = rope_axes(torch.ones(1, 1, 1, D, dtype=BF16, device=dev), None, pos[:1], scheme)[0]
+    rope_axes(x, None, pos, scheme, out=(x, None))
+    for at in range(0, S, 2**22):
+        assert bool((x[:, :, at : at + 2**22] == one).all()), at
+    assert buf[0] == 1
