@@ -1169,10 +1169,15 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   p.zero_tail = a->zero_tail;
   // Rows whose matrix rows fit one tile of 16 go to the few-row kernel, the others
   // to the wide one (16 rows over 8192 keys each, 32 matrix rows a row: 113 us, by the
-  // few-row kernel 124; 64: 114 and 204; 128: 131 and 389); a call of at most 16 matrix
-  // rows per row on average is taken to be a decoding step, all of it the few-row
-  // kernel's (the wide kernel's launch, empty, costs such a step 2.5 us).
-  const bool step = p.T * p.G <= kRows * p.B;
+  // few-row kernel 124; 64: 114 and 204; 128: 131 and 389).  The host does not know the
+  // rows, and the wide kernel's launch, empty, costs a decoding step 2 to 5 us (64 rows of
+  // 1000 keys 54 us, with it 59; one row of 1000 keys 10.9 and 13.0), so a step goes to the
+  // few-row kernel as a whole where no row of it can be longer while the others have a
+  // token each.  A chunk taken for a part of such a step costs far more: 63 rows of 1000
+  // keys beside 193 tokens over 8192 keys 201 us, 117 by both kernels; 900 tokens at 32 kv
+  // heads 895 and 352.  Rows without tokens can still hide one (64 of them, 64 tokens over
+  // 8192 keys 67 us and 45, over 1000 keys 27 and 36), so it is bound to four wide tiles.
+  const bool step = (p.T - p.B + 1) * p.G <= kRows && p.T * p.G <= 1024;
   pl.both = !step;
   // The few-row kernel has as many workgroups as find a place at once (16 rows over
   // 8192 keys: 4 per CU 104.5 us, 8 110.6, 16 120), of 64 keys or more each (a row of

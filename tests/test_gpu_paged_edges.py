@@ -226,3 +226,20 @@ def test_rotation_of_more_workgroups_than_a_launch_has(dev):
     for at in range(0, S, 2**22):
         assert bool((x[:, :, at : at + 2**22] == one).all()), at
     assert buf[0] == 1
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,Hq,Hkv,n,L,others", [(70, 8, 2, 200, 3000, 1), (64, 2, 2, 900, 2000, 1), (64, 8, 2, 193, 193, 1), (70, 8, 2, 70, 3000, 0), (300, 4, 1, 300, 1500, 0), (257, 2, 2, 257, 2000, 0)])
+def test_attention_of_a_chunk_among_decoding_rows(dev, B, Hq, Hkv, n, L, others, dtype):
+    """Many rows of one token, or of none, and one of many: few matrix rows a row on average."""
+    D = 64
+    g = torch.Generator(device=dev).manual_seed(B)
+    lens, new = [(53 * i) % 200 + 1 for i in range(B)], [others] * B
+    lens[B // 2], new[B // 2] = L, n
+    k, v, table = _pages(g, dev, lens, Hkv, D, dtype, junk=math.nan)
+    starts = _starts(new)
+    q = torch.randn(starts[-1], Hq, D, generator=g, device=dev).to(dtype)
+    for mask in ("bottom_right", "none"):
+        want, tol = _reference(q, k, v, table, lens, starts, 1 / math.sqrt(D), mask)
+        got = paged_attention(q, k, v, table, _i32(lens, dev), _i32(starts, dev), mask=mask)
+        _check(got, want, tol, mask)

@@ -151,3 +151,26 @@ def test_gather_of_no_tokens():
         assert pool.gather(torch.zeros(B, 3, dtype=torch.int32), 70)[0].shape == (B, 2, 70, 16)
     with pytest.raises(ValueError, match=">= 0"):
         pool.gather(torch.zeros(2, 3, dtype=torch.int32), -1)
+
+
+def _workspace(**kw):
+    a, nb = _lib.PagedAttnArgs(), ctypes.c_int64(0)
+    at = 1 << 20
+    base = dict(Hq=32, Hkv=8, D=128, n_pages=9000, pages_per_row=128, q=at, q_st=4096, q_sh=128, out=at, o_st=4096, o_sh=128, k_pages=at,
+                v_pages=at, table=at, lens=at, starts=at, sm_scale=0.1)
+    for name, x in {**base, **kw}.items():
+        setattr(a, name, x)
+    assert _lib.load().fade_paged_attn_workspace_bytes(ctypes.byref(a), nb) == 0
+    return nb.value
+
+
+def test_a_chunk_among_decoding_rows_goes_to_the_wide_kernel():
+    """The workspace has the wide kernel's sums wherever a row may be longer than a tile of the few-row kernel
+    while the others have a token each, whatever the rows' average."""
+    for B, Hq in ((2, 32), (16, 32), (64, 32), (64, 8), (200, 32)):
+        G = Hq // 8
+        step = _workspace(B=B, T=B, Hq=Hq)
+        assert _workspace(B=B, T=B - 1 + 16 // G, Hq=Hq) == step or B * G + 16 > 1024
+        for T in (B + 16 // G, B - 1 + 193, 16 // G * B, 16 // G * B + 1):
+            assert _workspace(B=B, T=T, Hq=Hq) > 2 * step, (B, T, Hq)
+    assert _workspace(B=2000, T=2000) > 2 * _workspace(B=2000, T=256)  # rows without tokens: a chunk of 1024 matrix rows at most
