@@ -83,12 +83,12 @@ struct Params {
   int least;       // fewest keys of a piece
   int snap;        // a border this near to a tile's is moved there
   float* part_o;   // [workgroup][2][M][D]: a tile's end (0), a tile's beginning (1)
-  float2* part_ml; // [workgroup][2][M]: maximum (log2 units), sum
+  float2* part_ml; // [workgroup][2][M]: maximum (log2 units, less what its kernel holds probabilities larger by), sum
   int4* cuts;      // [workgroup]: the tile that begins in its piece and ends in another: first new token, its
                    // first matrix row, matrix rows of the row, parts (0: none)
 };
 
-// A piece of a tile (wave-uniform): keys' pages or 32-key steps from `from` on, in keys.
+// A tile (wave-uniform).
 struct Tile {
   int b, q0, n, len;   // row, its first new token, new tokens, tokens
   int tile;            // of the row's tiles
@@ -378,7 +378,8 @@ struct Few {
   static constexpr int kTensor = kKeys * DP * 2;   // bytes of a step's K or V
   static constexpr int kStage = 2 * kTensor;
   static constexpr int kLoads = kStage / 1024;     // direct loads per step
-  static constexpr int kStages = 2;
+  static constexpr int kStages = 2;                // (the waits below count one step ahead)
+  static_assert(kLoads < 64, "vmcnt counts to 63");
   static constexpr int kQBytes = kRows * DP * 2;
   static constexpr int kLds = kStages * kStage + kQBytes;
   static constexpr int kSwizzle = kUnits - 1;
@@ -460,9 +461,7 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
       u32x4 qf[NKS];
       {
         // the query's loads are done when no more than the steps' are in flight
-        const int steps = (ahead - key + F::kKeys - 1) / F::kKeys;
-        if (steps >= 2 && F::kStages > 2) __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * F::kLoads));
-        else if (steps >= 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
+        if (ahead > key) __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
         else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
         asm volatile("" ::: "memory");
 #pragma unroll
@@ -481,8 +480,6 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
           issue(ahead, __builtin_amdgcn_readfirstlane(next), t == 0 ? F::kStages - 1 : t - 1);
           ahead += F::kKeys;
           if (ahead < k.hi) next = trow[ahead / kPage];
-          __builtin_amdgcn_s_waitcnt(vmcnt_imm((F::kStages - 1) * F::kLoads));
-        } else if (F::kStages > 2 && key + F::kKeys < k.hi) {
           __builtin_amdgcn_s_waitcnt(vmcnt_imm(F::kLoads));
         } else {
           __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
@@ -1096,7 +1093,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(Params wide, Para
 bool aligned16(const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
 
 template <int DP>
-struct Wide {  // waves, blocks of 32 rows per wave, keys per step
+struct Wide {  // waves, matrix rows, keys per step, steps' buffers
   static constexpr int NW = 8, M = 32 * NW, KT = DP > 128 ? 32 : 64, NST = DP > 128 ? 4 : 3;
 };
 constexpr int kWideLog = 8;
