@@ -122,7 +122,10 @@ class PagedAttentionPlan:
     """Validated launch of the paged attention for fixed tensors, whose contents (the
     queries, the pages, the block table, lengths and starts) may change from run to run.
     The plan keeps the workspace of the key splits' sums for runs on the stream that it
-    was made on; a run on another stream takes one of its own.
+    was made on; a run on another stream takes one of its own.  On 256 CUs it has up to
+    16 MiB for a decoding step (whose rows all fit 16 matrix rows), with chunks 81 MiB at
+    head_dim 128 and 145 MiB at 256, in each plan; ``paged_attention`` takes and returns
+    it at every call.
 
     Args:
         q: [tokens, Hq, D] fp16 or bf16, every row's new tokens one row after the other;

@@ -222,7 +222,13 @@ class MRope(RopeScheme):
 
     ``mrope_section`` gives each axis its number of frequencies: the first section
     to axis 0, the next to axis 1, ...; ``interleaved``: frequency i belongs to axis
-    i modulo the axes while that axis has frequencies left, the rest to axis 0."""
+    i modulo the axes while that axis has frequencies left, the rest to axis 0.
+
+    ``rope_axes`` pairs channels i and i + rotary_dim / 2, as the models do; the tables
+    (the cache's eviction turns keys with them, and knows one position per token) pair
+    i and i + head_dim / 2, as the reference does.  They agree on one axis with
+    ``partial_rotary_factor`` 1; keys of other rotations belong into a cache that does
+    not evict."""
 
     partial_rotary_factor: float = 1.0
     mrope_section: list[int] | None = None
@@ -484,7 +490,8 @@ def rope_axes(
     frequency by its own axis's position (time, height, width), and takes positions
     without an axis dimension as the same on every axis.  Frequency i mixes channels i
     and i + rotated / 2; channels past the scheme's rotated ones are copied.
-    ``inverse`` turns back.  Angles are reduced exactly whatever the position; products
+    ``inverse`` turns back.  (The cache's eviction cannot turn keys rotated on several axes
+    or by a partial ``MRope``: see there.)  Angles are reduced exactly whatever the position; products
     in fp32, one rounding to the dtype.  Returns new tensors (contiguous), or ``out``
     = (q_out, k_out), which may be the inputs themselves (q_out q, k_out k), else other memory.
     """

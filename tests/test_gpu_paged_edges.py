@@ -11,7 +11,7 @@ from torch.autograd import forward_ad
 
 from fade_amd.kernels import paged_append, paged_attention
 from fade_amd.pages import PAGE_TOKENS, PageSlots, TokenPagePool, page_slots
-from fade_amd.rope import MRope, Vanilla, rope_axes
+from fade_amd.rope import Llama3, MRope, Proportional, Vanilla, rerope_gather, rope_axes
 from test_gpu_paged import BF16, F16, F32, _check, _i32, _pages, _reference, _starts
 
 pytestmark = pytest.mark.gpu
@@ -243,3 +243,21 @@ def test_attention_of_a_chunk_among_decoding_rows(dev, B, Hq, Hkv, n, L, others,
         want, tol = _reference(q, k, v, table, lens, starts, 1 / math.sqrt(D), mask)
         got = paged_attention(q, k, v, table, _i32(lens, dev), _i32(starts, dev), mask=mask)
         _check(got, want, tol, mask)
+
+
+@pytest.mark.parametrize("scheme", [Vanilla(theta=1e6, head_dim=128), Llama3(theta=5e5, head_dim=128, factor=8.0),
+                                    Proportional(theta=1e6, head_dim=128, partial_rotary_factor=0.25), MRope(theta=1e6, head_dim=128)])
+def test_eviction_turns_keys_that_rope_axes_rotated(dev, scheme):
+    """One axis, all channels paired i and i + D / 2: the cache's tables turn such keys to their new positions."""
+    H, S, D = 2, 300, 128
+    g = torch.Generator(device=dev).manual_seed(6)
+    k = torch.randn(1, H, S, D, generator=g, device=dev)
+    old = torch.arange(S, device=dev)
+    keep = torch.randperm(S, generator=g, device=dev)[:100].sort().values
+    rotated = rope_axes(None, k, old, scheme)[1]
+    tables = [*scheme.host_cos_sin(old.cpu(), F32), *scheme.host_cos_sin(torch.arange(100), F32)]
+    got, _ = rerope_gather(rotated, None, keep, *tables)
+    want = rope_axes(None, k[:, :, keep].contiguous(), torch.arange(100, device=dev), scheme)[1]
+    # the tables' angles are fp32 products of at most 300 (2^-24 of it each, the inverse frequency's as well: 2^-15 over three
+    # rotations), turning a pair by as much of its length, at most 12 of N(0, 1)'s pairs here
+    assert float((got - want).abs().max()) <= 2.0**-15 * 12
