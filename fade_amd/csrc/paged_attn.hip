@@ -624,7 +624,8 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
 // 525 (they pass their bound, and are rescaled, more often).
 //
 // Eight chunks of 128 to 2048 tokens over up to 11K keys (32 heads, 8 kv heads of
-// 128): 560 to 580 us, 1040 TFLOP/s of visible keys.  What bounds it is the power
+// 128): 500 to 670 us by the drawn lengths and the card's state, 1040 TFLOP/s of
+// visible keys at 565.  What bounds it is the power
 // that the card has: its matrix instructions alone reach 1370 TFLOP/s on random
 // numbers (2200 on constant ones), with this kernel's LDS reads and exponentials
 // beside them 1296, with its loads and barriers 1090.  Measured without gain: scores

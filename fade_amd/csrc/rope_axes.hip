@@ -19,10 +19,11 @@
 // walks the heads of its workgroup's tensor with them, so the trigonometry is paid
 // once per workgroup's heads and a wave's access covers whole 128-byte runs of the
 // rows: 16384 tokens of 40 heads (128 channels of 16 bits, 64 rotated on three
-// axes) 71.5 us, 4.7 TB/s, where a large copy has 5.2; 7900 tokens appended to their
-// pages 37 us, 5.2 TB/s.  Calls of few tokens are bound by latency: no load waits
-// for another one but for its address in the arguments (1187 tokens of 32 heads 7.5
-// us, 32 tokens appended 3.7).
+// axes) 72 to 76 us, 4.4 to 4.7 TB/s, where a large copy has 5.2; in fp32 126 us,
+// 5.3 TB/s; 7900 tokens appended to their pages 44 us on new inputs, 32 on the same
+// ones again (194 MB, partly in the last-level cache).  Calls of few tokens are bound
+// by latency: no load waits for another one but for its address in the arguments (1187
+// tokens of 32 heads 7.2 us, 32 tokens appended 4.1).
 #include "fade_common.h"
 
 namespace fade {

@@ -139,8 +139,10 @@ class PagedAttentionPlan:
         out: like q, contiguous along D, q itself or other memory; rows at and past ``starts[B]``
             are left as they are.  Default: a new tensor, zeros there.
 
-    A query that sees no key gets zeros; a NaN or an infinity in a value reaches the
-    queries that see its key and no others.  Lengths, starts and pages are read on the
+    A query that sees no key, or none with a score over -inf, gets zeros; a NaN or an infinity
+    in a value reaches the queries that see its key and no others.  Probabilities times
+    values are added up in fp32 before the division, so bf16 values must stay under
+    2^120 / tokens.  Lengths, starts and pages are read on the
     GPU and kept inside the tensors there: tokens past a row's table do not count, and
     a page id outside the pool reads page 0."""
 
