@@ -261,3 +261,20 @@ def test_eviction_turns_keys_that_rope_axes_rotated(dev, scheme):
     # the tables' angles are fp32 products of at most 300 (2^-24 of it each, the inverse frequency's as well: 2^-15 over three
     # rotations), turning a pair by as much of its length, at most 12 of N(0, 1)'s pairs here
     assert float((got - want).abs().max()) <= 2.0**-15 * 12
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens,new", [([70, 200], [1, 1]), ([400, 130], [100, 90]), ([3000], [300])])
+def test_queries_whose_scores_are_all_minus_infinity(dev, lens, new, dtype):
+    """They get zeros, as those that see no key, and a row beside them what it gets alone."""
+    H, D = 2, 128
+    g = torch.Generator(device=dev).manual_seed(8)
+    k, v, table = _pages(g, dev, lens, H, D, dtype)
+    starts = _starts(new)
+    q = torch.randn(starts[-1], H, D, generator=g, device=dev).to(dtype)
+    q[..., 5] = 1.0
+    k[:, 0, :, 5] = 0.0
+    want = paged_attention(q, k, v, table, _i32(lens, dev), _i32(starts, dev))
+    k[:, 1, :, 5] = -math.inf
+    got = paged_attention(q, k, v, table, _i32(lens, dev), _i32(starts, dev))
+    assert not got[:, 1].any() and torch.equal(got[:, 0], want[:, 0])
