@@ -337,7 +337,12 @@ def _fork_inputs(case: dict, seed: int) -> dict:
 
 def prepare(case: dict, seed: int) -> dict:
     make = dict(tree=_tree_inputs, attend=_attend_inputs, verify=_verify_inputs, accept=_accept_inputs, fork=_fork_inputs)[case["kind"]]
-    return dict(make(case, seed), kind=case["kind"])
+    s = dict(make(case, seed), kind=case["kind"])
+    if own and "pages" in s:
+        from fade_amd.pages import PageLayers
+
+        s["layers"] = PageLayers(s["pages"])  # a program makes it with its pages
+    return s
 
 
 # ------------------------------------------------------------- the plain forms
@@ -518,7 +523,7 @@ def run(s: dict):
         from fade_amd.kernels.paged import paged_compact
         from fade_amd.pages import page_fork
 
-        kept = paged_compact(s["path"], s["counts"], s["table"], s["lens"], s["starts"], s["pages"])
+        kept = paged_compact(s["path"], s["counts"], s["table"], s["lens"], s["starts"], s["layers"])
         r = page_fork(s["lens"], s["table"], s["free"], s["ring"], keep=kept)
     else:
         if not own:
@@ -529,7 +534,7 @@ def run(s: dict):
         from fade_amd.pages import page_fork
 
         r = page_fork(s["lens"], s["table"], s["free"], s["ring"], source=s["source"], keep=s["keep"])
-        paged_copy(r.copies, s["pages"])
+        paged_copy(r.copies, s["layers"])
     return dict(table=r.table, lens=r.lens, copies=r.copies, ring=r.ring, free=s["free"], pages=s["pages"])
 
 
