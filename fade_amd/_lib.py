@@ -36,6 +36,7 @@ MID_ASYM = 4
 MASK_BOTTOM_RIGHT = 0
 MASK_TOP_LEFT = 1
 MASK_NONE = 2
+MASK_TREE = 3
 
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -199,6 +200,50 @@ class PagedAttnArgs(ctypes.Structure):
         ("q", _p), ("q_st", _i64), ("q_sh", _i64), ("out", _p), ("o_st", _i64), ("o_sh", _i64),
         ("k_pages", _p), ("v_pages", _p), ("table", _p), ("lens", _p), ("starts", _p),
         ("sm_scale", ctypes.c_float), ("mask_mode", _i32), ("dtype", _i32), ("zero_tail", _i32),
+        ("tree", _p), ("tree_words", _i64),
+    ]
+
+
+DRAFT_MAX_NODES = 1024
+DRAFT_STATUS = {1: "more drafted tokens than the masks have bits", 2: "a parent that is no earlier token of the row"}
+FORK_STATUS = {1: "more copies needed than pages are free", 8: "an impossible source, count, page or ring"}
+
+
+class DraftTreeArgs(ctypes.Structure):
+    """``fade_draft_tree_args`` of include/fade_hip.h."""
+
+    _fields_ = [("B", _i64), ("T", _i64), ("words", _i64), ("parents", _p), ("lens", _p), ("starts", _p),
+                ("bits", _p), ("depth", _p), ("positions", _p), ("status", _p)]
+
+
+class VerifyArgs(ctypes.Structure):
+    """``fade_verify_args`` of include/fade_hip.h."""
+
+    _fields_ = [
+        ("B", _i64), ("T", _i64), ("V", _i64), ("max_path", _i64),
+        ("target", _p), ("target_st", _i64), ("draft", _p), ("draft_st", _i64),
+        ("tokens", _p), ("parents", _p), ("starts", _p), ("uniforms", _p), ("final_u", _p),
+        ("path", _p), ("counts", _p), ("tokens_out", _p), ("next", _p), ("dtype", _i32), ("tok64", _i32),
+    ]
+
+
+class PageForkArgs(ctypes.Structure):
+    """``fade_page_fork_args`` of include/fade_hip.h."""
+
+    _fields_ = [
+        ("B", _i64), ("R", _i64), ("pages_per_row", _i64), ("n_free", _i64),
+        ("lens", _p), ("source", _p), ("keep", _p), ("table", _p), ("free_pages", _p), ("ring", _p),
+        ("table_out", _p), ("lens_out", _p), ("copies", _p), ("ring_out", _p), ("status", _p),
+    ]
+
+
+class PagedMoveArgs(ctypes.Structure):
+    """``fade_paged_move_args`` of include/fade_hip.h."""
+
+    _fields_ = [
+        ("n_pools", _i64), ("n_pages", _i64), ("Hkv", _i64), ("D", _i64), ("pools", _p), ("rows", _i64), ("copies", _p),
+        ("max_path", _i64), ("pages_per_row", _i64), ("path", _p), ("counts", _p), ("table", _p), ("lens", _p), ("starts", _p),
+        ("kept", _p),
     ]
 
 
@@ -253,6 +298,13 @@ _SIGNATURES: dict[str, list] = {
     "fade_paged_append": [ctypes.POINTER(RopeArgs), _p],
     "fade_paged_attn_workspace_bytes": [ctypes.POINTER(PagedAttnArgs), _pi64],
     "fade_paged_attn": [ctypes.POINTER(PagedAttnArgs), _p, _i64, _p],
+    "fade_draft_tree": [ctypes.POINTER(DraftTreeArgs), _p],
+    "fade_verify_workspace_bytes": [ctypes.POINTER(VerifyArgs), _pi64],
+    "fade_verify_drafts": [ctypes.POINTER(VerifyArgs), _p, _i64, _p],
+    "fade_page_fork_workspace_bytes": [ctypes.POINTER(PageForkArgs), _pi64],
+    "fade_page_fork": [ctypes.POINTER(PageForkArgs), _p, _i64, _p],
+    "fade_paged_copy": [ctypes.POINTER(PagedMoveArgs), _p],
+    "fade_paged_compact": [ctypes.POINTER(PagedMoveArgs), _p],
 }
 _RESTYPES = {"fade_hip_last_error": ctypes.c_char_p}
 
@@ -307,6 +359,7 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
+_WORKSPACE_OF = {"fade_verify_drafts": "fade_verify_workspace_bytes", "fade_page_fork": "fade_page_fork_workspace_bytes"}
 _GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
@@ -320,6 +373,22 @@ def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
         return
     with torch.cuda.device(device):
         check(getattr(load(), name)(ctypes.byref(args), current_stream_handle(device)), name)
+
+
+def launch_with_workspace(name: str, args: ctypes.Structure, device: torch.device) -> None:
+    """``launch`` of an entry point with a workspace, taken for the call and returned with it."""
+    if device.index != _GET_DEVICE():
+        with torch.cuda.device(device):
+            return launch_with_workspace(name, args, device)
+    lib, a = _lib or load(), ctypes.byref(args)
+    need = ctypes.c_int64(0)
+    rc = getattr(lib, _WORKSPACE_OF[name])(a, need)
+    if not rc:
+        n = need.value
+        ws = scratch(n, device) if n else None
+        rc = getattr(lib, name)(a, None if ws is None else ws.data_ptr(), n, current_stream_handle(device))
+    if rc:
+        check(rc, name)
 
 
 def no_gradient(op: str, *tensors: torch.Tensor | None) -> None:

@@ -3,7 +3,8 @@
 // Row b brings n_b = starts[b + 1] - starts[b] new tokens (one in a decoding step,
 // any number in a prompt's chunk) and holds L_b = lens[b] tokens, the new ones
 // included, in pages of 64: token i lies in page table[b][i / 64].  Query i of the
-// row sees keys 0 .. L_b - n_b + i (bottom-right causal) or all L_b:
+// row sees keys 0 .. L_b - n_b + i (bottom-right causal), all L_b, or those that the
+// row held before its new tokens and the new ones of its own mask (draft trees):
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = exp2((q.k_j - m) * scale * log2 e)
 // in one pass over the keys with the running maximum m and the sums in fp32.  A
 // query that sees no key gets zeros.
@@ -72,6 +73,8 @@ struct Params {
   const int32_t* starts;
   float scale_log2;
   int causal;
+  const uint32_t* tree;  // [T][words]: the row's new tokens that each one sees, as bits
+  int words;
   int zero_tail;
   // the cut of one kernel's work
   int rows_of;     // kAll, or the rows of the batch whose matrix rows fit one tile of 16 (kFew) or do not (kMany)
@@ -284,6 +287,23 @@ __device__ __forceinline__ void zero_tail(const Params& p, int end, int64_t bloc
       p.out[t * p.o_st + (static_cast<int64_t>(kvh) * G + i / p.D) * p.o_sh + i % p.D] = 0;
 }
 
+// Draft trees: of the 32 keys from `key` on, those that a query sees, as bits.  It sees
+// what the row held before its new tokens (keys up to `base`) and the new tokens of its
+// mask `at`; `lim`: the row's tokens, or 0 for a matrix row that holds none.
+__device__ __forceinline__ uint32_t seen_of(const uint32_t* at, int words, int key, int base, int lim) {
+  const int off = key - base, left = lim - key;
+  if (left <= 0) return 0;
+  uint32_t v = ~0u;
+  if (off >= 0) {
+    const int w = off >> 5;
+    const uint64_t lo = w < words ? at[w] : 0u, hi = w + 1 < words ? at[w + 1] : 0u;
+    v = static_cast<uint32_t>((hi << 32 | lo) >> (off & 31));
+  } else if (off > -32) {
+    v = at[0] << -off | ((1u << -off) - 1u);
+  }
+  return left < 32 ? v & ((1u << left) - 1u) : v;
+}
+
 // The end of a workgroup.  What the second launch has to join: the piece's last
 // tile, if it begins here and ends elsewhere.
 __device__ __forceinline__ void finish(const Params& p, const Walk& k, bool any) {
@@ -391,7 +411,7 @@ __device__ __forceinline__ int few_unit(int row, int u) {
   return u ^ ((2 * row) & Few<DP>::kSwizzle);
 }
 
-template <int DP, bool BF>
+template <int DP, bool BF, bool TREE>
 __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
   typedef Few<DP> F;
   constexpr int NKS = DP / 32, NCB = DP / 16;
@@ -421,7 +441,9 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
       return x < 0 ? 0 : x;
     };
     const int lim = live ? limit(qi) : 0;
-    const int seen_by_all = __builtin_amdgcn_readfirstlane(limit(w.tile * kRows / p.G));  // the tile's first row sees the fewest
+    const int held = w.len > w.n ? w.len - w.n : 0;  // keys ahead of the new tokens
+    const int seen_by_all = __builtin_amdgcn_readfirstlane(TREE ? held : limit(w.tile * kRows / p.G));  // (the tile's first row sees the fewest)
+    const uint32_t* const sight = TREE ? p.tree + static_cast<int64_t>(w.q0 + qi) * p.words : nullptr;
 
     const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + w.b * p.ppr);  // (scalar loads: vmcnt counts the steps' alone)
     auto issue = [&](int key, int id, int buf) {
@@ -476,6 +498,9 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
       m = -INFINITY;
       l = 0.0f;
       for (int t = 0; key < k.hi; key += F::kKeys, t = t + 1 == F::kStages ? 0 : t + 1) {
+        const bool whole = key + F::kKeys <= seen_by_all;
+        uint32_t vis = 0;  // (asked for ahead of the wait for the step)
+        if (TREE && !whole) vis = seen_of(sight, p.words, key, w.len - w.n, lim);
         if (ahead < k.hi) {
           issue(ahead, __builtin_amdgcn_readfirstlane(next), t == 0 ? F::kStages - 1 : t - 1);
           ahead += F::kKeys;
@@ -504,11 +529,11 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
           }
         }
         float x[8], tm = -INFINITY;
-        const bool whole = key + F::kKeys <= seen_by_all;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[i] = s[i >> 2][i & 3] * p.scale_log2;
-          if (!whole && key + 16 * (i >> 2) + 4 * g + (i & 3) >= lim) x[i] = -INFINITY;
+          if (!whole && (TREE ? (vis >> (4 * g) >> (16 * (i >> 2) + (i & 3)) & 1u) == 0 : key + 16 * (i >> 2) + 4 * g + (i & 3) >= lim))
+            x[i] = -INFINITY;
           tm = fmaxf(tm, x[i]);
         }
         tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
@@ -549,13 +574,15 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[cb][i] *= alpha;
 #pragma unroll 1
-          for (int j = 0; j < F::kKeys && key + j < lim; ++j)
+          for (int j = 0; j < F::kKeys && key + j < lim; ++j) {
+            if (TREE && !whole && (vis >> j & 1u) == 0) continue;
 #pragma unroll
             for (int cb = 0; cb < NCB; ++cb) {  // channels 16 cb + 4 g .. + 3
               const u32x2 v = *reinterpret_cast<const u32x2*>(vt + j * DP * 2 + 16 * few_unit<DP>(j, 2 * cb + (g >> 1)) + 8 * (g & 1));
 #pragma unroll
               for (int i = 0; i < 4; ++i) acc[cb][i] = Odd<BF>::added(acc[cb][i], v[i >> 1] >> (16 * (i & 1)));
             }
+          }
           Odd<BF>::template clear<F::kTensor, 64>(vt);
           asm volatile("" ::: "memory");
           alpha = 1.0f;
@@ -660,7 +687,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <int DP, int NW, int KT, int NST, bool BF>
+template <int DP, int NW, int KT, int NST, bool BF, bool TREE>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_wide_kernel(Params p) {
   constexpr int M = 32 * NW;
   constexpr int NKS = DP / 16, NCB = DP / 32, UNITS = DP / 8;
@@ -739,7 +766,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int r0 = w.tile * M + 32 * wave;
     const bool active = r0 < all;
     const int rl = r0 + 32 < all ? r0 + 32 : all;
-    const int wlo = __builtin_amdgcn_readfirstlane(active ? limit(r0 / p.G) : 0);
+    const int wlo = __builtin_amdgcn_readfirstlane(!active ? 0 : (!TREE ? limit(r0 / p.G) : (w.len > w.n ? w.len - w.n : 0)));
     const int whi = __builtin_amdgcn_readfirstlane(active ? limit((rl - 1) / p.G) : 0);
     const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + w.b * p.ppr);  // (scalar loads: vmcnt counts the steps' alone)
     auto issue = [&](int key, int id, int buf) {
@@ -775,6 +802,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       hd = kvh * p.G + r - qi * p.G;
     };
     int lim;
+    const uint32_t* sight = nullptr;
     f32x16 acc[NCB];
     float m, l;  // of row n32: the running maximum (raw scores), the sum over this half's keys
     for (bool again = false;; again = true) {
@@ -795,6 +823,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         int qi, hd;
         row(qi, hd);
         lim = live ? limit(qi) : 0;
+        if (TREE) sight = p.tree + static_cast<int64_t>(w.q0 + qi) * p.words;
         const uint16_t* qr = p.q + static_cast<int64_t>(w.q0 + qi) * p.q_st + static_cast<int64_t>(hd) * p.q_sh;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
@@ -815,6 +844,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       for (int i = 1; i < NST - 1; ++i)
         if (ahead < k.hi) issue_next(buf + i < NST ? buf + i : buf + i - NST);
       for (int key = k.lo; key < k.hi; key += KT, flip()) {
+        uint32_t vis[NKB];  // (asked for ahead of the wait for the step)
+        if (TREE && key + KT > wlo) {
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) vis[kb] = seen_of(sight, p.words, key + 32 * kb, w.len - w.n, lim);
+        }
         // this wave's share of the step: later steps' may be in flight
         const int later = ahead - key - KT;
         if (NST > 3 && later > KT) __builtin_amdgcn_s_waitcnt(vmcnt_imm(4 * LPW));
@@ -867,7 +901,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             __builtin_amdgcn_sched_barrier(kCompute);
           }
         }
-        if (key + KT > wlo) {
+        if (TREE && key + KT > wlo) {
+#pragma unroll
+          for (int kb = 0; kb < NKB; ++kb) {
+            const uint32_t v = vis[kb] >> (4 * h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if ((v >> (8 * (i >> 2) + (i & 3)) & 1u) == 0) s[kb][i] = -INFINITY;
+          }
+        } else if (key + KT > wlo) {
           const int left = lim - key - 4 * h;
 #pragma unroll
           for (int kb = 0; kb < NKB; ++kb)
@@ -922,7 +964,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
           }
           if (odd) {
 #pragma unroll 1
-            for (int j = 0; j < KT && key + j < lim; ++j)
+            for (int j = 0; j < KT && key + j < lim; ++j) {
+              if (TREE && key + KT > wlo && ((j < 32 ? vis[0] : vis[NKB - 1]) >> (j & 31) & 1u) == 0) continue;
 #pragma unroll
               for (int cb = 0; cb < NCB; ++cb)
 #pragma unroll
@@ -931,6 +974,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
                   for (int i = 0; i < 4; ++i) acc[cb][4 * q + i] = Odd<BF>::added(acc[cb][4 * q + i], v[i >> 1] >> (16 * (i & 1)));
                 }
+            }
             __syncthreads();
             Odd<BF>::template clear<TENSOR, 64 * NW>(vt);
             __syncthreads();
@@ -1139,8 +1183,11 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   if (!aligned16(a->k_pages) || !aligned16(a->v_pages)) return einval("%s: pages must be 16-byte aligned", what);
   if (a->dtype != FADE_DTYPE_F16 && a->dtype != FADE_DTYPE_BF16)
     return einval("%s: dtype must be FADE_DTYPE_F16 or FADE_DTYPE_BF16, got %d", what, a->dtype);
-  if (a->mask_mode != FADE_MASK_BOTTOM_RIGHT && a->mask_mode != FADE_MASK_NONE)
-    return einval("%s: mask_mode must be FADE_MASK_BOTTOM_RIGHT or FADE_MASK_NONE, got %d", what, a->mask_mode);
+  const bool tree = a->mask_mode == FADE_MASK_TREE;
+  if (a->mask_mode != FADE_MASK_BOTTOM_RIGHT && a->mask_mode != FADE_MASK_NONE && !tree)
+    return einval("%s: mask_mode must be FADE_MASK_BOTTOM_RIGHT, FADE_MASK_NONE or FADE_MASK_TREE, got %d", what, a->mask_mode);
+  if (tree && (!a->tree || a->tree_words < 1 || a->tree_words > (1 << 20) || (reinterpret_cast<uintptr_t>(a->tree) & 3)))
+    return einval("%s: FADE_MASK_TREE needs tree, 4-byte aligned, with 1 to 2^20 words a token", what);
   if (!(a->sm_scale > 0.0f) || !(a->sm_scale < INFINITY)) return einval("%s: sm_scale must be positive and finite", what);
   Params p{};
   p.B = a->B;
@@ -1164,6 +1211,8 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   p.starts = a->starts;
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   p.causal = a->mask_mode == FADE_MASK_BOTTOM_RIGHT;
+  p.tree = tree ? a->tree : nullptr;
+  p.words = tree ? static_cast<int>(a->tree_words) : 0;
   p.zero_tail = a->zero_tail;
   // Rows whose matrix rows fit one tile of 16 go to the few-row kernel, the others
   // to the wide one (16 rows over 8192 keys each, 32 matrix rows a row: 113 us, by the
@@ -1202,15 +1251,15 @@ int64_t part_bytes(const Plan& pl) {
   return n == 0 ? 0 : cut_bytes(pl.few) + cut_bytes(pl.wide) + n * (pl.few.D * 4 + static_cast<int64_t>(sizeof(float2)));
 }
 
-template <int DP, bool BF>
+template <int DP, bool BF, bool TREE>
 int launch(const Plan& pl, hipStream_t st) {
   if (pl.both) {
     typedef Wide<DP> W;
-    hipLaunchKernelGGL((paged_wide_kernel<DP, W::NW, W::KT, W::NST, BF>), dim3(static_cast<unsigned>(pl.wide.Hkv * pl.wide.pieces)), dim3(64 * W::NW), 0, st, pl.wide);
+    hipLaunchKernelGGL((paged_wide_kernel<DP, W::NW, W::KT, W::NST, BF, TREE>), dim3(static_cast<unsigned>(pl.wide.Hkv * pl.wide.pieces)), dim3(64 * W::NW), 0, st, pl.wide);
     const int rc = check_launch("fade_paged_attn");
     if (rc) return rc;
   }
-  hipLaunchKernelGGL((paged_few_kernel<DP, BF>), dim3(static_cast<unsigned>(pl.few.Hkv * pl.few.pieces)), dim3(64), 0, st, pl.few);
+  hipLaunchKernelGGL((paged_few_kernel<DP, BF, TREE>), dim3(static_cast<unsigned>(pl.few.Hkv * pl.few.pieces)), dim3(64), 0, st, pl.few);
   const int rc = check_launch("fade_paged_attn");
   // (the last piece's tiles end in it)
   const int wide = pl.both ? pl.wide.Hkv * (pl.wide.pieces - 1) * kWideBlocks : 0, few = pl.few.Hkv * (pl.few.pieces - 1) * kFewBlocks;
@@ -1219,12 +1268,12 @@ int launch(const Plan& pl, hipStream_t st) {
   return check_launch("fade_paged_attn (merge)");
 }
 
-template <bool BF>
+template <bool BF, bool TREE>
 int launch_any(const Plan& pl, void* stream) {
   hipStream_t st = as_stream(stream);
-  if (pl.few.D <= 64) return launch<64, BF>(pl, st);
-  if (pl.few.D <= 128) return launch<128, BF>(pl, st);
-  return launch<256, BF>(pl, st);
+  if (pl.few.D <= 64) return launch<64, BF, TREE>(pl, st);
+  if (pl.few.D <= 128) return launch<128, BF, TREE>(pl, st);
+  return launch<256, BF, TREE>(pl, st);
 }
 
 }  // namespace
@@ -1260,5 +1309,6 @@ FADE_API int fade_paged_attn(const fade_paged_attn_args* a, void* workspace, int
     pl.wide.part_o = pl.few.part_o + few * pl.few.D;
     pl.wide.part_ml = pl.few.part_ml + few;
   }
-  return a->dtype == FADE_DTYPE_BF16 ? launch_any<true>(pl, stream) : launch_any<false>(pl, stream);
+  if (a->mask_mode == FADE_MASK_TREE) return a->dtype == FADE_DTYPE_BF16 ? launch_any<true, true>(pl, stream) : launch_any<false, true>(pl, stream);
+  return a->dtype == FADE_DTYPE_BF16 ? launch_any<true, false>(pl, stream) : launch_any<false, false>(pl, stream);
 }

@@ -11,12 +11,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+from collections.abc import Sequence
 
 import torch
 from torch import Tensor
 
 from .. import _lib
-from ..pages import PAGE_TOKENS
+from ..pages import PAGE_TOKENS, PageLayers
 from ..rope import RopeScheme, rope_args
 from .tiered_attn import _attn_dtype
 
@@ -115,7 +116,76 @@ def paged_append(
     return q_out
 
 
-_MASKS = {"bottom_right": _lib.MASK_BOTTOM_RIGHT, "none": _lib.MASK_NONE}
+def _layers(layers: PageLayers | Sequence[Tensor]) -> PageLayers:
+    return layers if isinstance(layers, PageLayers) else PageLayers(layers)
+
+
+def _move_args(layers: PageLayers) -> _lib.PagedMoveArgs:
+    a = _lib.PagedMoveArgs()
+    a.n_pools, a.n_pages, a.Hkv, a.D, a.pools = len(layers.pages), layers.n_pages, layers.n_kv_heads, layers.head_dim, layers.pointers
+    return a
+
+
+def _counts(op: str, device: torch.device, **tensors: tuple[Tensor, tuple]) -> None:
+    for name, (t, shape) in tensors.items():
+        if t.dtype is not torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} {list(t.shape)}")
+        if t.device != device:
+            raise ValueError(f"{op}: {name} is on {t.device}, the pages on {device}")
+
+
+def paged_copy(copies: Tensor, layers: PageLayers | Sequence[Tensor]) -> None:
+    """The copies that ``page_fork`` lists, made in the K and V pages of every layer by one launch.
+
+    ``copies`` int32 [R, 3]: page, its copy's page, tokens (the first ones of the page, 0 for no
+    copy); no page twice among the copies' pages, and none of them copied from.  ``layers``: the
+    pages ([n_pages, Hkv, 64, D] each), or better the ``PageLayers`` of them that a program
+    keeps.  Copies from or to pages outside the pool (page 0 included) are not made."""
+    op = "paged_copy"
+    layers = _layers(layers)
+    _lib.require_gpu(copies, op=op)
+    _counts(op, layers.device, copies=(copies, (copies.shape[0] if copies.dim() else 0, 3)))
+    layers.written(op, copies=copies)
+    a = _move_args(layers)
+    a.rows, a.copies = copies.shape[0], copies.data_ptr()
+    _lib.launch("fade_paged_copy", a, layers.device)
+
+
+def paged_compact(
+    path: Tensor,
+    counts: Tensor,
+    table: Tensor,
+    lens: Tensor,
+    starts: Tensor,
+    layers: PageLayers | Sequence[Tensor],
+) -> Tensor:
+    """Keep a path of each row's drafted tokens: K and V of its tokens to consecutive places, in
+    every layer, by one launch; returns the tokens that each row then has (int32 [B], for
+    ``page_fork``'s ``keep``).
+
+    Row b holds ``lens[b]`` tokens in the pages of ``table`` [B, pages_per_row], its last
+    ``n = starts[b + 1] - starts[b]`` ones drafted.  ``path`` int32 [B, max_path] numbers the
+    ones that stay, rising (``verify_drafts``), ``counts`` [B] how many of them; token
+    ``lens - n + path[b, i]`` goes to place ``lens - n + i``.  Numbers outside 0 .. n - 1 move
+    nothing.  The drafted tokens' pages must be the row's own, as ``page_fork`` leaves them.
+    ``layers``: the pages of all layers, or better the ``PageLayers`` of them."""
+    op = "paged_compact"
+    layers = _layers(layers)
+    _lib.require_gpu(path, counts, table, lens, starts, op=op)
+    if table.dim() != 2 or path.dim() != 2:
+        raise ValueError(f"{op}: table must be [B, pages_per_row] and path [B, max_path], got {tuple(table.shape)} and {tuple(path.shape)}")
+    B, ppr = table.shape
+    _counts(op, layers.device, path=(path, (B, path.shape[1])), counts=(counts, (B,)), table=(table, (B, ppr)), lens=(lens, (B,)), starts=(starts, (B + 1,)))
+    layers.written(op, path=path, counts=counts, table=table, lens=lens, starts=starts)
+    kept = torch.empty_like(lens)
+    a = _move_args(layers)
+    a.rows, a.max_path, a.pages_per_row = B, path.shape[1], ppr
+    a.path, a.counts, a.table, a.lens, a.starts, a.kept = (t.data_ptr() for t in (path, counts, table, lens, starts, kept))
+    _lib.launch("fade_paged_compact", a, layers.device)
+    return kept
+
+
+_MASKS = {"bottom_right": _lib.MASK_BOTTOM_RIGHT, "none": _lib.MASK_NONE, "tree": _lib.MASK_TREE}
 
 
 class PagedAttentionPlan:
@@ -134,10 +204,14 @@ class PagedAttentionPlan:
         table: int32 [B, pages_per_row], the pages of each row.
         lens: int32 [B], each row's tokens in its pages, the new ones included.
         starts: int32 [B + 1], the first of each row's tokens in q and their end; ``starts[0]`` is 0.
-        mask: ``"bottom_right"`` (query i of a row's n sees keys 0 .. lens - n + i) or
-            ``"none"`` (all lens of them, as a decoder's queries see an encoder's states).
+        mask: ``"bottom_right"`` (query i of a row's n sees keys 0 .. lens - n + i),
+            ``"none"`` (all lens of them, as a decoder's queries see an encoder's states) or
+            ``"tree"`` (keys 0 .. lens - n - 1, and of the row's n new tokens those of ``tree``).
         out: like q, contiguous along D, q itself or other memory; rows at and past ``starts[B]``
             are left as they are.  Default: a new tensor, zeros there.
+        tree: with the mask ``"tree"``: int32 [tokens, words], for each new token the row's new
+            tokens that it sees, number j as bit j % 32 of word j / 32 (``draft_tree``'s ``bits``, or
+            any other mask; tokens past the words are not seen).
 
     A query that sees no key, or none with a score over -inf, gets zeros; a NaN or an infinity
     in a value reaches the queries that see its key and no others.  Probabilities times
@@ -157,13 +231,16 @@ class PagedAttentionPlan:
         sm_scale: float | None = None,
         mask: str = "bottom_right",
         out: Tensor | None = None,
+        tree: Tensor | None = None,
     ) -> None:
         op = "paged_attention"
         if q.dim() != 3:
             raise ValueError(f"{op}: q must be [tokens, Hq, D], got {tuple(q.shape)}")
         if mask not in _MASKS:
             raise ValueError(f"{op}: mask must be one of {sorted(_MASKS)}, got {mask!r}")
-        _lib.require_gpu(q, k_pages, v_pages, table, lens, starts, out, op=op)
+        if (tree is None) != (mask != "tree"):
+            raise ValueError(f'{op}: the mask "tree" needs tree, and tree that mask')
+        _lib.require_gpu(q, k_pages, v_pages, table, lens, starts, out, tree, op=op)
         _lib.no_gradient(op, q, k_pages, v_pages, out)
         dtc = _attn_dtype(q, op)
         n_pages, Hkv, D = _check_pages(op, k_pages, v_pages, q.dtype)
@@ -176,6 +253,8 @@ class PagedAttentionPlan:
         for name, t, shape in (("table", table, (B, ppr)), ("lens", lens, (B,)), ("starts", starts, (B + 1,))):
             if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} {list(t.shape)}")
+        if tree is not None and (tree.dtype != torch.int32 or tree.dim() != 2 or tree.shape[0] != T or tree.shape[1] < 1 or not tree.is_contiguous()):
+            raise ValueError(f"{op}: tree must be a contiguous int32 [{T}, words], got {tree.dtype} {list(tree.shape)}")
         # (the stride of an axis of one element is never used, whatever it says)
         q_st, q_sh = q.stride(0) if T > 1 else 0, q.stride(1) if Hq > 1 else 0
         if q.is_neg() or q.stride(2) != 1 or (q_st | q_sh) % 8 or q.data_ptr() % 16:
@@ -188,7 +267,7 @@ class PagedAttentionPlan:
                 or not _lib.each_once(out) or out.data_ptr() % 8:
             raise ValueError(f"{op}: out must be {q.dtype} {tuple(q.shape)} with a contiguous head_dim axis, 8-byte aligned rows and no row twice")
         if not self._fresh:
-            _lib.apart(op, "out", out, q, k_pages=k_pages, v_pages=v_pages, table=table, lens=lens, starts=starts)
+            _lib.apart(op, "out", out, q, k_pages=k_pages, v_pages=v_pages, table=table, lens=lens, starts=starts, tree=tree)
         a = _lib.PagedAttnArgs()
         a.B, a.T, a.Hq, a.Hkv, a.D, a.n_pages, a.pages_per_row = B, T, Hq, Hkv, D, n_pages, ppr
         a.q, a.q_st, a.q_sh = q.data_ptr(), q_st, q_sh
@@ -197,7 +276,9 @@ class PagedAttentionPlan:
         a.table, a.lens, a.starts = table.data_ptr(), lens.data_ptr(), starts.data_ptr()
         a.sm_scale = float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale)
         a.mask_mode, a.dtype, a.zero_tail = _MASKS[mask], dtc, int(self._fresh)
-        self._keep = (q, k_pages, v_pages, table, lens, starts)
+        if tree is not None:
+            a.tree, a.tree_words = tree.data_ptr(), tree.shape[1]
+        self._keep = (q, k_pages, v_pages, table, lens, starts, tree)
         self.args, self.out = a, out
         self._argp = ctypes.byref(a)
         nb = ctypes.c_int64(0)
@@ -231,10 +312,11 @@ def paged_attention(
     sm_scale: float | None = None,
     mask: str = "bottom_right",
     out: Tensor | None = None,
+    tree: Tensor | None = None,
 ) -> Tensor:
     """Attention of each row's new tokens ``q`` [tokens, Hq, D] over the row's pages;
     returns [tokens, Hq, D] of q's dtype.  See ``PagedAttentionPlan`` for the arguments."""
-    return PagedAttentionPlan(q, k_pages, v_pages, table, lens, starts, sm_scale, mask, out).run()
+    return PagedAttentionPlan(q, k_pages, v_pages, table, lens, starts, sm_scale, mask, out, tree).run()
 
 
-__all__ = ["PagedAttentionPlan", "paged_append", "paged_attention"]
+__all__ = ["PagedAttentionPlan", "paged_append", "paged_attention", "paged_compact", "paged_copy"]

@@ -29,6 +29,7 @@ read of it in stream order.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -253,6 +254,114 @@ def page_slots(
     return out
 
 
+@dataclass
+class PageFork:
+    """What ``page_fork`` writes (int32, on the GPU).
+
+    ``table`` [R, pages_per_row], ``lens`` [R]: the rows' pages and tokens.  ``copies`` [R, 3]:
+    the page that row r goes on from, the page of its own that takes its place, and the tokens
+    in it (zeros: no copy), for ``paged_copy``.  ``ring`` [2], ``status`` [1] as in ``PageSlots``."""
+
+    table: Tensor
+    lens: Tensor
+    copies: Tensor
+    ring: Tensor
+    status: Tensor
+
+    def check(self) -> "PageFork":
+        """Raise RuntimeError where the call was not done (reads the status: a host synchronization)."""
+        word = int(self.status.item())
+        if word:
+            what = ", ".join(t for b, t in _lib.FORK_STATUS.items() if word & b)
+            raise RuntimeError(f"page_fork: {what} (nothing was changed)")
+        return self
+
+
+def page_fork(
+    lens: Tensor,
+    table: Tensor,
+    free: Tensor,
+    ring: Tensor,
+    source: Tensor | None = None,
+    keep: Tensor | None = None,
+) -> PageFork:
+    """Rows that go on from other rows: samples of one prompt, beams, rows cut back or dropped;
+    without a host synchronization.
+
+    Row r of the result holds the first ``keep[r]`` tokens (int32 [R]; default, and where it has
+    fewer: all) of row ``source[r]`` (int32 [R], -1: an empty row; default: row r itself) of the B rows
+    of ``lens`` [B] and ``table`` [B, pages_per_row] (B, R up to 4096), in the same pages.  The page that a row
+    goes on writing, its last one where that is not full, is its own: of the rows that end in one
+    page the first keeps it, unless a row holds it as a full one, and the others get a free page,
+    listed in ``copies``.  Pages without a row are returned to the ring, in the order of their
+    numbers.  ``free`` int32 [n] and ``ring`` [2] as in ``page_slots``; pages are numbered
+    1 .. n.  ``page_slots``' ``reset`` returns pages without a look at other rows: rows that may
+    share pages are dropped here, as ``source[r] = -1``.
+
+    All or nothing: where free pages run out, or a source, a count or a page is impossible,
+    ``status`` says so, row r comes out as row r went in (empty from row B on), without copies.
+    The same inputs give the same results again, so a captured graph can be replayed on them."""
+    op = "page_fork"
+    _lib.require_gpu(lens, table, free, ring, source, keep, op=op)
+    if table.dim() != 2:
+        raise ValueError(f"{op}: table must be [B, pages_per_row], got {tuple(table.shape)}")
+    B, ppr = table.shape
+    R = B if source is None else source.numel()
+    for name, t, size in (("lens", lens, B), ("table", table, B * ppr), ("free", free, free.numel()), ("ring", ring, 2), ("source", source, R), ("keep", keep, R)):
+        if t is not None and (t.dtype is not torch.int32 or t.numel() != size or not t.is_contiguous() or (t.dim() != 1 and t is not table)):
+            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of {size} elements, got {t.dtype} {list(t.shape)}")
+    sizes = (R * ppr, R, 3 * R, 2, 1)
+    buf = table.new_empty(sum(sizes))
+    parts = buf.split_with_sizes(sizes)
+    ptrs, at = [], buf.data_ptr()
+    for size in sizes:
+        ptrs.append(at)
+        at += 4 * size
+    _lib.written(op, free)
+    a = _lib.PageForkArgs(B, R, ppr, free.numel(), lens.data_ptr(), _lib.ptr(source), _lib.ptr(keep), table.data_ptr(), free.data_ptr(),
+                          ring.data_ptr(), *ptrs)
+    _lib.launch_with_workspace("fade_page_fork", a, table.device)
+    return PageFork(parts[0].view(R, ppr), parts[1], parts[2].view(R, 3), parts[3], parts[4])
+
+
+class PageLayers:
+    """The pages of several layers, checked once: ``pages``, a sequence of tensors
+    [n_pages, Hkv, 64, D] (each layer's K and V), fp16 or bf16, alike and contiguous, each with
+    memory of its own.  Moves within them (``paged_copy``, ``paged_compact``) take all of them in one launch."""
+
+    def __init__(self, pages) -> None:
+        op = "PageLayers"
+        self.pages = tuple(pages)
+        if not self.pages:
+            raise ValueError(f"{op}: needs at least one tensor of pages")
+        first = self.pages[0]
+        for t in self.pages:
+            if t.dim() != 4 or t.shape[2] != PAGE_TOKENS or t.shape[0] < 1 or t.shape[1] < 1 or t.shape[3] < 8 or t.shape[3] % 8 or t.shape[3] > 256:
+                raise ValueError(f"{op}: pages must be [n_pages, Hkv, {PAGE_TOKENS}, D], D a multiple of 8 up to 256, got {tuple(t.shape)}")
+            if t.shape != first.shape or t.dtype != first.dtype or t.dtype not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"{op}: pages must all be float16 or all bfloat16 of one shape, got {first.dtype} {tuple(first.shape)} and {t.dtype} {tuple(t.shape)}")
+            if not t.is_contiguous() or t.is_neg() or t.data_ptr() % 16:
+                raise ValueError(f"{op}: pages must be contiguous and 16-byte aligned")
+        _lib.require_gpu(*self.pages, op=op)
+        at = sorted(t.data_ptr() for t in self.pages)
+        if any(y - x < first.nbytes for x, y in zip(at, at[1:])):
+            raise ValueError(f"{op}: pages overlap in memory")
+        self.device = first.device
+        self.n_pages, self.n_kv_heads, self.head_dim = int(first.shape[0]), int(first.shape[1]), int(first.shape[3])
+        self._pointers = (ctypes.c_void_p * len(self.pages))(*(t.data_ptr() for t in self.pages))
+        self.pointers = ctypes.addressof(self._pointers)
+
+    def written(self, op: str, **read: Tensor) -> None:
+        """What a kernel that is about to write the pages looks at first: gradients, and ``read``'s memory."""
+        _lib.no_gradient(op, *self.pages)
+        first = self.pages[0]
+        for name, t in read.items():
+            at, end = t.data_ptr(), t.data_ptr() + t.nbytes
+            if t.numel() and any(x.data_ptr() < end and at < x.data_ptr() + first.nbytes for x in self.pages):
+                raise ValueError(f"{op}: {name} lies in the pages' memory")
+        _lib.written(op, *self.pages)
+
+
 class TokenPagePool:
     """``n_pages`` pages of 64 tokens of 16-bit K and V: ``k``, ``v`` [n_pages + 1, Hkv, 64, D]
     of ``dtype`` (page 0 holds no tokens), and the free pages on the GPU.
@@ -260,7 +369,12 @@ class TokenPagePool:
     One step of a batch: ``state = pool.step(state, new, n_tokens)`` gives every new
     token its slot, ``paged_append`` writes K and V there, ``paged_attention`` reads
     the rows' pages.  ``start`` gives the state of an empty batch.  Several layers share
-    one pool's tables by holding tensors like ``k`` and ``v`` of their own."""
+    one pool's tables by holding tensors like ``k`` and ``v`` of their own.
+
+    Rows branch and shrink: ``fork`` makes a batch whose rows go on from rows of another
+    (samples of one prompt, beams; -1 drops a row), ``accept`` keeps the verified path of each
+    row's drafted tokens.  Both take ``layers``, the ``PageLayers`` of all layers' pages, where
+    there are more than the pool's own ``k`` and ``v``."""
 
     def __init__(self, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16, device="cuda") -> None:
         if n_pages < 1 or n_kv_heads < 1 or head_dim < 8 or head_dim % 8 or head_dim > 256:
@@ -274,10 +388,19 @@ class TokenPagePool:
         self.v = torch.zeros(shape, dtype=dtype, device=device)
         self.free = torch.arange(1, self.n_pages + 1, dtype=torch.int32, device=device)
         self.ring = torch.tensor([0, self.n_pages], dtype=torch.int32, device=device)
+        self._own_layers: PageLayers | None = None
+        self._shared = False  # rows may share pages
 
     @property
     def device(self) -> torch.device:
         return self.k.device
+
+    @property
+    def layers(self) -> PageLayers:
+        """The pool's own pages, as ``fork`` and ``accept`` take them."""
+        if self._own_layers is None or self._own_layers.pages[0] is not self.k or self._own_layers.pages[1] is not self.v:
+            self._own_layers = PageLayers((self.k, self.v))
+        return self._own_layers
 
     def start(self, batch: int, pages_per_row: int) -> PageSlots:
         """The state of ``batch`` empty rows of at most ``pages_per_row`` pages."""
@@ -285,10 +408,38 @@ class TokenPagePool:
         return PageSlots(z(batch, pages_per_row), z(batch), z(batch + 1), z(0), z(0), self.ring, z(1))
 
     def step(self, state: PageSlots, new: Tensor, n_tokens: int, reset: Tensor | None = None) -> PageSlots:
-        """``page_slots`` for the next ``new[b]`` tokens of every row; the pool keeps the ring."""
+        """``page_slots`` for the next ``new[b]`` tokens of every row; the pool keeps the ring.  After a
+        ``fork`` rows may share pages, and finished ones are dropped by ``fork`` too, not by ``reset``."""
+        if reset is not None and self._shared:
+            raise ValueError("TokenPagePool.step: rows may share pages after fork; drop finished rows with fork (source -1) instead of reset")
         nxt = page_slots(state.lens, new, state.table, self.free, self.ring, n_tokens, reset=reset)
         self.ring = nxt.ring
         return nxt
+
+    def _rows(self, f: PageFork) -> PageSlots:
+        self.ring = f.ring
+        z = lambda n: torch.zeros(n, dtype=torch.int32, device=self.device)  # noqa: E731
+        return PageSlots(f.table, f.lens, z(f.lens.numel() + 1), z(0), z(0), f.ring, f.status)
+
+    def fork(self, state: PageSlots, source: Tensor, keep: Tensor | None = None, layers: PageLayers | None = None) -> PageSlots:
+        """The state of rows that go on from ``state``'s (``page_fork``): row r has the first ``keep[r]``
+        tokens (default: all) of row ``source[r]``, or none where that is -1.  Rows share full pages; the
+        page that each goes on writing is copied in every layer where it would be shared."""
+        from .kernels.paged import paged_copy
+
+        f = page_fork(state.lens, state.table, self.free, self.ring, source=source, keep=keep)
+        self._shared = True
+        paged_copy(f.copies, self.layers if layers is None else layers)
+        return self._rows(f)
+
+    def accept(self, state: PageSlots, path: Tensor, counts: Tensor, layers: PageLayers | None = None) -> PageSlots:
+        """The state after a step of drafted tokens of which each row keeps those numbered
+        ``path[b, :counts[b]]`` (``verify_drafts``): their K and V moved together in every layer,
+        the pages behind them returned."""
+        from .kernels.paged import paged_compact
+
+        kept = paged_compact(path, counts, state.table, state.lens, state.starts, self.layers if layers is None else layers)
+        return self._rows(page_fork(state.lens, state.table, self.free, self.ring, keep=kept))
 
     def gather(self, table: Tensor, length: int) -> tuple[Tensor, Tensor]:
         """K and V [B, Hkv, length, D] that a block table describes (what stands in a row's
@@ -307,4 +458,4 @@ class TokenPagePool:
         return one(self.k), one(self.v)
 
 
-__all__ = ["MiddlePagePool", "PAGE_TOKENS", "PageSlots", "TokenPagePool", "page_slots"]
+__all__ = ["MiddlePagePool", "PAGE_TOKENS", "PageFork", "PageLayers", "PageSlots", "TokenPagePool", "page_fork", "page_slots"]

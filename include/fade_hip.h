@@ -414,6 +414,7 @@ int fade_tiered_decode_attn_noalloc(const fade_decode_args* args, void* stream);
                                     [sink | middle | recent | chunk], as the reference's fused
                                     kernel applies is_causal (fade/kernels/fused_int4_attn.py:165-169) */
 #define FADE_MASK_NONE 2         /* every key visible to every query */
+#define FADE_MASK_TREE 3         /* fade_paged_attn: a mask of its own for each new token */
 /* A chunk of Sq new tokens per batch row attends to that row's cache
  * [sink | middle | recent] followed by the chunk itself, bottom-right causal:
  * query j of row b sees cache tokens and chunk tokens 0..j (mask_mode
@@ -534,7 +535,9 @@ int fade_paged_append(const fade_rope_args* args, void* stream);
 /* Attention of ragged chunks of new tokens over the pages: row b's queries are
  * tokens starts[b] .. starts[b + 1] - 1 of q, its keys the lens[b] tokens that its
  * pages hold, the new ones included.  mask_mode FADE_MASK_BOTTOM_RIGHT: query i of
- * n sees keys 0 .. lens[b] - n + i; FADE_MASK_NONE: all of them.  A query that sees no
+ * n sees keys 0 .. lens[b] - n + i; FADE_MASK_NONE: all of them; FADE_MASK_TREE: keys
+ * 0 .. lens[b] - n - 1 and the row's new token j where bit j % 32 of word j / 32 of
+ * the query's tree mask is set.  A query that sees no
  * key gets zeros; what stands in a page past a row's tokens never counts.  Rows of
  * out at and past starts[B] are left as they were, or zeroed (zero_tail).  Any
  * Hq / Hkv; D a multiple of 8 up to 256; dtype FADE_DTYPE_F16 or FADE_DTYPE_BF16. */
@@ -554,12 +557,135 @@ typedef struct fade_paged_attn_args {
   int32_t mask_mode;
   int32_t dtype;
   int32_t zero_tail;
+  const uint32_t* tree;      /* FADE_MASK_TREE (else not read): [T][tree_words] */
+  int64_t tree_words;
 } fade_paged_attn_args;
 /* The keys are split over workgroups by the rows' lengths, on the device; the
  * splits' fp32 sums go through the workspace (16-byte aligned, contents arbitrary,
  * not shared by calls that may overlap) and are joined in a fixed order. */
 int fade_paged_attn_workspace_bytes(const fade_paged_attn_args* args, int64_t* bytes);
 int fade_paged_attn(const fade_paged_attn_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------- speculative decoding and branching rows ------------------ */
+/* A row's new tokens may be a tree of drafted ones: token 0 is the row's last known
+ * token, parents[t] (below the token's own number in the row) the token that token t
+ * follows, -1 for one that follows none. */
+#define FADE_DRAFT_MAX_NODES 1024 /* of a row */
+/* status bits of a row */
+#define FADE_DRAFT_TOO_MANY 1   /* more new tokens than its masks have bits: the others see and are seen by none */
+#define FADE_DRAFT_BAD_PARENT 2 /* a parent that is no earlier token, taken for -1 */
+/* Row b's new tokens are starts[b] .. starts[b + 1] - 1 of parents, its tokens in the
+ * cache (the new ones included) lens[b].  Writes for each token the bits of the row's
+ * tokens that it sees (its ancestors and itself; fade_paged_attn's tree), its depth
+ * below the token that follows none, its position lens[b] - n + depth, and for each row
+ * its status.  Tokens at and past starts[B]: zeros. */
+typedef struct fade_draft_tree_args {
+  int64_t B, T, words; /* words: 1 to FADE_DRAFT_MAX_NODES / 32 */
+  const int32_t* parents; /* [T] */
+  const int32_t* lens;    /* [B] */
+  const int32_t* starts;  /* [B + 1] */
+  uint32_t* bits;         /* [T][words] */
+  int32_t* depth;         /* [T] */
+  int32_t* positions;     /* [T] */
+  int32_t* status;        /* [B] */
+} fade_draft_tree_args;
+int fade_draft_tree(const fade_draft_tree_args* args, void* stream);
+
+/* Which drafted tokens of each row stay, and the token after them, so that the result
+ * is distributed as the target's own tokens are.  target[t] are the probabilities of
+ * the token after t.  From token 0 on: the children of a token, in the order of their
+ * numbers, are accepted or refused one after the other, the walk goes on at the first
+ * accepted one, and where there is none, the next token is drawn from what is left of
+ * the token's probabilities.  With x the child's token, u its uniform number:
+ *   draft given (each child drawn from q = draft[parent] by itself): after k refusals
+ *     left_i = max(target_i - s q_i, 0) (s = 0; s += N, N = sum left at each refusal;
+ *     N = 1 first), accepted where u N q_x < left_x;
+ *   draft NULL (children chosen without chance): left_i = target_i, 0 at refused
+ *     tokens, N = 1 - sum of target at those; accepted where u N < left_x.
+ * The next token is the first i with left_0 + .. + left_i > final[b] * sum left; where
+ * nothing is left, left = target; where that has nothing above zero, -1.  Sums in
+ * 64 bits.  Probabilities that are not above zero (NaN too) count as 0; infinite ones
+ * give an unspecified token.  A path ends at max_path tokens, whose last one's children
+ * are not tried; tokens past a row's first FADE_DRAFT_MAX_NODES are not tried either.
+ * Writes path [B][max_path] (numbers in the row, -1 past the end), counts [B] (tokens of
+ * the path; 0 for a row without tokens), tokens_out [B][max_path] (the path's tokens
+ * after its first, then the next one, -1 past them) and next [B]. */
+typedef struct fade_verify_args {
+  int64_t B, T, V, max_path;
+  const void* target;     /* [T][V] at element stride target_st, unit stride along V */
+  int64_t target_st;
+  const void* draft;      /* the same, or NULL */
+  int64_t draft_st;
+  const void* tokens;     /* [T], int64 where tok64, else int32 */
+  const int32_t* parents; /* [T] */
+  const int32_t* starts;  /* [B + 1] */
+  const float* uniforms;  /* [T], in [0, 1) */
+  const float* final_u;   /* [B], in [0, 1) */
+  int32_t* path;
+  int32_t* counts;
+  void* tokens_out;       /* tokens' type */
+  void* next;             /* tokens' type */
+  int32_t dtype;          /* FADE_DTYPE_F16, BF16 or F32: target and draft */
+  int32_t tok64;
+} fade_verify_args;
+/* The workspace (16-byte aligned, contents arbitrary) must not be shared by calls that may overlap. */
+int fade_verify_workspace_bytes(const fade_verify_args* args, int64_t* bytes);
+int fade_verify_drafts(const fade_verify_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* status bits of fade_page_fork: FADE_SLOTS_EXHAUSTED, FADE_SLOTS_BAD_COUNT (a source, a
+ * length, a page or the ring that cannot be); with any of them set row r comes out as
+ * row r came in (empty from row B on), without copies, and the ring as it was */
+/* Row r goes on from row source[r] of the B rows (-1: an empty row; NULL: from row r) with
+ * its first keep[r] tokens (NULL: all of them; more than it has: all of them).  Rows share
+ * the pages of a common source, but the page that a row goes on writing (its last one, where
+ * that is not full) is its own: of the rows that end in one page the first keeps it, if no
+ * row holds it as a full one, and each other gets a free page and copies[r] = {page, its
+ * page, tokens} (zeros elsewhere) for fade_paged_copy.  Pages that the B rows held and none
+ * of the R rows does are returned to the ring, in the order of their numbers.  Pages are
+ * 1 .. n_free.  The ring as in fade_page_slots (whose reset must not be used on rows that
+ * share pages); what is written must be other memory than the rest of the call's. */
+typedef struct fade_page_fork_args {
+  int64_t B, R, pages_per_row, n_free; /* B, R: 1 to FADE_SLOTS_MAX_ROWS */
+  const int32_t* lens;     /* [B] */
+  const int32_t* source;   /* [R] or NULL (R == B) */
+  const int32_t* keep;     /* [R] or NULL */
+  const int32_t* table;    /* [B][pages_per_row] */
+  int32_t* free_pages;     /* [n_free] */
+  const int32_t* ring;     /* [2] */
+  int32_t* table_out;      /* [R][pages_per_row] */
+  int32_t* lens_out;       /* [R] */
+  int32_t* copies;         /* [R][3] */
+  int32_t* ring_out;       /* [2] */
+  int32_t* status;         /* [1] */
+} fade_page_fork_args;
+/* The workspace (16-byte aligned, contents arbitrary) must not be shared by calls that may overlap. */
+int fade_page_fork_workspace_bytes(const fade_page_fork_args* args, int64_t* bytes);
+int fade_page_fork(const fade_page_fork_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Tokens moved within the pages of n_pools tensors [n_pages][Hkv][64][D] of 16-bit
+ * elements (K and V of every layer), 16-byte aligned. */
+typedef struct fade_paged_move_args {
+  int64_t n_pools, n_pages, Hkv, D;
+  void* const* pools;      /* host array of device pointers */
+  int64_t rows;            /* R of copies, or B of paths */
+  const int32_t* copies;   /* fade_paged_copy: [R][3] */
+  int64_t max_path, pages_per_row; /* the rest: fade_paged_compact */
+  const int32_t* path;     /* [B][max_path] */
+  const int32_t* counts;   /* [B] */
+  const int32_t* table;    /* [B][pages_per_row] */
+  const int32_t* lens;     /* [B] */
+  const int32_t* starts;   /* [B + 1] */
+  int32_t* kept;           /* [B] */
+} fade_paged_move_args;
+/* The first copies[r][2] tokens (0 to 64) of page copies[r][0] to page copies[r][1], for every r;
+ * no page is written twice or both read and written.  Copies from or to pages outside 1 .. n_pages - 1
+ * are not made. */
+int fade_paged_copy(const fade_paged_move_args* args, void* stream);
+/* Of the n = starts[b + 1] - starts[b] last of row b's lens[b] tokens those numbered path[b][0] <
+ * path[b][1] < .. (counts[b] of them) move to the first counts[b] places of the n, in order;
+ * kept[b] = lens[b] - n + counts[b].  Path entries outside 0 .. n - 1 move nothing.  The places lie in pages
+ * that no other row holds. */
+int fade_paged_compact(const fade_paged_move_args* args, void* stream);
 
 #ifdef __cplusplus
 }
