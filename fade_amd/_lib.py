@@ -223,7 +223,7 @@ class VerifyArgs(ctypes.Structure):
         ("B", _i64), ("T", _i64), ("V", _i64), ("max_path", _i64),
         ("target", _p), ("target_st", _i64), ("draft", _p), ("draft_st", _i64),
         ("tokens", _p), ("parents", _p), ("starts", _p), ("uniforms", _p), ("final_u", _p),
-        ("path", _p), ("counts", _p), ("tokens_out", _p), ("next", _p), ("dtype", _i32), ("tok64", _i32),
+        ("path", _p), ("counts", _p), ("tokens_out", _p), ("next", _p), ("dtype", _i32), ("tok64", _i32), ("polls", _i32),
     ]
 
 
@@ -380,13 +380,15 @@ def launch_with_workspace(name: str, args: ctypes.Structure, device: torch.devic
     if device.index != _GET_DEVICE():
         with torch.cuda.device(device):
             return launch_with_workspace(name, args, device)
-    lib, a = _lib or load(), ctypes.byref(args)
-    need = ctypes.c_int64(0)
+    lib, a, need = _lib or load(), ctypes.byref(args), ctypes.c_int64(0)
     rc = getattr(lib, _WORKSPACE_OF[name])(a, need)
     if not rc:
         n = need.value
-        ws = scratch(n, device) if n else None
-        rc = getattr(lib, name)(a, None if ws is None else ws.data_ptr(), n, current_stream_handle(device))
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=device)
+            rc = getattr(lib, name)(a, ws.data_ptr(), n, current_stream_handle(device))
+        else:
+            rc = getattr(lib, name)(a, None, 0, current_stream_handle(device))
     if rc:
         check(rc, name)
 

@@ -235,6 +235,133 @@ __global__ __launch_bounds__(kThreads) void fork_write_kernel(Params p) {
   }
 }
 
+// Small calls: all of it in one workgroup, the pages' words in LDS.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallRows = kSmallThreads;  // one a thread
+constexpr int kSmallPages = 16384;
+constexpr int kSmallEntries = 65536;  // of both tables
+
+__global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(Params p) {
+  __shared__ uint32_t word[kSmallPages + 1], begun[kSmallPages + 1];
+  __shared__ int32_t s_len[kSmallRows], s_src[kSmallRows], s_n[kSmallRows], s_copy[kSmallRows];
+  __shared__ int32_t s_wave[kSmallThreads / 64];
+  __shared__ uint32_t s_bad;
+  const int tid = threadIdx.x, ppr = p.ppr;
+  const int head = p.ring[0], count = p.ring[1];
+  int len = tid < p.B ? p.lens[tid] : 0;
+  int src = tid >= p.R ? -1 : (p.source != nullptr ? p.source[tid] : tid);
+  const int keep = p.keep != nullptr && tid < p.R ? p.keep[tid] : 0x7FFFFFFF;
+  if (tid == 0) s_bad = 0;
+  for (int i = tid; i <= p.cap; i += kSmallThreads) word[i] = begun[i] = 0;
+  bool ok = len >= 0 && len <= static_cast<int64_t>(ppr) * kPage && src >= -1 && src < p.B && keep >= 0;
+  if (!ok) {
+    len = 0;
+    src = -1;
+  }
+  s_len[tid] = len;
+  s_src[tid] = src;
+  __syncthreads();
+  const int n = src < 0 ? 0 : (s_len[src] < keep ? s_len[src] : keep);
+  s_n[tid] = n;
+  __syncthreads();
+
+  // f(row, page of the row) over rows of ppr pages, four at a time
+  auto each = [&](int rows, auto&& load, auto&& use) {
+    constexpr int K = 4;
+    const int all = rows * ppr, step_row = kSmallThreads / ppr, step_j = kSmallThreads - step_row * ppr;
+    int row = tid / ppr, j = tid - row * ppr;
+    for (int e = tid; e < all; e += K * kSmallThreads) {
+      int rows_of[K], js[K], ids[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        rows_of[k] = row;
+        js[k] = j;
+        ids[k] = e + k * kSmallThreads < all ? load(row, j) : 0;
+        row += step_row;
+        j += step_j;
+        if (j >= ppr) {
+          j -= ppr;
+          ++row;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (e + k * kSmallThreads < all) use(rows_of[k], js[k], ids[k], e + k * kSmallThreads);
+    }
+  };
+  each(p.B, [&](int row, int j) { return j < pages_of(s_len[row]) ? p.table[row * ppr + j] : 0; },
+       [&](int row, int j, int id, int) {
+         if (j >= pages_of(s_len[row])) return;
+         if (id < 1 || id > p.cap) ok = false;
+         else atomicOr(&word[id], kHeld);
+       });
+  auto of_source = [&](int row, int j) { return j < pages_of(s_n[row]) ? p.table[s_src[row] * ppr + j] : 0; };
+  each(p.R, of_source, [&](int row, int j, int id, int) {
+    if (j >= pages_of(s_n[row])) return;
+    if (id < 1 || id > p.cap) {
+      ok = false;
+      return;
+    }
+    const bool end = (j + 1) * kPage > s_n[row];
+    atomicAdd(&word[id], end ? kEnds + 1 : 1u);
+    if (end) atomicMax(&begun[id], static_cast<uint32_t>(p.R - row));
+  });
+  if (!ok) atomicOr(&s_bad, 1u);
+  __syncthreads();
+  const bool bad = s_bad != 0;
+
+  int last = 0;  // the page that the row goes on writing, where it is not its own
+  if (!bad && n % kPage != 0) {
+    last = p.table[src * ppr + n / kPage];
+    const uint32_t w = word[last];
+    if ((w & kCount) == ((w & ~kHeld) / kEnds) && static_cast<int>(begun[last]) == p.R - tid) last = 0;
+  }
+  int copies, left;
+  const int rank = block_scan<kSmallThreads>(last != 0, s_wave, copies);
+  s_copy[tid] = last != 0 ? rank : -1;
+  const int each_pages = p.cap / kSmallThreads + 1;
+  const int id0 = tid * each_pages, id1 = id0 + each_pages <= p.cap + 1 ? id0 + each_pages : p.cap + 1;
+  int mine = 0;
+  for (int id = id0; id < id1; ++id) mine += is_left(word[id]);
+  int to = block_scan<kSmallThreads>(mine, s_wave, left);
+  int fail = bad ? FADE_SLOTS_BAD_COUNT : 0;
+  if (head < 0 || head >= p.cap || count < 0 || count > p.cap - left) fail |= FADE_SLOTS_BAD_COUNT;
+  else if (copies > count) fail |= FADE_SLOTS_EXHAUSTED;
+  if (tid == 0) p.status[0] = fail;
+  if (fail) {  // nothing changes
+    for (int e = tid; e < p.R * ppr; e += kSmallThreads) p.table_out[e] = e < p.B * ppr ? p.table[e] : 0;
+    if (tid < p.R) {
+      p.lens_out[tid] = tid < p.B ? p.lens[tid] : 0;
+      p.copies[3 * tid] = p.copies[3 * tid + 1] = p.copies[3 * tid + 2] = 0;
+    }
+    if (tid < 2) p.ring_out[tid] = p.ring[tid];
+    return;
+  }
+  const uint32_t cap = static_cast<uint32_t>(p.cap);
+  auto place = [&](int i) { return (static_cast<uint32_t>(head) + static_cast<uint32_t>(i)) % cap; };
+  each(p.R, of_source, [&](int row, int j, int id, int e) {
+    const int c = s_copy[row];
+    p.table_out[e] = c >= 0 && j == s_n[row] / kPage ? p.free_pages[place(c)] : id;
+  });
+  if (tid < p.R) {
+    p.lens_out[tid] = n;
+    p.copies[3 * tid] = last;
+    p.copies[3 * tid + 1] = last != 0 ? p.free_pages[place(rank)] : 0;
+    p.copies[3 * tid + 2] = last != 0 ? n % kPage : 0;
+  }
+  if (tid == 0) {
+    p.ring_out[0] = static_cast<int32_t>(place(copies));
+    p.ring_out[1] = count - copies + left;
+  }
+  if (mine != 0)
+    for (int id = id0; id < id1; ++id)
+      if (is_left(word[id])) p.free_pages[place(count + to++)] = id;
+}
+
+bool is_small(const fade_page_fork_args* a) {
+  return a->B <= kSmallRows && a->R <= kSmallRows && a->n_free <= kSmallPages && (a->B + a->R) * a->pages_per_row <= kSmallEntries;
+}
+
 int64_t words_of(int64_t cap) { return 2 * (cap + 1) + cap / kSegment + 1 + 2; }
 
 int check_args(const fade_page_fork_args* a) {
@@ -278,7 +405,7 @@ FADE_API int fade_page_fork_workspace_bytes(const fade_page_fork_args* a, int64_
   if (bytes == nullptr) return einval("fade_page_fork_workspace_bytes: null output");
   const int rc = fade::fork::check_args(a);
   if (rc) return rc;
-  *bytes = 4 * fade::fork::words_of(a->n_free);
+  *bytes = fade::fork::is_small(a) ? 0 : 4 * fade::fork::words_of(a->n_free);
   return FADE_OK;
 }
 
@@ -286,10 +413,11 @@ FADE_API int fade_page_fork(const fade_page_fork_args* a, void* workspace, int64
   using namespace fade::fork;
   int rc = check_args(a);
   if (rc) return rc;
-  const int64_t words = words_of(a->n_free);
-  if (workspace == nullptr || workspace_bytes < 4 * words || (reinterpret_cast<uintptr_t>(workspace) & 15))
+  const bool small = is_small(a);
+  const int64_t words = small ? 0 : words_of(a->n_free);
+  if (!small && (workspace == nullptr || workspace_bytes < 4 * words || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return einval("fade_page_fork: needs a 16-byte aligned workspace of %lld bytes", (long long)(4 * words));
-  Params p;
+  Params p{};
   p.B = static_cast<int>(a->B);
   p.R = static_cast<int>(a->R);
   p.ppr = static_cast<int>(a->pages_per_row);
@@ -305,11 +433,15 @@ FADE_API int fade_page_fork(const fade_page_fork_args* a, void* workspace, int64
   p.copies = a->copies;
   p.ring_out = a->ring_out;
   p.status = a->status;
+  hipStream_t st = as_stream(stream);
+  if (small) {
+    hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kSmallThreads), 0, st, p);
+    return check_launch("fade_page_fork");
+  }
   p.word = static_cast<uint32_t*>(workspace);
   p.first = p.word + p.cap + 1;
   p.left = p.first + p.cap + 1;
   p.bad = p.left + p.cap / kSegment + 1;
-  hipStream_t st = as_stream(stream);
   const int64_t most = 2 * static_cast<int64_t>(num_cus());
   auto blocks = [&](int64_t n) { return dim3(static_cast<unsigned>(n < 1 ? 1 : (n > most ? most : n))); };
   const int64_t spans = cdiv(p.ppr, kThreads);

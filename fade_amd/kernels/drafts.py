@@ -41,11 +41,6 @@ class DraftTree:
         return self
 
 
-def _vector(op: str, name: str, t: Tensor, size: int, dtype: torch.dtype = torch.int32) -> None:
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
-        raise ValueError(f"{op}: {name} must be a contiguous {dtype} [{size}], got {t.dtype} {list(t.shape)}")
-
-
 def draft_tree(parents: Tensor, lens: Tensor, starts: Tensor, max_nodes: int) -> DraftTree:
     """Masks, depths and positions of each row's drafted tokens, in one launch.
 
@@ -61,17 +56,17 @@ def draft_tree(parents: Tensor, lens: Tensor, starts: Tensor, max_nodes: int) ->
     if max_nodes < 1 or max_nodes > _lib.DRAFT_MAX_NODES:
         raise ValueError(f"{op}: max_nodes must be 1 to {_lib.DRAFT_MAX_NODES}, got {max_nodes}")
     T, B = parents.numel(), lens.numel()
-    _vector(op, "parents", parents, T)
-    _vector(op, "lens", lens, B)
-    _vector(op, "starts", starts, B + 1)
+    for name, t, size in (("parents", parents, T), ("lens", lens, B), ("starts", starts, B + 1)):
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of {size} elements, got {t.dtype} {list(t.shape)}")
     sizes = (T * words, T, T, B)
-    buf = parents.new_empty(sum(sizes))
-    parts = buf.split_with_sizes(sizes)
+    buf = parents.new_empty(sum(sizes))  # (one allocation)
+    bits, depth, positions, status = buf.split_with_sizes(sizes)
     at = buf.data_ptr()
     a = _lib.DraftTreeArgs(B, T, words, parents.data_ptr(), lens.data_ptr(), starts.data_ptr(), at, at + 4 * T * words,
                            at + 4 * T * (words + 1), at + 4 * T * (words + 2))
     _lib.launch("fade_draft_tree", a, parents.device)
-    return DraftTree(parts[0].view(T, words), parts[1], parts[2], parts[3])
+    return DraftTree(bits.view(T, words), depth, positions, status)
 
 
 @dataclass
@@ -132,25 +127,22 @@ def verify_drafts(
     for name, t in (("target", target), ("draft", draft)):
         if t is not None and ((t.stride(1) != 1 and V > 1) or t.is_neg()):
             raise ValueError(f"{op}: {name} needs a contiguous vocabulary axis (make a copy)")
-    B = final.numel()
-    if tokens.dtype not in (torch.int64, torch.int32):
+    B, M, i32 = final.numel(), int(max_path), torch.int32
+    if tokens.dtype not in (torch.int64, i32):
         raise ValueError(f"{op}: tokens must be int64 or int32, got {tokens.dtype}")
-    _vector(op, "tokens", tokens, T, tokens.dtype)
-    _vector(op, "parents", parents, T)
-    _vector(op, "starts", starts, B + 1)
-    _vector(op, "uniforms", uniforms, T, torch.float32)
-    _vector(op, "final", final, B, torch.float32)
-    M = int(max_path)
+    for name, t, size, dtype in (("tokens", tokens, T, tokens.dtype), ("parents", parents, T, i32), ("starts", starts, B + 1, i32),
+                                 ("uniforms", uniforms, T, torch.float32), ("final", final, B, torch.float32)):
+        if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be a contiguous {dtype} [{size}], got {t.dtype} {list(t.shape)}")
     if not 1 <= M <= _lib.DRAFT_MAX_NODES:
         raise ValueError(f"{op}: max_path must be 1 to {_lib.DRAFT_MAX_NODES}, got {max_path}")
-    path, counts = starts.new_empty(B * (M + 1)).split_with_sizes((B * M, B))
-    out, nxt = tokens.new_empty(B * (M + 1)).split_with_sizes((B * M, B))
+    r = VerifiedDrafts(starts.new_empty((B, M)), starts.new_empty(B), tokens.new_empty((B, M)), tokens.new_empty(B))
     a = _lib.VerifyArgs(B, T, V, M, target.data_ptr(), target.stride(0), _lib.ptr(draft), 0 if draft is None else draft.stride(0),
                         tokens.data_ptr(), parents.data_ptr(), starts.data_ptr(), uniforms.data_ptr(), final.data_ptr(),
-                        path.data_ptr(), counts.data_ptr(), out.data_ptr(), nxt.data_ptr(), _lib.DTYPE_CODES[target.dtype],
+                        r.path.data_ptr(), r.counts.data_ptr(), r.tokens.data_ptr(), r.next.data_ptr(), _lib.DTYPE_CODES[target.dtype],
                         int(tokens.dtype is torch.int64))
     _lib.launch_with_workspace("fade_verify_drafts", a, target.device)
-    return VerifiedDrafts(path.view(B, M), counts, out.view(B, M), nxt)
+    return r
 
 
 __all__ = ["DraftTree", "VerifiedDrafts", "draft_tree", "verify_drafts"]

@@ -120,18 +120,12 @@ def _layers(layers: PageLayers | Sequence[Tensor]) -> PageLayers:
     return layers if isinstance(layers, PageLayers) else PageLayers(layers)
 
 
-def _move_args(layers: PageLayers) -> _lib.PagedMoveArgs:
-    a = _lib.PagedMoveArgs()
-    a.n_pools, a.n_pages, a.Hkv, a.D, a.pools = len(layers.pages), layers.n_pages, layers.n_kv_heads, layers.head_dim, layers.pointers
-    return a
-
-
-def _counts(op: str, device: torch.device, **tensors: tuple[Tensor, tuple]) -> None:
-    for name, (t, shape) in tensors.items():
-        if t.dtype is not torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+def _counts(op: str, layers: PageLayers, shapes: tuple, tensors: dict[str, Tensor]) -> None:
+    for (name, t), shape in zip(tensors.items(), shapes):
+        if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of shape {list(shape)}, got {t.dtype} {list(t.shape)}")
-        if t.device != device:
-            raise ValueError(f"{op}: {name} is on {t.device}, the pages on {device}")
+    _lib.require_gpu(layers.pages[0], *tensors.values(), op=op)
+    layers.about_to_write(op, tensors)
 
 
 def paged_copy(copies: Tensor, layers: PageLayers | Sequence[Tensor]) -> None:
@@ -143,11 +137,8 @@ def paged_copy(copies: Tensor, layers: PageLayers | Sequence[Tensor]) -> None:
     keeps.  Copies from or to pages outside the pool (page 0 included) are not made."""
     op = "paged_copy"
     layers = _layers(layers)
-    _lib.require_gpu(copies, op=op)
-    _counts(op, layers.device, copies=(copies, (copies.shape[0] if copies.dim() else 0, 3)))
-    layers.written(op, copies=copies)
-    a = _move_args(layers)
-    a.rows, a.copies = copies.shape[0], copies.data_ptr()
+    _counts(op, layers, ((copies.shape[0] if copies.dim() else 0, 3),), dict(copies=copies))
+    a = _lib.PagedMoveArgs(len(layers.pages), layers.n_pages, layers.n_kv_heads, layers.head_dim, layers.pointers, copies.shape[0], copies.data_ptr())
     _lib.launch("fade_paged_copy", a, layers.device)
 
 
@@ -171,16 +162,14 @@ def paged_compact(
     ``layers``: the pages of all layers, or better the ``PageLayers`` of them."""
     op = "paged_compact"
     layers = _layers(layers)
-    _lib.require_gpu(path, counts, table, lens, starts, op=op)
     if table.dim() != 2 or path.dim() != 2:
         raise ValueError(f"{op}: table must be [B, pages_per_row] and path [B, max_path], got {tuple(table.shape)} and {tuple(path.shape)}")
-    B, ppr = table.shape
-    _counts(op, layers.device, path=(path, (B, path.shape[1])), counts=(counts, (B,)), table=(table, (B, ppr)), lens=(lens, (B,)), starts=(starts, (B + 1,)))
-    layers.written(op, path=path, counts=counts, table=table, lens=lens, starts=starts)
+    (B, ppr), M = table.shape, path.shape[1]
+    tensors = dict(path=path, counts=counts, table=table, lens=lens, starts=starts)
+    _counts(op, layers, ((B, M), (B,), (B, ppr), (B,), (B + 1,)), tensors)
     kept = torch.empty_like(lens)
-    a = _move_args(layers)
-    a.rows, a.max_path, a.pages_per_row = B, path.shape[1], ppr
-    a.path, a.counts, a.table, a.lens, a.starts, a.kept = (t.data_ptr() for t in (path, counts, table, lens, starts, kept))
+    a = _lib.PagedMoveArgs(len(layers.pages), layers.n_pages, layers.n_kv_heads, layers.head_dim, layers.pointers, B, None, M, ppr,
+                           path.data_ptr(), counts.data_ptr(), table.data_ptr(), lens.data_ptr(), starts.data_ptr(), kept.data_ptr())
     _lib.launch("fade_paged_compact", a, layers.device)
     return kept
 

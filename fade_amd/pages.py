@@ -29,7 +29,9 @@ read of it in stream order.
 
 from __future__ import annotations
 
+import bisect
 import ctypes
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -38,6 +40,7 @@ from torch import Tensor
 from . import _lib
 
 PAGE_TOKENS = 64
+_REQUIRES_GRAD = operator.attrgetter("requires_grad")
 
 
 class MiddlePagePool:
@@ -311,17 +314,15 @@ def page_fork(
         if t is not None and (t.dtype is not torch.int32 or t.numel() != size or not t.is_contiguous() or (t.dim() != 1 and t is not table)):
             raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of {size} elements, got {t.dtype} {list(t.shape)}")
     sizes = (R * ppr, R, 3 * R, 2, 1)
-    buf = table.new_empty(sum(sizes))
-    parts = buf.split_with_sizes(sizes)
-    ptrs, at = [], buf.data_ptr()
-    for size in sizes:
-        ptrs.append(at)
-        at += 4 * size
+    buf = table.new_empty(sum(sizes))  # (one allocation)
+    out, lens_out, copies, ring_out, status = buf.split_with_sizes(sizes)
+    at = buf.data_ptr()
+    lens_at = at + 4 * R * ppr
     _lib.written(op, free)
-    a = _lib.PageForkArgs(B, R, ppr, free.numel(), lens.data_ptr(), _lib.ptr(source), _lib.ptr(keep), table.data_ptr(), free.data_ptr(),
-                          ring.data_ptr(), *ptrs)
+    a = _lib.PageForkArgs(B, R, ppr, free.numel(), lens.data_ptr(), _lib.ptr(source), _lib.ptr(keep), table.data_ptr(), free.data_ptr(), ring.data_ptr(),
+                          at, lens_at, lens_at + 4 * R, lens_at + 16 * R, lens_at + 16 * R + 8)
     _lib.launch_with_workspace("fade_page_fork", a, table.device)
-    return PageFork(parts[0].view(R, ppr), parts[1], parts[2].view(R, 3), parts[3], parts[4])
+    return PageFork(out.view(R, ppr), lens_out, copies.view(R, 3), ring_out, status)
 
 
 class PageLayers:
@@ -343,23 +344,30 @@ class PageLayers:
             if not t.is_contiguous() or t.is_neg() or t.data_ptr() % 16:
                 raise ValueError(f"{op}: pages must be contiguous and 16-byte aligned")
         _lib.require_gpu(*self.pages, op=op)
-        at = sorted(t.data_ptr() for t in self.pages)
-        if any(y - x < first.nbytes for x, y in zip(at, at[1:])):
+        self._starts = sorted(t.data_ptr() for t in self.pages)
+        self._bytes = first.nbytes
+        if any(y - x < self._bytes for x, y in zip(self._starts, self._starts[1:])):
             raise ValueError(f"{op}: pages overlap in memory")
+        self._inference = any(t.is_inference() for t in self.pages)
         self.device = first.device
         self.n_pages, self.n_kv_heads, self.head_dim = int(first.shape[0]), int(first.shape[1]), int(first.shape[3])
         self._pointers = (ctypes.c_void_p * len(self.pages))(*(t.data_ptr() for t in self.pages))
         self.pointers = ctypes.addressof(self._pointers)
 
-    def written(self, op: str, **read: Tensor) -> None:
-        """What a kernel that is about to write the pages looks at first: gradients, and ``read``'s memory."""
-        _lib.no_gradient(op, *self.pages)
-        first = self.pages[0]
+    def about_to_write(self, op: str, read: dict[str, Tensor]) -> None:
+        """Before a kernel writes the pages: refuses gradients, and the memory of what it reads beside them."""
+        pages = self.pages
+        if torch.autograd.forward_ad._current_level >= 0 or True in map(_REQUIRES_GRAD, pages):
+            _lib.no_gradient(op, *pages)
         for name, t in read.items():
-            at, end = t.data_ptr(), t.data_ptr() + t.nbytes
-            if t.numel() and any(x.data_ptr() < end and at < x.data_ptr() + first.nbytes for x in self.pages):
+            at = t.data_ptr()
+            i = bisect.bisect_left(self._starts, at + t.nbytes)
+            if i and self._starts[i - 1] + self._bytes > at and t.numel():
                 raise ValueError(f"{op}: {name} lies in the pages' memory")
-        _lib.written(op, *self.pages)
+        if self._inference:
+            _lib.written(op, *pages)
+        else:
+            torch.autograd.graph.increment_version(pages)
 
 
 class TokenPagePool:

@@ -627,6 +627,8 @@ typedef struct fade_verify_args {
   void* next;             /* tokens' type */
   int32_t dtype;          /* FADE_DTYPE_F16, BF16 or F32: target and draft */
   int32_t tok64;
+  int32_t polls;          /* bound of the workgroups' wait for one another's sums (0: the library's own, below 0: none);
+                             what is not there then is summed anew, to the same results */
 } fade_verify_args;
 /* The workspace (16-byte aligned, contents arbitrary) must not be shared by calls that may overlap. */
 int fade_verify_workspace_bytes(const fade_verify_args* args, int64_t* bytes);

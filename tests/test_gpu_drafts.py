@@ -10,6 +10,7 @@ import random
 import pytest
 import torch
 
+from fade_amd import _lib
 from fade_amd.kernels import PagedAttentionPlan, draft_tree, paged_attention, verify_drafts
 from fade_amd.pages import PAGE_TOKENS
 from test_gpu_paged import _check, _i32, _pages, _starts
@@ -466,6 +467,33 @@ def test_verify_keeps_the_targets_distribution(dev, with_draft):
     # six deviations of a share of B drawings
     assert bool(((share - p.double()).abs() <= 6 * (p * (1 - p) / B).sqrt().double()).all()), share.tolist()
     assert 0.2 < float((got.counts == 2).double().mean()) < 0.99
+
+
+@pytest.mark.parametrize("wait", [True, False])
+@pytest.mark.parametrize("with_draft", [True, False])
+@pytest.mark.parametrize("rows,V", [([15], 70000), ([15, 3, 0, 9], 50000), ([12] * 40, 40011), ([12] * 3, 9000)])
+def test_verify_many_refusals(dev, monkeypatch, rows, V, with_draft, wait):
+    """Stars, whose children are all refused or nearly so: more sums than a row's workgroups share, with and without
+    their wait for one another."""
+    if not wait:
+        launch = _lib.launch_with_workspace
+
+        def without(name, args, device):
+            args.polls = -1
+            launch(name, args, device)
+
+        monkeypatch.setattr(_lib, "launch_with_workspace", without)
+    rng = random.Random(V)
+    torch.manual_seed(V)
+    g = torch.Generator(device=dev).manual_seed(V)
+    trees = [[-1] + [0] * (n - 1) if n else [] for n in rows]
+    target, draft = _probs(g, dev, sum(rows), V, F32, peak=1.0)
+    tokens = _drafted(rng, draft, trees, dup=0.2)
+    for u in (0.9999, 0.97):
+        _verified(dev, target, draft if with_draft else None, tokens, trees, [u] * len(tokens), [rng.random() for _ in rows], 4)
+    # nothing left after the refusals: drawn from the target itself
+    same = target[:1].expand(sum(rows), V)
+    _verified(dev, same, same if with_draft else None, tokens, trees, [0.9999] * len(tokens), [rng.random() for _ in rows], 4)
 
 
 def test_verify_rows_far_apart(dev):
