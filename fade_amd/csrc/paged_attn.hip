@@ -50,6 +50,7 @@ typedef __attribute__((address_space(4))) int32_t const_i32;
 constexpr int kThreads = 256;
 constexpr int kPage = 64;
 constexpr int kRows = 16;  // matrix rows of an item of the few-row kernel
+constexpr int kWideLog = 8;  // log2 of those of a tile of the wide kernel
 constexpr float kNegBig = -3.402823466e38f;  // no score is lower
 
 template <int V>
@@ -1141,9 +1142,8 @@ template <int DP>
 struct Wide {  // waves, matrix rows, keys per step, steps' buffers
   static constexpr int NW = 8, M = 32 * NW, KT = DP > 128 ? 32 : 64, NST = DP > 128 ? 4 : 3;
 };
-constexpr int kWideLog = 8;
 
-// The two kernels' cuts of a call.
+// The two kernels' cuts of a call; no pieces: the kernel is not needed.
 struct Plan {
   Params few, wide;
   bool both;  // the wide kernel runs too
@@ -1239,6 +1239,16 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   pl.few = pl.wide = p;
   set_cut(pl.few, step ? kAll : kFew, 4, 32, static_cast<int64_t>(per_cu) * num_cus(), 64, 0);
   set_cut(pl.wide, kMany, kWideLog, 300, num_cus(), 256, 256);
+  if (tree && pl.both) {
+    // Rows of drafted tokens seldom fit 16 matrix rows, and one that does is read by the wide kernel nearly as fast (16
+    // rows over 8192 keys 113 us and 104.5): the few-row kernel's launch, which would find nothing in most
+    // steps, is spared (16 trees of 16 tokens over 8192 keys 114.5 us, now 110.5).  Pieces from 128 keys on, borders moved
+    // by up to as many: eight tokens of one row over 1000 keys 17.5 us, now 13 (from 256 on 18, from 64 on 12.5,
+    // but 16 tokens over 1000 keys of 32 heads 17.8 instead of 17.2); 32 rows of eight over up to 2000 keys 42 and 38.5.
+    set_cut(pl.wide, kAll, kWideLog, 300, num_cus(), 128, 128);
+    pl.few.pieces = 0;
+    return FADE_OK;
+  }
   pl.wide.zero_tail = 0;
   return FADE_OK;
 }
@@ -1259,10 +1269,14 @@ int launch(const Plan& pl, hipStream_t st) {
     const int rc = check_launch("fade_paged_attn");
     if (rc) return rc;
   }
-  hipLaunchKernelGGL((paged_few_kernel<DP, BF, TREE>), dim3(static_cast<unsigned>(pl.few.Hkv * pl.few.pieces)), dim3(64), 0, st, pl.few);
-  const int rc = check_launch("fade_paged_attn");
+  int rc = FADE_OK;
+  if (!TREE || pl.few.pieces > 0) {
+    hipLaunchKernelGGL((paged_few_kernel<DP, BF, TREE>), dim3(static_cast<unsigned>(pl.few.Hkv * pl.few.pieces)), dim3(64), 0, st, pl.few);
+    rc = check_launch("fade_paged_attn");
+  }
   // (the last piece's tiles end in it)
-  const int wide = pl.both ? pl.wide.Hkv * (pl.wide.pieces - 1) * kWideBlocks : 0, few = pl.few.Hkv * (pl.few.pieces - 1) * kFewBlocks;
+  const int wide = pl.both ? pl.wide.Hkv * (pl.wide.pieces - 1) * kWideBlocks : 0;
+  const int few = pl.few.pieces > 1 ? pl.few.Hkv * (pl.few.pieces - 1) * kFewBlocks : 0;
   if (rc || wide + few == 0) return rc;
   hipLaunchKernelGGL((paged_merge_kernel<BF>), dim3(static_cast<unsigned>(wide + few)), dim3(kThreads), 0, st, pl.wide, pl.few, wide);
   return check_launch("fade_paged_attn (merge)");

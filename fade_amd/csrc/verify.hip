@@ -302,6 +302,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(fade_verify_args a, Sh
 
   enum { kWalk, kEnd, kEndAgain, kNarrow };  // what the next sum is for
   int phase = kWalk, round = 0, item = 0, i0 = 0, i1 = 0;
+  int polls = sh.polls;  // (of all rounds)
   double before = 0.0, t = 0.0;
   Rest<E> r;
   r.V = V;
@@ -409,9 +410,9 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(fade_verify_args a, Sh
         }
         if (static_cast<int>(threadIdx.x) < parts && static_cast<int>(threadIdx.x) != part) {
           uint64_t v;
-          for (int left = sh.polls;;) {
+          for (;;) {
             v = __hip_atomic_load(slots + threadIdx.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            if ((v & kMark) != 0 || --left < 0) break;
+            if ((v & kMark) != 0 || --polls < 0) break;
             __builtin_amdgcn_s_sleep(1);
           }
           part_sums[threadIdx.x] = (v & kMark) != 0 ? __builtin_bit_cast(double, v & ~kMark) : -1.0;

@@ -118,7 +118,7 @@ def verify_drafts(
     unspecified token; where the target has none above zero, ``next`` is -1."""
     op = "verify_drafts"
     _lib.require_gpu(target, tokens, parents, starts, uniforms, final, draft, op=op)
-    _lib.no_gradient(op, target, draft)
+    _lib.no_gradient(op, target, draft, uniforms, final)
     if target.dim() != 2 or target.dtype not in _lib.DTYPE_CODES or target.shape[1] < 1:
         raise ValueError(f"{op}: target must be [tokens, V] of float32, float16 or bfloat16, got {target.dtype} {tuple(target.shape)}")
     if draft is not None and (draft.shape != target.shape or draft.dtype != target.dtype):

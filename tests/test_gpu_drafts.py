@@ -223,6 +223,30 @@ def test_tree_attention_values_that_are_no_numbers(dev, lens, new, Hq, Hkv, D, d
     assert not at, [(i, float(got[tuple(i)]), float(want[tuple(i)])) for i in at]
 
 
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_tree_attention_strides_tail_and_scale(dev, new):
+    g = torch.Generator(device=dev).manual_seed(new)
+    rng = random.Random(new)
+    lens, Hq, Hkv, D = [500, 1200, 64], 12, 4, 128
+    starts = _starts([new] * 3)
+    k, v, table = _pages(g, dev, lens, Hkv, D, F16)
+    T = starts[-1] + 9
+    qkv = torch.randn(T, Hq + 2 * Hkv, D, generator=g, device=dev).half()
+    q = qkv[:, :Hq]
+    masks = _masks(rng, "tree", [new] * 3)
+    tree = _i32(_words(masks + [-1 & 2**64 - 1] * 9, 2), dev)
+    args, kw = (q, k, v, table, _i32(lens, dev), _i32(starts, dev)), dict(mask="tree", tree=tree, sm_scale=0.3)
+    want, tol = _reference(q, k, v, table, lens, starts, 0.3, masks)
+    got = paged_attention(*args, **kw)
+    _check(got, want, tol)
+    assert not got[starts[-1] :].any()  # a new tensor: zeros behind the last sequence
+    out = torch.full((Hq, T, D + 8), 7.0, device=dev).half()[:, :, 4 : 4 + D].transpose(0, 1)
+    assert paged_attention(*args, **kw, out=out) is out and torch.equal(out[: starts[-1]], got[: starts[-1]])
+    assert bool((out[starts[-1] :] == 7.0).all())  # the caller's: left as they were
+    mine = q.clone()
+    assert torch.equal(paged_attention(mine, *args[1:], **kw, out=mine)[: starts[-1]], got[: starts[-1]])
+
+
 def test_tree_attention_device_data_out_of_range(dev):
     """Fewer tokens than new ones, lengths and starts that cannot be: kept inside the tensors."""
     H, D = 2, 64
@@ -553,7 +577,8 @@ def test_verify_refusals(dev):
     for bad in (dict(target=f(6, 50).double()), dict(target=f(6, 50).long()), dict(target=f(300)), dict(target=f(50, 6).t()), dict(target=f(5, 50)), dict(draft=f(6, 49)),
                 dict(draft=f(6, 50).half()), dict(draft=f(50, 6).t()), dict(tokens=z(5)), dict(tokens=z(6).short()), dict(tokens=z(2, 3)), dict(parents=z(6).long()),
                 dict(starts=z(4)), dict(uniforms=f(6).double()), dict(uniforms=f(7)), dict(final=f(2).half()), dict(final=f(2, 1)), dict(max_path=0),
-                dict(max_path=1025), dict(target=f(6, 0), draft=f(6, 0)), dict(target=f(6, 50).requires_grad_())):
+                dict(max_path=1025), dict(target=f(6, 0), draft=f(6, 0)), dict(target=f(6, 50).requires_grad_()), dict(draft=f(6, 50).requires_grad_()),
+                dict(uniforms=f(6).requires_grad_())):
         with pytest.raises(ValueError):
             verify_drafts(**{**ok, **bad})
     with pytest.raises(RuntimeError, match="no CPU fallback"):
