@@ -74,8 +74,6 @@ struct Params {
   const int32_t* starts;
   float scale_log2;
   int causal;
-  const uint32_t* tree;  // [T][words]: the row's new tokens that each one sees, as bits
-  int words;
   int zero_tail;
   // the cut of one kernel's work
   int rows_of;     // kAll, or the rows of the batch whose matrix rows fit one tile of 16 (kFew) or do not (kMany)
@@ -90,6 +88,8 @@ struct Params {
   float2* part_ml; // [workgroup][2][M]: maximum (log2 units, less what its kernel holds probabilities larger by), sum
   int4* cuts;      // [workgroup]: the tile that begins in its piece and ends in another: first new token, its
                    // first matrix row, matrix rows of the row, parts (0: none)
+  const uint32_t* tree;  // [T][words]: the row's new tokens that each one sees, as bits
+  int words;
 };
 
 // A tile (wave-uniform).
@@ -725,10 +725,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   // (at head_dim over 128 no register is left to keep them: spilled, their reloads would wait for the loads in flight)
   constexpr bool kKeep = DP <= 128;
   uint32_t ko[kKeep ? LPW : 1], vo[kKeep ? LPW : 1];
-  bool kin[kKeep ? LPW : 1], vin[kKeep ? LPW : 1];
   if constexpr (kKeep) {
 #pragma unroll
-    for (int i = 0; i < LPW; ++i) place(i, lane, ko[i], vo[i], kin[i], vin[i]);
+    for (int i = 0; i < LPW; ++i) {
+      bool k_in, v_in;
+      place(i, lane, ko[i], vo[i], k_in, v_in);
+    }
   }
   // where this lane reads: K row n32 (+ 32), unit 2 ks + h; V row 4 h + (l16 >> 2) (+ 16 ks, + 8), channels
   // 32 cb + 16 ((lane >> 4) & 1) + 4 (l16 & 3), l16 = lane & 15.  Units are exchanged by an exclusive or within
@@ -739,6 +741,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int vrow = 4 * h + ((lane & 15) >> 2);
   uint32_t kat = base + n32 * DP * 2 + 16 * wide_k_unit<DP>(n32, h);
   uint32_t vat = base + TENSOR + vrow * DP * 2 + 16 * wide_v_unit<DP>(vrow, 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
+  // What a step's loads take of the arguments, in registers of its own: kept in the tuples that the arguments are
+  // loaded into, a spilled tuple is read back as a whole at each load (eighteen instructions).
+  const uint64_t head_at = 2 * static_cast<uint64_t>(kvh) * kPage * D;
+  uint64_t k_head = reinterpret_cast<uint64_t>(p.kp) + head_at, v_head = reinterpret_cast<uint64_t>(p.vp) + head_at;
+  uint64_t page_bytes = 2 * static_cast<uint64_t>(p.Hkv) * kPage * D;
+  uint32_t n_pages = static_cast<uint32_t>(p.n_pages);
+  asm volatile("" : "+s"(k_head), "+s"(v_head), "+s"(page_bytes), "+s"(n_pages));
   int buf = 0;
   auto flip = [&]() {  // the next buffer
     const uint32_t d = buf == NST - 1 ? -static_cast<uint32_t>((NST - 1) * STAGE) : STAGE;
@@ -771,26 +780,37 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int whi = __builtin_amdgcn_readfirstlane(active ? limit((rl - 1) / p.G) : 0);
     const const_i32* trow = (const const_i32*)(uintptr_t)(p.table + w.b * p.ppr);  // (scalar loads: vmcnt counts the steps' alone)
     auto issue = [&](int key, int id, int buf) {
-      id = id < 0 || id >= p.n_pages ? 0 : id;
-      const int64_t at = ((static_cast<int64_t>(id) * p.Hkv + kvh) * kPage + key % kPage) * D;
+      const uint64_t at = (static_cast<uint32_t>(id) < n_pages ? static_cast<uint32_t>(id) : 0u) * page_bytes + 2 * (key & (kPage - 1)) * D;
+      const void* const kat = reinterpret_cast<const void*>(k_head + at);
+      const void* const vat = reinterpret_cast<const void*>(v_head + at);
       const uint32_t to = base + buf * STAGE + 1024 * LPW * wave;
-      if constexpr (kKeep) {
-#pragma unroll
-        for (int i = 0; i < LPW; ++i) {
-          if (kin[i]) lds_dma16(p.kp + at, ko[i], to + 1024 * i);
-          if (vin[i]) lds_dma16(p.vp + at, vo[i], to + TENSOR + 1024 * i);
-        }
-      } else {
-        int l = threadIdx.x & 63;
-        asm volatile("" : "+v"(l));  // (not computed ahead of the loop)
+      if (DP == D) {  // (no lane is left out)
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
           uint32_t k_off, v_off;
           bool k_in, v_in;
-          place(i, l, k_off, v_off, k_in, v_in);
-          if (k_in) lds_dma16(p.kp + at, k_off, to + 1024 * i);
-          if (v_in) lds_dma16(p.vp + at, v_off, to + TENSOR + 1024 * i);
+          if constexpr (kKeep) {
+            k_off = ko[i];
+            v_off = vo[i];
+          } else {
+            int l = threadIdx.x & 63;
+            asm volatile("" : "+v"(l));  // (not computed ahead of the loop)
+            place(i, l, k_off, v_off, k_in, v_in);
+          }
+          lds_dma16(kat, k_off, to + 1024 * i);
+          lds_dma16(vat, v_off, to + TENSOR + 1024 * i);
         }
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < LPW; ++i) {
+        int l = threadIdx.x & 63;
+        asm volatile("" : "+v"(l));
+        uint32_t k_off, v_off;
+        bool k_in, v_in;
+        place(i, l, k_off, v_off, k_in, v_in);
+        if (k_in) lds_dma16(kat, k_off, to + 1024 * i);
+        if (v_in) lds_dma16(vat, v_off, to + TENSOR + 1024 * i);
       }
     };
     const bool live = r0 + n32 < all;
@@ -923,9 +943,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
           for (int st = 0; st < 2 * NKB; ++st)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              pa[st][j] = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j], sl2, nm)),
-                                    __builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j + 1], sl2, nm)));
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w = pack2<BF>(__builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j], sl2, nm)),
+                                     __builtin_amdgcn_exp2f(fmaf(s[st >> 1][8 * (st & 1) + 2 * j + 1], sl2, nm)));
+              asm("" : "+v"(w));  // (else the compiler rounds each half once more for the maximum below)
+              pa[st][j] = w;
+            }
         };
         probs(held(m));
         // 16-bit patterns of the non-negative probabilities order as their values do
