@@ -1209,7 +1209,7 @@ int plan_of(const fade_paged_attn_args* a, Plan& pl) {
   const bool tree = a->mask_mode == FADE_MASK_TREE;
   if (a->mask_mode != FADE_MASK_BOTTOM_RIGHT && a->mask_mode != FADE_MASK_NONE && !tree)
     return einval("%s: mask_mode must be FADE_MASK_BOTTOM_RIGHT, FADE_MASK_NONE or FADE_MASK_TREE, got %d", what, a->mask_mode);
-  if (tree && (!a->tree || a->tree_words < 1 || a->tree_words > (1 << 20) || (reinterpret_cast<uintptr_t>(a->tree) & 3)))
+  if (tree && ((!a->tree && a->T > 0) || a->tree_words < 1 || a->tree_words > (1 << 20) || (reinterpret_cast<uintptr_t>(a->tree) & 3)))
     return einval("%s: FADE_MASK_TREE needs tree, 4-byte aligned, with 1 to 2^20 words a token", what);
   if (!(a->sm_scale > 0.0f) || !(a->sm_scale < INFINITY)) return einval("%s: sm_scale must be positive and finite", what);
   Params p{};

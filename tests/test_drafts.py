@@ -30,6 +30,8 @@ def test_tree_attention_arguments():
     for bad in (dict(tree=None), dict(tree=AT + 2), dict(tree_words=0), dict(tree_words=-1), dict(tree_words=1 << 21), dict(mask_mode=4)):
         _refused("fade_paged_attn_workspace_bytes", _args(_lib.PagedAttnArgs, base, **bad), nb)
         _refused("fade_paged_attn", _args(_lib.PagedAttnArgs, base, **bad), None, 0, None)
+    # no tokens: nothing to look at, nothing is launched
+    assert _lib.load().fade_paged_attn(ctypes.byref(_args(_lib.PagedAttnArgs, base, T=0, tree=None)), None, 0, None) == 0
     # the other masks do not look at it
     assert _lib.load().fade_paged_attn_workspace_bytes(ctypes.byref(_args(_lib.PagedAttnArgs, base, mask_mode=0, tree=None, tree_words=0)), nb) == 0
 

@@ -280,6 +280,7 @@ def test_tree_attention_refusals(dev):
             paged_attention(**{**ok, **bad})
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         paged_attention(**{**ok, "tree": ok["tree"].cpu()})
+    assert paged_attention(**{**ok, "q": h(0, 4, 64), "tree": z(0, 1)}).shape == (0, 4, 64)
 
 
 def test_tree_attention_plans_streams_graph(dev):
@@ -532,6 +533,18 @@ def test_verify_rows_far_apart(dev):
     for u in (0.0, 0.9):
         _verified(dev, far, d, tokens, [[-1, 0, 1, 2]], [u] * 4, [0.6], 4)
         _verified(dev, d, far, tokens, [[-1, 0, 1, 2]], [u] * 4, [0.6], 4)
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_verify_more_rows_than_workgroups_at_once(dev, with_draft):
+    """Rows so many that each has one workgroup, whatever the vocabulary."""
+    rng = random.Random(11)
+    g = torch.Generator(device=dev).manual_seed(11)
+    trees = [[-1, 0, 0][: rng.randint(1, 3)] for _ in range(300)]
+    T = sum(map(len, trees))
+    target, draft = _probs(g, dev, T, 40960, BF16)
+    tokens = _drafted(rng, draft, trees)
+    _verified(dev, target, draft if with_draft else None, tokens, trees, [rng.random() for _ in tokens], [rng.random() for _ in trees], 3)
 
 
 def test_verify_graph_streams_and_repeats(dev):

@@ -479,6 +479,47 @@ def test_drafted_steps_in_two_graphs(dev):
     assert int(lens.sum()) > 8 * B
 
 
+@pytest.mark.parametrize("B,ppr,pages", [(6, 5, 60), (200, 100, 30000)])
+def test_fork_in_two_graphs(dev, B, ppr, pages):
+    """Captured in two graphs and replayed in turn, with eager calls between: every replay as the eager call."""
+    rng = random.Random(B)
+    lens, table, free = _i32([0] * B, dev), torch.zeros(B, ppr, dtype=torch.int32, device=dev), _i32([0] * pages, dev)
+    ring, source, keep = _i32([0, 0], dev), _i32([0] * B, dev), _i32([0] * B, dev)
+    call = lambda: page_fork(lens, table, free, ring, source=source, keep=keep)  # noqa: E731
+    call()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    for i in range(6):
+        m = _Model(pages, ppr, head=rng.randrange(pages))
+        m.rows, m.lens = [[] for _ in range(B)], [0] * B
+        m.grow([rng.randint(0, ppr * PAGE_TOKENS // 2) for _ in range(B)])
+        src, kept = [rng.randint(-1, B - 1) for _ in range(B)], [rng.choice((10**6, rng.randint(0, 300))) for _ in range(B)]
+        for dst, x in ((lens, m.lens), (table, m.table()), (free, m.free), (ring, [m.head, m.count]), (source, src), (keep, kept)):
+            dst.copy_(_i32(x, dev))
+        was = free.clone()
+        copies = m.fork(src, kept)
+        graph, out = graphs[i % 2]
+        graph.replay()
+        _same(out, m, copies, free, out.ring)
+        free.copy_(was)
+        got = call()
+        _same(got, m, copies, free, got.ring)
+        torch.cuda.synchronize()
+
+
+def test_moves_in_inference_mode(dev):
+    with torch.inference_mode():
+        layers = PageLayers([torch.randn(4, 2, 64, 16, device=dev).half() for _ in range(2)])
+        paged_copy(_i32([[1, 2, 9]], dev), layers)
+        assert all(torch.equal(x[2, :, :9], x[1, :, :9]) for x in layers.pages)
+    with pytest.raises(RuntimeError, match="inference"):
+        paged_copy(_i32([[1, 2, 9]], dev), layers)
+
+
 def test_off_the_current_device(dev, monkeypatch):
     """Every entry point makes its tensors' GPU the current one for its launch (seen on one GPU by its guard)."""
     pool = TokenPagePool(9, 2, 64, F16, dev)
