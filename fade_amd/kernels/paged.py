@@ -155,7 +155,7 @@ def paged_compact(
     ``page_fork``'s ``keep``).
 
     Row b holds ``lens[b]`` tokens in the pages of ``table`` [B, pages_per_row], its last
-    ``n = starts[b + 1] - starts[b]`` ones drafted.  ``path`` int32 [B, max_path] numbers the
+    ``n = starts[b + 1] - starts[b]`` ones drafted.  ``path`` int32 [B, max_path], max_path up to 1024, numbers the
     ones that stay, rising (``verify_drafts``), ``counts`` [B] how many of them; token
     ``lens - n + path[b, i]`` goes to place ``lens - n + i``.  Numbers outside 0 .. n - 1 move
     nothing.  The drafted tokens' pages must be the row's own, as ``page_fork`` leaves them.

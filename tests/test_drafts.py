@@ -1,10 +1,13 @@
-"""Drafted tokens and branching rows on the CPU: what the C entry points refuse."""
+"""Drafted tokens and branching rows on the CPU: what the C entry points refuse, and how the tree attention's work is
+cut (a model of the device code's sums, in its precision)."""
 
 from __future__ import annotations
 
 import ctypes
+import random
 
 from fade_amd import _lib
+from test_paged import _cut
 
 AT = 1 << 20
 
@@ -34,6 +37,29 @@ def test_tree_attention_arguments():
     assert _lib.load().fade_paged_attn(ctypes.byref(_args(_lib.PagedAttnArgs, base, T=0, tree=None)), None, 0, None) == 0
     # the other masks do not look at it
     assert _lib.load().fade_paged_attn_workspace_bytes(ctypes.byref(_args(_lib.PagedAttnArgs, base, mask_mode=0, tree=None, tree_words=0)), nb) == 0
+
+
+def test_tree_attention_is_cut_into_pieces():
+    """Every tile's keys are walked once and in order, whole or in a beginning and ends of consecutive pieces, none
+    past the last one, which is what the second launch joins."""
+    rng = random.Random(3)
+    for _ in range(150):
+        B, G, most = rng.choice((1, 2, 16, 61, 130)), rng.choice((1, 4, 7, 8)), rng.choice((20, 1000, 32000))
+        lens = [rng.randint(1, most) for _ in range(B)]
+        new = [min(n, rng.randint(0, rng.choice((1, 12, 64, 300)))) for n in lens]
+        pieces, grain = rng.choice((1, 16, 32, 128, 256)), rng.choice((32, 64))
+        tiles, done, cuts = _cut(lens, new, G, 256, False, 300, pieces, 128, grain, 128)
+        by_tile = {}
+        for w, b, t, lo, hi, first, last in done:
+            by_tile.setdefault((b, t), []).append((w, lo, hi, first, last))
+        assert sorted(by_tile) == [(b, t) for b in range(B) for t in range(tiles[b])]
+        for (b, t), parts in by_tile.items():
+            assert parts[0][1] == 0 and parts[0][3] and parts[-1][4] and parts[-1][2] == lens[b]
+            assert [p[0] for p in parts] == list(range(parts[0][0], parts[0][0] + len(parts))) and parts[-1][0] < pieces
+            assert all(p[2] == q[1] for p, q in zip(parts, parts[1:])) and not any(p[3] for p in parts[1:])
+            if len(parts) > 1:
+                assert cuts.pop(parts[0][0]) == len(parts)
+        assert not cuts
 
 
 def test_draft_tree_arguments():
