@@ -72,12 +72,12 @@ __global__ __launch_bounds__(kThreads) void compact_kernel(Pools pools, CompactP
   const int b = blockIdx.x / p.slices, slice = blockIdx.x - b * p.slices;
   int n = p.starts[b + 1] - p.starts[b];
   n = n < 0 ? 0 : n;
-  const int base = p.lens[b] - n, cap = static_cast<int>(p.ppr) * kPage;
+  const int len = p.lens[b] < 0 ? 0 : p.lens[b], base = len - n, cap = static_cast<int>(p.ppr) * kPage;
   int count = p.counts[b];
   count = count < 0 ? 0 : (count > n ? n : count);
   count = count > p.max_path ? static_cast<int>(p.max_path) : count;
   if (p.kept != nullptr && blockIdx.y == 0 && slice == 0 && threadIdx.x == 0) p.kept[b] = base + count < 0 ? 0 : base + count;
-  if (base < 0 || p.lens[b] > cap) return;
+  if (base < 0 || len > cap) return;
   const int columns = p.Hkv * p.units;
   const int32_t* const trow = p.table + b * p.ppr;
   for (int m0 = 0; m0 < count; m0 += kMoves) {

@@ -328,7 +328,8 @@ def page_fork(
 class PageLayers:
     """The pages of several layers, checked once: ``pages``, a sequence of tensors
     [n_pages, Hkv, 64, D] (each layer's K and V), fp16 or bf16, alike and contiguous, each with
-    memory of its own.  Moves within them (``paged_copy``, ``paged_compact``) take all of them in one launch."""
+    memory of its own that stays where it is (no ``resize_`` or ``set_`` of them).  Moves within them
+    (``paged_copy``, ``paged_compact``) take all of them in one launch."""
 
     def __init__(self, pages) -> None:
         op = "PageLayers"

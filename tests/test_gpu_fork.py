@@ -250,6 +250,15 @@ def test_compact_impossible_counts(dev):
     assert args([[2, 3, 4]], [2], [[1, 2]], [70], [5, 0]) == [70] and torch.equal(x, was)
 
 
+def test_compact_lengths_below_zero(dev):
+    """A length below zero, the lowest one included, is an empty row: no place is made from it and nothing moves."""
+    x = torch.randn(6, 2, PAGE_TOKENS, 16, device=dev).half()
+    layers, was = PageLayers([x]), x.clone()
+    for low in (-1, -70, -(2**31) + 3, -(2**31)):
+        kept = paged_compact(_i32([[0, 2], [1, 2]], dev), _i32([2, 2], dev), _i32([[1, 2], [3, 4]], dev), _i32([low, low], dev), _i32([0, 5, 5], dev), layers)
+        assert kept.tolist() == [0, 0] and torch.equal(x, was), low
+
+
 def test_moves_refusals(dev):
     z = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
     h = lambda *s: torch.zeros(s, dtype=F16, device=dev)  # noqa: E731
