@@ -730,14 +730,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     ko = static_cast<uint32_t>(2 * (row * D + 8 * ku));
     vo = static_cast<uint32_t>(2 * (row * D + 8 * vu));
   };
-  // (at head_dim over 128 no register is left to keep them: spilled, their reloads would wait for the loads in flight)
+  // (at head_dim over 128 no register is left to keep them: spilled, their reloads would wait for the loads in flight).
+  // A unit past the head_dim, which is not loaded, has kNone for its place: made anew in every step instead, 16 rows of 16
+  // tokens over 8192 keys at head_dim 80 take 102 us, not 95; kept as lane masks, in scalar registers that the loop
+  // lacks, 98.
   constexpr bool kKeep = DP <= 128;
+  constexpr uint32_t kNone = ~0u;
   uint32_t ko[kKeep ? LPW : 1], vo[kKeep ? LPW : 1];
   if constexpr (kKeep) {
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
       bool k_in, v_in;
       place(i, lane, ko[i], vo[i], k_in, v_in);
+      if (!k_in) ko[i] = kNone;
+      if (!v_in) vo[i] = kNone;
     }
   }
   // where this lane reads: K row n32 (+ 32), unit 2 ks + h; V row 4 h + (l16 >> 2) (+ 16 ks, + 8), channels
@@ -792,31 +798,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       const void* const kat = reinterpret_cast<const void*>(k_head + at);
       const void* const vat = reinterpret_cast<const void*>(v_head + at);
       const uint32_t to = base + buf * STAGE + 1024 * LPW * wave;
-      if (DP == D) {  // (no lane is left out)
+      // Without a mask where no lane is left out; not at head_dim over 128, where the loop's second form costs more (head_dim
+      // 200, 16 rows of 16 tokens over 8192 keys: 190 us, not 187; at 256 alike).
+      if constexpr (kKeep) {
+        if (DP == D) {
 #pragma unroll
-        for (int i = 0; i < LPW; ++i) {
-          uint32_t k_off, v_off;
-          bool k_in, v_in;
-          if constexpr (kKeep) {
-            k_off = ko[i];
-            v_off = vo[i];
-          } else {
-            int l = threadIdx.x & 63;
-            asm volatile("" : "+v"(l));  // (not computed ahead of the loop)
-            place(i, l, k_off, v_off, k_in, v_in);
+          for (int i = 0; i < LPW; ++i) {
+            lds_dma16(kat, ko[i], to + 1024 * i);
+            lds_dma16(vat, vo[i], to + TENSOR + 1024 * i);
           }
-          lds_dma16(kat, k_off, to + 1024 * i);
-          lds_dma16(vat, v_off, to + TENSOR + 1024 * i);
+          return;
         }
-        return;
       }
 #pragma unroll
       for (int i = 0; i < LPW; ++i) {
-        int l = threadIdx.x & 63;
-        asm volatile("" : "+v"(l));
         uint32_t k_off, v_off;
         bool k_in, v_in;
-        place(i, l, k_off, v_off, k_in, v_in);
+        if constexpr (kKeep) {
+          k_off = ko[i];
+          v_off = vo[i];
+          asm volatile("" : "+v"(k_off), "+v"(v_off));  // (the masks are not made ahead of the loop)
+          k_in = k_off != kNone;
+          v_in = v_off != kNone;
+        } else {
+          int l = threadIdx.x & 63;
+          asm volatile("" : "+v"(l));  // (not computed ahead of the loop)
+          place(i, l, k_off, v_off, k_in, v_in);
+        }
         if (k_in) lds_dma16(kat, k_off, to + 1024 * i);
         if (v_in) lds_dma16(vat, v_off, to + TENSOR + 1024 * i);
       }
