@@ -63,7 +63,7 @@ __device__ __forceinline__ float of_lane(float x, int l) { return __uint_as_floa
 // What the tests of a row's tokens need, in LDS.
 struct Nodes {
   int16_t up[kMaxNodes];
-  int32_t tok[kMaxNodes];  // -1: outside the vocabulary
+  int32_t tok[kMaxNodes];  // -1: outside the vocabulary (then up is -1 too)
   float p[kMaxNodes], q[kMaxNodes], u[kMaxNodes];
 };
 
@@ -272,7 +272,9 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(fade_verify_args a, Sh
     else static_cast<int32_t*>(to)[at] = static_cast<int32_t>(x);
   };
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const int up = parent_of(a, row, i), x = token_of(a, row, i);
+    // A token outside the vocabulary was drawn from nothing: it follows none, and so is never tried.  (Refused instead,
+    // it would take draft's share from what is left, and the next token would not be the target's.)
+    const int x = token_of(a, row, i), up = x < 0 ? -1 : parent_of(a, row, i);
     const float2 pq = SHARED ? sh.probs[row.s + i] : probs_of<E>(a, row, up, x);
     nodes.up[i] = static_cast<int16_t>(up);
     nodes.tok[i] = x;

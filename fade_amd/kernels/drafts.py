@@ -112,7 +112,8 @@ def verify_drafts(
 
     Where none is accepted, ``next`` is drawn from what is left: the first token at which the running
     sum passes ``final[b]`` of the sum.  ``uniforms`` [tokens] and ``final`` [B]: fp32 in [0, 1).
-    ``tokens`` int64 or int32 [tokens]; one outside the vocabulary is never accepted.  ``max_path``: the most
+    ``tokens`` int64 or int32 [tokens]; one outside the vocabulary, e.g. the -1 that fills up a tree
+    of a fixed number of tokens, is not tried, and what is left stays as it is.  ``max_path``: the most
     tokens that a path may have, up to 1024, the first included; behind so many no token is tried, nor any past
     a row's first 1024.  Sums are held in 64 bits.  Probabilities that are NaN or not above zero count as zero, infinite ones give an
     unspecified token; where the target has none above zero, ``next`` is -1."""

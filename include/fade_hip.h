@@ -606,7 +606,8 @@ int fade_draft_tree(const fade_draft_tree_args* args, void* stream);
  * nothing is left, left = target; where that has nothing above zero, -1.  Sums in
  * 64 bits.  Probabilities that are not above zero (NaN too) count as 0; infinite ones
  * give an unspecified token.  A path ends at max_path tokens, whose last one's children
- * are not tried; tokens past a row's first FADE_DRAFT_MAX_NODES are not tried either.
+ * are not tried; tokens past a row's first FADE_DRAFT_MAX_NODES are not tried either, nor
+ * tokens outside 0 .. V - 1 (filler of a tree of a fixed size), as if they were not there.
  * Writes path [B][max_path] (numbers in the row, -1 past the end), counts [B] (tokens of
  * the path; 0 for a row without tokens), tokens_out [B][max_path] (the path's tokens
  * after its first, then the next one, -1 past them) and next [B]. */
