@@ -303,6 +303,7 @@ _SIGNATURES: dict[str, list] = {
     "fade_verify_drafts": [ctypes.POINTER(VerifyArgs), _p, _i64, _p],
     "fade_page_fork_workspace_bytes": [ctypes.POINTER(PageForkArgs), _pi64],
     "fade_page_fork": [ctypes.POINTER(PageForkArgs), _p, _i64, _p],
+    "fade_page_fork_after": [ctypes.POINTER(PageForkArgs), _p, _p, _i64, _p],
     "fade_paged_copy": [ctypes.POINTER(PagedMoveArgs), _p],
     "fade_paged_compact": [ctypes.POINTER(PagedMoveArgs), _p],
 }
@@ -359,7 +360,8 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
-_WORKSPACE_OF = {"fade_verify_drafts": "fade_verify_workspace_bytes", "fade_page_fork": "fade_page_fork_workspace_bytes"}
+_WORKSPACE_OF = {"fade_verify_drafts": "fade_verify_workspace_bytes", "fade_page_fork": "fade_page_fork_workspace_bytes",
+                 "fade_page_fork_after": "fade_page_fork_workspace_bytes"}
 _GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
@@ -375,20 +377,21 @@ def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
         check(getattr(load(), name)(ctypes.byref(args), current_stream_handle(device)), name)
 
 
-def launch_with_workspace(name: str, args: ctypes.Structure, device: torch.device) -> None:
-    """``launch`` of an entry point with a workspace, taken for the call and returned with it."""
+def launch_with_workspace(name: str, args: ctypes.Structure, device: torch.device, *more) -> None:
+    """``launch`` of an entry point with a workspace, taken for the call and returned with it.  ``more``: its
+    arguments between the struct and the workspace."""
     if device.index != _GET_DEVICE():
         with torch.cuda.device(device):
-            return launch_with_workspace(name, args, device)
+            return launch_with_workspace(name, args, device, *more)
     lib, a, need = _lib or load(), ctypes.byref(args), ctypes.c_int64(0)
     rc = getattr(lib, _WORKSPACE_OF[name])(a, need)
     if not rc:
         n = need.value
         if n:
             ws = torch.empty(n, dtype=torch.uint8, device=device)
-            rc = getattr(lib, name)(a, ws.data_ptr(), n, current_stream_handle(device))
+            rc = getattr(lib, name)(a, *more, ws.data_ptr(), n, current_stream_handle(device))
         else:
-            rc = getattr(lib, name)(a, None, 0, current_stream_handle(device))
+            rc = getattr(lib, name)(a, *more, None, 0, current_stream_handle(device))
     if rc:
         check(rc, name)
 

@@ -37,6 +37,7 @@ struct Params {
   const int32_t* table;
   int32_t* free_pages;
   const int32_t* ring;
+  const int32_t* before;  // status of an earlier call, or null
   int32_t* table_out;
   int32_t* lens_out;
   int32_t* copies;
@@ -66,6 +67,12 @@ __device__ __forceinline__ bool row_of(const Params& p, int r, int& src, int& n)
 
 __global__ __launch_bounds__(kThreads) void fork_clear_kernel(uint32_t* at, int64_t n) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * kThreads) at[i] = 0;
+}
+
+// The status bits of an earlier call that was not done.
+__device__ __forceinline__ int failed_before(const Params& p) {
+  const int x = p.before != nullptr ? p.before[0] : 0;
+  return ((x | x >> 8) & 0xFF) << 8;
 }
 
 // The words of all pages.
@@ -145,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void fork_write_kernel(Params p) {
   __shared__ int32_t s_wave[kThreads / 64];
   const int tid = threadIdx.x;
   const int head = p.ring[0], count = p.ring[1], left = static_cast<int>(p.bad[1]);
-  int fail = p.bad[0] ? FADE_SLOTS_BAD_COUNT : 0;
+  int fail = (p.bad[0] ? FADE_SLOTS_BAD_COUNT : 0) | failed_before(p);
   int mine = 0;
   uint32_t flags = 0;
   if (!fail) {
@@ -254,7 +261,7 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(Params p) {
   __shared__ int32_t s_wave[kSmallThreads / 64];
   __shared__ uint32_t s_bad;
   const int tid = threadIdx.x, ppr = p.ppr;
-  const int head = p.ring[0], count = p.ring[1];
+  const int head = p.ring[0], count = p.ring[1], before = failed_before(p);
   int len = tid < p.B ? p.lens[tid] : 0;
   int src = tid >= p.R ? -1 : (p.source != nullptr ? p.source[tid] : tid);
   const int keep = p.keep != nullptr && tid < p.R ? p.keep[tid] : 0x7FFFFFFF;
@@ -331,7 +338,7 @@ __global__ __launch_bounds__(kSmallThreads) void fork_small_kernel(Params p) {
   int mine = 0;
   for (int id = id0; id < id1; ++id) mine += is_left(word[id]);
   int to = block_scan<kSmallThreads>(mine, s_wave, left);
-  int fail = bad ? FADE_SLOTS_BAD_COUNT : 0;
+  int fail = (bad ? FADE_SLOTS_BAD_COUNT : 0) | before;
   if (head < 0 || head >= p.cap || count < 0 || count > p.cap - left) fail |= FADE_SLOTS_BAD_COUNT;
   else if (copies > count) fail |= FADE_SLOTS_EXHAUSTED;
   if (tid == 0) p.status[0] = fail;
@@ -371,7 +378,7 @@ bool is_small(const fade_page_fork_args* a) {
 
 int64_t words_of(int64_t cap) { return 2 * (cap + 1) + cap / kSegment + 1 + 2; }
 
-int check_args(const fade_page_fork_args* a) {
+int check_args(const fade_page_fork_args* a, const int32_t* before) {
   const char* what = "fade_page_fork";
   if (a == nullptr) return einval("%s: null args", what);
   if (a->B < 1 || a->B > FADE_SLOTS_MAX_ROWS || a->R < 1 || a->R > FADE_SLOTS_MAX_ROWS)
@@ -391,9 +398,9 @@ int check_args(const fade_page_fork_args* a) {
   const Span spans[] = {{a->table_out, 4 * a->R * a->pages_per_row, "table_out"}, {a->lens_out, 4 * a->R, "lens_out"}, {a->copies, 12 * a->R, "copies"},
                         {a->ring_out, 8, "ring_out"}, {a->status, 4, "status"}, {a->free_pages, 4 * a->n_free, "free_pages"},  // (written so far)
                         {a->lens, 4 * a->B, "lens"}, {a->source, a->source ? 4 * a->R : 0, "source"}, {a->keep, a->keep ? 4 * a->R : 0, "keep"},
-                        {a->ring, 8, "ring"}, {a->table, 4 * a->B * a->pages_per_row, "table"}};
+                        {a->ring, 8, "ring"}, {a->table, 4 * a->B * a->pages_per_row, "table"}, {before, before ? 4 : 0, "before"}};
   for (int i = 0; i < 6; ++i)
-    for (int j = i + 1; j < 11; ++j) {
+    for (int j = i + 1; j < 12; ++j) {
       const uintptr_t x = reinterpret_cast<uintptr_t>(spans[i].at), y = reinterpret_cast<uintptr_t>(spans[j].at);
       if (spans[i].bytes == 0 || spans[j].bytes == 0) continue;
       if (x < y + spans[j].bytes && y < x + spans[i].bytes)
@@ -410,15 +417,19 @@ using namespace fade;
 
 FADE_API int fade_page_fork_workspace_bytes(const fade_page_fork_args* a, int64_t* bytes) {
   if (bytes == nullptr) return einval("fade_page_fork_workspace_bytes: null output");
-  const int rc = fade::fork::check_args(a);
+  const int rc = fade::fork::check_args(a, nullptr);
   if (rc) return rc;
   *bytes = fade::fork::is_small(a) ? 0 : 4 * fade::fork::words_of(a->n_free);
   return FADE_OK;
 }
 
 FADE_API int fade_page_fork(const fade_page_fork_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
+  return fade_page_fork_after(a, nullptr, workspace, workspace_bytes, stream);
+}
+
+FADE_API int fade_page_fork_after(const fade_page_fork_args* a, const int32_t* before, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace fade::fork;
-  int rc = check_args(a);
+  int rc = check_args(a, before);
   if (rc) return rc;
   const bool small = is_small(a);
   const int64_t words = small ? 0 : words_of(a->n_free);
@@ -435,6 +446,7 @@ FADE_API int fade_page_fork(const fade_page_fork_args* a, void* workspace, int64
   p.table = a->table;
   p.free_pages = a->free_pages;
   p.ring = a->ring;
+  p.before = before;
   p.table_out = a->table_out;
   p.lens_out = a->lens_out;
   p.copies = a->copies;

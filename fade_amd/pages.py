@@ -166,6 +166,15 @@ class MiddlePagePool:
         return one(self.k_codes), one(self.v_codes), one(self.v_scale)
 
 
+def _check_status(op: str, texts: dict[int, str], status: Tensor) -> None:
+    word = int(status.item())
+    if word:
+        what = [t for b, t in texts.items() if word & b]
+        # bits 8 to 15: of the call that it was to go on from
+        what += [f"the call before it was not done ({t})" for b, t in _lib.SLOTS_STATUS.items() if word >> 8 & b]
+        raise RuntimeError(f"{op}: {', '.join(what)} (nothing was changed)")
+
+
 @dataclass
 class PageSlots:
     """What ``page_slots`` writes (int32, on the GPU).
@@ -175,7 +184,8 @@ class PageSlots:
     ``slots`` / ``positions`` [n_tokens]: where each new token goes (64 * page + place in
     it) and its position in the row; -1 and 0 past the last one.  ``ring`` [2]: the first
     free page's place and the number of free pages.  ``status`` [1]: 0, or why nothing
-    was done (``check()``)."""
+    was done (``check()``): of the call that made this state alone, but ``TokenPagePool.accept``
+    carries its step's on.  ``by``: the call that made it."""
 
     table: Tensor
     lens: Tensor
@@ -184,13 +194,11 @@ class PageSlots:
     positions: Tensor
     ring: Tensor
     status: Tensor
+    by: str = "page_slots"
 
     def check(self) -> "PageSlots":
         """Raise RuntimeError where the call was not done (reads the status: a host synchronization)."""
-        word = int(self.status.item())
-        if word:
-            what = ", ".join(t for b, t in _lib.SLOTS_STATUS.items() if word & b)
-            raise RuntimeError(f"page_slots: {what} (nothing was changed)")
+        _check_status(self.by, _lib.SLOTS_STATUS if self.by == "page_slots" else _lib.FORK_STATUS, self.status)
         return self
 
 
@@ -273,10 +281,7 @@ class PageFork:
 
     def check(self) -> "PageFork":
         """Raise RuntimeError where the call was not done (reads the status: a host synchronization)."""
-        word = int(self.status.item())
-        if word:
-            what = ", ".join(t for b, t in _lib.FORK_STATUS.items() if word & b)
-            raise RuntimeError(f"page_fork: {what} (nothing was changed)")
+        _check_status("page_fork", _lib.FORK_STATUS, self.status)
         return self
 
 
@@ -287,6 +292,7 @@ def page_fork(
     ring: Tensor,
     source: Tensor | None = None,
     keep: Tensor | None = None,
+    before: Tensor | None = None,
 ) -> PageFork:
     """Rows that go on from other rows: samples of one prompt, beams, rows cut back or dropped;
     without a host synchronization.
@@ -303,14 +309,16 @@ def page_fork(
 
     All or nothing: where free pages run out, or a source, a count or a page is impossible,
     ``status`` says so, row r comes out as row r went in (empty from row B on), without copies.
+    ``before`` int32 [1]: the status of the call that made the rows, where that was not looked at: if it
+    is not 0, nothing is done either, and ``status`` carries it on.
     The same inputs give the same results again, so a captured graph can be replayed on them."""
     op = "page_fork"
-    _lib.require_gpu(lens, table, free, ring, source, keep, op=op)
+    _lib.require_gpu(lens, table, free, ring, source, keep, before, op=op)
     if table.dim() != 2:
         raise ValueError(f"{op}: table must be [B, pages_per_row], got {tuple(table.shape)}")
     B, ppr = table.shape
     R = B if source is None else source.numel()
-    for name, t, size in (("lens", lens, B), ("table", table, B * ppr), ("free", free, free.numel()), ("ring", ring, 2), ("source", source, R), ("keep", keep, R)):
+    for name, t, size in (("lens", lens, B), ("table", table, B * ppr), ("free", free, free.numel()), ("ring", ring, 2), ("source", source, R), ("keep", keep, R), ("before", before, 1)):
         if t is not None and (t.dtype is not torch.int32 or t.numel() != size or not t.is_contiguous() or (t.dim() != 1 and t is not table)):
             raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of {size} elements, got {t.dtype} {list(t.shape)}")
     sizes = (R * ppr, R, 3 * R, 2, 1)
@@ -321,7 +329,7 @@ def page_fork(
     _lib.written(op, free)
     a = _lib.PageForkArgs(B, R, ppr, free.numel(), lens.data_ptr(), _lib.ptr(source), _lib.ptr(keep), table.data_ptr(), free.data_ptr(), ring.data_ptr(),
                           at, lens_at, lens_at + 4 * R, lens_at + 16 * R, lens_at + 16 * R + 8)
-    _lib.launch_with_workspace("fade_page_fork", a, table.device)
+    _lib.launch_with_workspace("fade_page_fork_after", a, table.device, _lib.ptr(before))
     return PageFork(out.view(R, ppr), lens_out, copies.view(R, 3), ring_out, status)
 
 
@@ -425,30 +433,33 @@ class TokenPagePool:
         self.ring = nxt.ring
         return nxt
 
-    def _rows(self, f: PageFork) -> PageSlots:
+    def _rows(self, f: PageFork, by: str) -> PageSlots:
         self.ring = f.ring
         z = lambda n: torch.zeros(n, dtype=torch.int32, device=self.device)  # noqa: E731
-        return PageSlots(f.table, f.lens, z(f.lens.numel() + 1), z(0), z(0), f.ring, f.status)
+        return PageSlots(f.table, f.lens, z(f.lens.numel() + 1), z(0), z(0), f.ring, f.status, by)
 
     def fork(self, state: PageSlots, source: Tensor, keep: Tensor | None = None, layers: PageLayers | None = None) -> PageSlots:
         """The state of rows that go on from ``state``'s (``page_fork``): row r has the first ``keep[r]``
         tokens (default: all) of row ``source[r]``, or none where that is -1.  Rows share full pages; the
-        page that each goes on writing is copied in every layer where it would be shared."""
+        page that each goes on writing is copied in every layer where it would be shared.  Its status is its
+        own: a step's is to be checked ahead of it, and its own ahead of the next step."""
         from .kernels.paged import paged_copy
 
         f = page_fork(state.lens, state.table, self.free, self.ring, source=source, keep=keep)
         self._shared = True
         paged_copy(f.copies, self.layers if layers is None else layers)
-        return self._rows(f)
+        return self._rows(f, "TokenPagePool.fork")
 
     def accept(self, state: PageSlots, path: Tensor, counts: Tensor, layers: PageLayers | None = None) -> PageSlots:
         """The state after a step of drafted tokens of which each row keeps those numbered
         ``path[b, :counts[b]]`` (``verify_drafts``): their K and V moved together in every layer,
-        the pages behind them returned."""
+        the pages behind them returned.  Where the step itself was not done (``state.status``), nothing
+        is, and the new state's ``check()`` says so."""
         from .kernels.paged import paged_compact
 
         kept = paged_compact(path, counts, state.table, state.lens, state.starts, self.layers if layers is None else layers)
-        return self._rows(page_fork(state.lens, state.table, self.free, self.ring, keep=kept))
+        f = page_fork(state.lens, state.table, self.free, self.ring, keep=kept, before=state.status)
+        return self._rows(f, "TokenPagePool.accept")
 
     def gather(self, table: Tensor, length: int) -> tuple[Tensor, Tensor]:
         """K and V [B, Hkv, length, D] that a block table describes (what stands in a row's

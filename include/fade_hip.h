@@ -664,6 +664,10 @@ typedef struct fade_page_fork_args {
 /* The workspace (16-byte aligned, contents arbitrary) must not be shared by calls that may overlap. */
 int fade_page_fork_workspace_bytes(const fade_page_fork_args* args, int64_t* bytes);
 int fade_page_fork(const fade_page_fork_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same behind another call of which `before` [1] is the status (device memory, read by the launch; fade_page_slots'
+ * of the step that brought the rows' last tokens, or fade_page_fork's): where it is not 0, nothing is done either, and bits 8 to 15 of
+ * the status are its bits (its bits 0 to 7 and 8 to 15 together). */
+int fade_page_fork_after(const fade_page_fork_args* args, const int32_t* before, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Tokens moved within the pages of n_pools tensors [n_pages][Hkv][64][D] of 16-bit
  * elements (K and V of every layer), 16-byte aligned. */

@@ -8,7 +8,9 @@ import random
 import pytest
 import torch
 
-from fade_amd.kernels import verify_drafts
+from fade_amd.kernels import draft_tree, paged_append, verify_drafts
+from fade_amd.pages import TokenPagePool, page_fork
+from fade_amd.rope import Vanilla
 from test_gpu_drafts import _drafted, _probs, _tree
 from test_gpu_paged import _i32, _starts
 
@@ -84,3 +86,72 @@ def test_filled_trees_keep_the_targets_distribution(dev, with_draft):
     # six deviations of a share of B drawings
     assert bool(((share - p.double()).abs() <= 6 * (p * (1 - p) / B).sqrt().double()).all()), share.tolist()
     assert 0.2 < float((got.counts == 2).double().mean()) < 0.99
+
+
+# ------------------------------------------------------------------ steps that could not be done
+def _drafted_step(pool, state, new, V, g, dev):
+    """A step of a chain of drafted tokens in every row, verified and accepted."""
+    T = sum(new)
+    parents = _i32([i - 1 for n in new for i in range(n)], dev)
+    state = pool.step(state, _i32(new, dev), T)
+    tree = draft_tree(parents, state.lens, state.starts, max(new))
+    k = torch.randn(T, pool.n_kv_heads, pool.head_dim, generator=g, device=dev).to(pool.k.dtype)
+    paged_append(k, k, pool.k, pool.v, state.slots, positions=tree.positions, scheme=Vanilla(theta=1e4, head_dim=pool.head_dim))
+    target = torch.softmax(torch.randn(T, V, generator=g, device=dev), -1)
+    got = verify_drafts(target, torch.randint(V, (T,), generator=g, device=dev), parents, state.starts, torch.zeros(T, device=dev), torch.rand(len(new), generator=g, device=dev), max(new))
+    return state, got, pool.accept(state, got.path, got.counts)
+
+
+@pytest.mark.parametrize("pages,ppr,B,new,why", [(3, 4, 2, [70, 70], "pages needed than are free"), (9, 1, 2, [60, 70], "pass its table's pages"),
+                                                 (20000, 300, 60, [330] * 60, "pages needed than are free")])
+def test_accept_carries_a_failed_step_on(dev, pages, ppr, B, new, why):
+    """A step that finds no room for its drafted tokens: what accept returns says so, with rows, pages and the ring as
+    they were; after it is looked at, a smaller step goes on."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    pool = TokenPagePool(pages, 1, 8, F16, dev)
+    if B == 60:  # (a call of several launches, with most pages in other hands)
+        held = torch.tensor([0, 300], dtype=torch.int32, device=dev)
+        pool.ring = held
+    state = pool.step(pool.start(B, ppr), _i32([5] * B, dev), 5 * B).check()
+    k, v = pool.k.normal_(generator=g).clone(), pool.v.normal_(generator=g).clone()
+    was = [t.clone() for t in (state.lens, state.table, pool.ring, pool.free)]
+    failed, got, after = _drafted_step(pool, state, new, 50, g, dev)
+    with pytest.raises(RuntimeError, match=f"^page_slots: .*{why}"):
+        failed.check()
+    with pytest.raises(RuntimeError, match=f"^TokenPagePool.accept: the call before it was not done .*{why}.*nothing was changed"):
+        after.check()
+    assert all(torch.equal(a, b) for a, b in zip((after.lens, after.table, pool.ring, pool.free), was)) and torch.equal(after.ring, was[2])
+    assert torch.equal(pool.k, k) and torch.equal(pool.v, v) and (got.next == -1).all() and not got.counts.any()
+    # and once more, from a state that carries a status on already
+    again = pool.accept(after, got.path, got.counts)
+    with pytest.raises(RuntimeError, match=f"accept: the call before it .*{why}"):
+        again.check()
+    _, got, after = _drafted_step(pool, again, [2] * B, 50, g, dev)
+    after.check()
+    assert after.lens.tolist() == [5 + c for c in got.counts.tolist()] and min(got.counts.tolist()) >= 1
+
+
+def test_fork_behind_an_earlier_call(dev):
+    """page_fork's ``before``: 0 is no matter, anything else leaves all as it is, beside what is wrong with the call itself."""
+    lens, table, ring = _i32([70, 3], dev), _i32([[1, 2], [3, 0]], dev), _i32([0, 1], dev)
+    free = _i32([4, 0, 0, 0], dev)
+    source = _i32([0, 0, -1], dev)
+    for before, want in ((0, 0), (1, 0x100), (8, 0x800), (0x200, 0x200), (0x401, 0x500)):
+        f = free.clone()
+        got = page_fork(lens, table, f, ring, source=source, before=_i32([before], dev))
+        assert int(got.status) == want, before
+        if want:
+            assert got.table.tolist() == [[1, 2], [3, 0], [0, 0]] and got.lens.tolist() == [70, 3, 0] and not got.copies.any() and got.ring.tolist() == [0, 1] and torch.equal(f, free)
+        else:
+            assert got.table.tolist() == [[1, 2], [1, 4], [0, 0]] and got.lens.tolist() == [70, 70, 0]
+    got = page_fork(lens, table, free, ring, source=_i32([7], dev), before=_i32([4], dev))
+    with pytest.raises(RuntimeError, match="page_fork: an impossible source.*the call before it was not done .*n_tokens"):
+        got.check()
+    for bad in (_i32([0, 0], dev), _i32([0], dev).long(), ring):
+        with pytest.raises(ValueError):
+            page_fork(lens, table, free, ring, source=source, before=bad)
+    # named by the call that made the state
+    pool = TokenPagePool(2, 1, 8, F16, dev)
+    state = pool.step(pool.start(1, 2), _i32([70], dev), 70).check()
+    with pytest.raises(RuntimeError, match="^TokenPagePool.fork: more copies needed"):
+        pool.fork(state, _i32([0, 0], dev)).check()
