@@ -433,6 +433,17 @@ class TokenPagePool:
         self.ring = nxt.ring
         return nxt
 
+    def _all_layers(self, op: str, layers: PageLayers | None) -> PageLayers:
+        """The pages to move tokens in: all that the tables may name have to be there (a move outside them is not made)."""
+        if layers is None:
+            return self.layers
+        from .kernels.paged import _layers
+
+        layers = _layers(layers)
+        if layers.n_pages <= self.n_pages or layers.device != self.device:
+            raise ValueError(f"{op}: layers need the pool's pages 0 .. {self.n_pages} on {self.device}, got {layers.n_pages} on {layers.device}")
+        return layers
+
     def _rows(self, f: PageFork, by: str) -> PageSlots:
         self.ring = f.ring
         z = lambda n: torch.zeros(n, dtype=torch.int32, device=self.device)  # noqa: E731
@@ -445,9 +456,10 @@ class TokenPagePool:
         own: a step's is to be checked ahead of it, and its own ahead of the next step."""
         from .kernels.paged import paged_copy
 
+        layers = self._all_layers("TokenPagePool.fork", layers)
         f = page_fork(state.lens, state.table, self.free, self.ring, source=source, keep=keep)
         self._shared = True
-        paged_copy(f.copies, self.layers if layers is None else layers)
+        paged_copy(f.copies, layers)
         return self._rows(f, "TokenPagePool.fork")
 
     def accept(self, state: PageSlots, path: Tensor, counts: Tensor, layers: PageLayers | None = None) -> PageSlots:
@@ -457,7 +469,7 @@ class TokenPagePool:
         is, and the new state's ``check()`` says so."""
         from .kernels.paged import paged_compact
 
-        kept = paged_compact(path, counts, state.table, state.lens, state.starts, self.layers if layers is None else layers)
+        kept = paged_compact(path, counts, state.table, state.lens, state.starts, self._all_layers("TokenPagePool.accept", layers))
         f = page_fork(state.lens, state.table, self.free, self.ring, keep=kept, before=state.status)
         return self._rows(f, "TokenPagePool.accept")
 

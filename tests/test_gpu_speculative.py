@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from fade_amd.kernels import draft_tree, paged_append, verify_drafts
-from fade_amd.pages import TokenPagePool, page_fork
+from fade_amd.pages import PageLayers, TokenPagePool, page_fork
 from fade_amd.rope import Vanilla
 from test_gpu_drafts import _drafted, _probs, _tree
 from test_gpu_paged import _i32, _starts
@@ -155,3 +155,28 @@ def test_fork_behind_an_earlier_call(dev):
     state = pool.step(pool.start(1, 2), _i32([70], dev), 70).check()
     with pytest.raises(RuntimeError, match="^TokenPagePool.fork: more copies needed"):
         pool.fork(state, _i32([0, 0], dev)).check()
+
+
+# ------------------------------------------------------------------ the pool's layers and rows
+def test_layers_that_do_not_fit_the_pool(dev):
+    """Layers with fewer pages than the tables may name are refused ahead of the call (a move outside them is not made,
+    without a word); more pages are no matter."""
+    h = lambda n: torch.zeros(n, 2, 64, 16, dtype=F16, device=dev)  # noqa: E731
+    pool = TokenPagePool(6, 2, 16, F16, dev)
+    state = pool.step(pool.start(1, 3), _i32([100], dev), 100).check()
+    path, counts = _i32([[0]], dev), _i32([1], dev)
+    was = [t.clone() for t in (pool.free, pool.ring)]
+    for n in (6, 3, 1):
+        few = PageLayers([h(n), h(n)])
+        with pytest.raises(ValueError, match="TokenPagePool.fork: layers need the pool's pages"):
+            pool.fork(state, _i32([0, 0], dev), layers=few)
+        with pytest.raises(ValueError, match="TokenPagePool.accept: layers need the pool's pages"):
+            pool.accept(state, path, counts, few)
+        with pytest.raises(ValueError, match="layers need"):
+            pool.fork(state, _i32([0, 0], dev), layers=[h(n)])
+    assert all(torch.equal(a, b) for a, b in zip((pool.free, pool.ring), was))
+    pool.step(state, _i32([0], dev), 0, reset=torch.zeros(1, dtype=torch.bool, device=dev)).check()  # nothing was forked
+    more = [h(9).normal_(), h(9)]
+    state = pool.fork(state, _i32([0, 0], dev), layers=more).check()
+    a, b = state.table[:, 1].tolist()
+    assert a != b and torch.equal(more[0][a, :, :36], more[0][b, :, :36])
