@@ -419,6 +419,13 @@ class TokenPagePool:
             self._own_layers = PageLayers((self.k, self.v))
         return self._own_layers
 
+    def clear(self) -> None:
+        """All pages free, as in a new pool (the tokens in them stay until they are overwritten), e.g. at the
+        end of a batch: no state made so far may be used any more, and ``reset`` is taken again."""
+        torch.arange(1, self.n_pages + 1, dtype=torch.int32, device=self.device, out=self.free)
+        self.ring = torch.tensor([0, self.n_pages], dtype=torch.int32, device=self.device)
+        self._shared = False
+
     def start(self, batch: int, pages_per_row: int) -> PageSlots:
         """The state of ``batch`` empty rows of at most ``pages_per_row`` pages."""
         z = lambda *s: torch.zeros(s, dtype=torch.int32, device=self.device)  # noqa: E731
@@ -426,9 +433,10 @@ class TokenPagePool:
 
     def step(self, state: PageSlots, new: Tensor, n_tokens: int, reset: Tensor | None = None) -> PageSlots:
         """``page_slots`` for the next ``new[b]`` tokens of every row; the pool keeps the ring.  After a
-        ``fork`` rows may share pages, and finished ones are dropped by ``fork`` too, not by ``reset``."""
+        ``fork`` rows may share pages, and finished ones are dropped by ``fork`` too, not by ``reset``,
+        until the pool is ``clear``ed."""
         if reset is not None and self._shared:
-            raise ValueError("TokenPagePool.step: rows may share pages after fork; drop finished rows with fork (source -1) instead of reset")
+            raise ValueError("TokenPagePool.step: rows may share pages after fork; drop finished rows with fork (source -1) instead of reset, or clear the pool")
         nxt = page_slots(state.lens, new, state.table, self.free, self.ring, n_tokens, reset=reset)
         self.ring = nxt.ring
         return nxt

@@ -180,3 +180,19 @@ def test_layers_that_do_not_fit_the_pool(dev):
     state = pool.fork(state, _i32([0, 0], dev), layers=more).check()
     a, b = state.table[:, 1].tolist()
     assert a != b and torch.equal(more[0][a, :, :36], more[0][b, :, :36])
+
+
+def test_clear(dev):
+    """A pool that was forked takes ``reset`` again once it is cleared, with all of its pages and in the same memory."""
+    pool = TokenPagePool(7, 1, 8, F16, dev)
+    none = torch.zeros(2, dtype=torch.bool, device=dev)
+    state = pool.step(pool.start(2, 3), _i32([130, 3], dev), 133).check()
+    state = pool.fork(state, _i32([1, 0], dev)).check()
+    with pytest.raises(ValueError, match="clear the pool"):
+        pool.step(state, _i32([1, 1], dev), 2, reset=none)
+    at = pool.free.data_ptr()
+    pool.clear()
+    assert pool.free.data_ptr() == at and pool.free.tolist() == [1, 2, 3, 4, 5, 6, 7] and pool.ring.tolist() == [0, 7]
+    state = pool.step(pool.start(2, 3), _i32([192, 65], dev), 257).check()
+    state = pool.step(state, _i32([1, 1], dev), 2, reset=torch.tensor([True, False], device=dev)).check()
+    assert state.lens.tolist() == [1, 66] and state.ring.tolist()[1] == 4
