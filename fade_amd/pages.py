@@ -303,7 +303,10 @@ def page_fork(
     goes on writing, its last one where that is not full, is its own: of the rows that end in one
     page the first keeps it, unless a row holds it as a full one, and the others get a free page,
     listed in ``copies``.  Pages without a row are returned to the ring, in the order of their
-    numbers.  ``free`` int32 [n] and ``ring`` [2] as in ``page_slots``; pages are numbered
+    numbers, for the calls after this one: the copies take pages that were free before it (where those
+    are too few, rows are dropped by one call and branch in the next).  Holders are counted among
+    these rows alone: none of their pages may be held by rows elsewhere, such as a copy of ``lens`` and
+    ``table`` that is to be forked again.  ``free`` int32 [n] and ``ring`` [2] as in ``page_slots``; pages are numbered
     1 .. n.  ``page_slots``' ``reset`` returns pages without a look at other rows: rows that may
     share pages are dropped here, as ``source[r] = -1``.
 
@@ -391,7 +394,12 @@ class TokenPagePool:
     Rows branch and shrink: ``fork`` makes a batch whose rows go on from rows of another
     (samples of one prompt, beams; -1 drops a row), ``accept`` keeps the verified path of each
     row's drafted tokens.  Both take ``layers``, the ``PageLayers`` of all layers' pages, where
-    there are more than the pool's own ``k`` and ``v``."""
+    there are more than the pool's own ``k`` and ``v``.
+
+    A state that was given to ``step``, ``fork`` or ``accept`` is used up, once that call was done: its
+    pages are the new state's, or returned, and the holders of a page are counted among the rows of one
+    state alone.  Used once more it would return pages that the new state's rows hold, or go on
+    writing one of them.  A prompt that is to be sampled again later stays a row of the batch."""
 
     def __init__(self, n_pages: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16, device="cuda") -> None:
         if n_pages < 1 or n_kv_heads < 1 or head_dim < 8 or head_dim % 8 or head_dim > 256:

@@ -644,7 +644,8 @@ int fade_verify_drafts(const fade_verify_args* args, void* workspace, int64_t wo
  * that is not full) is its own: of the rows that end in one page the first keeps it, if no
  * row holds it as a full one, and each other gets a free page and copies[r] = {page, its
  * page, tokens} (zeros elsewhere) for fade_paged_copy.  Pages that the B rows held and none
- * of the R rows does are returned to the ring, in the order of their numbers.  Pages are
+ * of the R rows does are returned to the ring, in the order of their numbers; the copies take
+ * pages that were free before.  No page is held by rows that are not among the B.  Pages are
  * 1 .. n_free.  The ring as in fade_page_slots (whose reset must not be used on rows that
  * share pages); what is written must be other memory than the rest of the call's. */
 typedef struct fade_page_fork_args {
