@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(Pools pools, CopyParams 
 
 struct CompactParams {
   int64_t max_path, ppr, n_pages;
-  int B, Hkv, units, slices;  // slices of a token's units over workgroups
+  int Hkv, units, slices;  // slices of a token's units over workgroups
   const int32_t* path;
   const int32_t* counts;
   const int32_t* table;
@@ -120,22 +120,27 @@ int check_args(const fade_paged_move_args* a, const char* what) {
   if (a->n_pools < 1 || a->n_pools > 65535 || a->n_pages < 1 || a->n_pages >= (1ll << 31) || a->Hkv < 1 || a->Hkv > 65535)
     return einval("%s: n_pools and Hkv must be 1 to 65535, n_pages 1 to 2^31 - 1", what);
   if (a->D < 8 || a->D > 256 || a->D % 8) return einval("%s: head_dim must be a multiple of 8 in [8, 256], got %lld", what, (long long)a->D);
-  if (a->rows < 0 || a->rows > (1 << 20) || a->rows * a->Hkv >= (1ll << 31)) return einval("%s: too many rows", what);
+  if (a->rows < 0 || a->rows > (1 << 20)) return einval("%s: too many rows", what);
   if (!a->pools) return einval("%s: null pools", what);
   for (int64_t i = 0; i < a->n_pools; ++i)
     if (!a->pools[i] || (reinterpret_cast<uintptr_t>(a->pools[i]) & 15)) return einval("%s: pools must be 16-byte aligned", what);
   return FADE_OK;
 }
 
+// launch(tensors, how many, number of the first, rows r0 .., how many of them), `per_row` workgroups a row; a launch
+// has fewer than 2^32 threads along x.
 template <class F>
-int each_pools(const fade_paged_move_args* a, const char* what, F&& launch) {
+int each_launch(const fade_paged_move_args* a, int64_t per_row, const char* what, F&& launch) {
+  const int64_t most = ((1ll << 32) / kThreads - 1) / per_row;
   for (int64_t i0 = 0; i0 < a->n_pools; i0 += kPools) {
     Pools pools;
     const int64_t n = a->n_pools - i0 < kPools ? a->n_pools - i0 : kPools;
     for (int64_t i = 0; i < n; ++i) pools.at[i] = static_cast<u32x4*>(a->pools[i0 + i]);
-    launch(pools, static_cast<unsigned>(n), i0);
-    const int rc = check_launch(what);
-    if (rc) return rc;
+    for (int64_t r0 = 0; r0 < a->rows; r0 += most) {
+      launch(pools, static_cast<unsigned>(n), i0, r0, a->rows - r0 < most ? a->rows - r0 : most);
+      const int rc = check_launch(what);
+      if (rc) return rc;
+    }
   }
   return FADE_OK;
 }
@@ -153,9 +158,9 @@ FADE_API int fade_paged_copy(const fade_paged_move_args* a, void* stream) {
   if (rc) return rc;
   if (a->rows == 0) return FADE_OK;
   if (!a->copies) return einval("%s: null copies", what);
-  const CopyParams p{a->copies, a->n_pages, static_cast<int>(a->Hkv), static_cast<int>(a->D / 8)};
-  return each_pools(a, what, [&](const Pools& pools, unsigned n, int64_t) {
-    hipLaunchKernelGGL(copy_kernel, dim3(static_cast<unsigned>(a->rows * a->Hkv), n), dim3(kThreads), 0, as_stream(stream), pools, p);
+  return each_launch(a, a->Hkv, what, [&](const Pools& pools, unsigned n, int64_t, int64_t r0, int64_t rows) {
+    const CopyParams p{a->copies + 3 * r0, a->n_pages, static_cast<int>(a->Hkv), static_cast<int>(a->D / 8)};
+    hipLaunchKernelGGL(copy_kernel, dim3(static_cast<unsigned>(rows * a->Hkv), n), dim3(kThreads), 0, as_stream(stream), pools, p);
   });
 }
 
@@ -167,22 +172,21 @@ FADE_API int fade_paged_compact(const fade_paged_move_args* a, void* stream) {
     return einval("%s: max_path must be 1 to %d, pages_per_row 1 to 2^24", what, FADE_DRAFT_MAX_NODES);
   if (a->rows < 1 || !a->path || !a->counts || !a->table || !a->lens || !a->starts || !a->kept)
     return einval("%s: needs rows, path, counts, table, lens, starts and kept", what);
-  CompactParams p;
-  p.max_path = a->max_path;
-  p.ppr = a->pages_per_row;
-  p.n_pages = a->n_pages;
-  p.B = static_cast<int>(a->rows);
-  p.Hkv = static_cast<int>(a->Hkv);
-  p.units = static_cast<int>(a->D / 8);
-  p.slices = static_cast<int>(cdiv(a->Hkv * p.units, kThreads));
-  p.path = a->path;
-  p.counts = a->counts;
-  p.table = a->table;
-  p.lens = a->lens;
-  p.starts = a->starts;
-  if (a->rows * p.slices >= (1ll << 31)) return einval("%s: too many rows", what);
-  return each_pools(a, what, [&](const Pools& pools, unsigned n, int64_t i0) {
-    p.kept = i0 == 0 ? a->kept : nullptr;
-    hipLaunchKernelGGL(compact_kernel, dim3(static_cast<unsigned>(a->rows * p.slices), n), dim3(kThreads), 0, as_stream(stream), pools, p);
+  const int64_t slices = cdiv(a->Hkv * (a->D / 8), kThreads);
+  return each_launch(a, slices, what, [&](const Pools& pools, unsigned n, int64_t i0, int64_t r0, int64_t rows) {
+    CompactParams p;
+    p.max_path = a->max_path;
+    p.ppr = a->pages_per_row;
+    p.n_pages = a->n_pages;
+    p.Hkv = static_cast<int>(a->Hkv);
+    p.units = static_cast<int>(a->D / 8);
+    p.slices = static_cast<int>(slices);
+    p.path = a->path + r0 * a->max_path;
+    p.counts = a->counts + r0;
+    p.table = a->table + r0 * a->pages_per_row;
+    p.lens = a->lens + r0;
+    p.starts = a->starts + r0;
+    p.kept = i0 == 0 ? a->kept + r0 : nullptr;
+    hipLaunchKernelGGL(compact_kernel, dim3(static_cast<unsigned>(rows * slices), n), dim3(kThreads), 0, as_stream(stream), pools, p);
   });
 }

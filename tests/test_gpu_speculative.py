@@ -8,7 +8,7 @@ import random
 import pytest
 import torch
 
-from fade_amd.kernels import draft_tree, paged_append, verify_drafts
+from fade_amd.kernels import draft_tree, paged_append, paged_compact, paged_copy, verify_drafts
 from fade_amd.pages import PageLayers, TokenPagePool, page_fork
 from fade_amd.rope import Vanilla
 from test_gpu_drafts import _drafted, _probs, _tree
@@ -196,3 +196,32 @@ def test_clear(dev):
     state = pool.step(pool.start(2, 3), _i32([192, 65], dev), 257).check()
     state = pool.step(state, _i32([1, 1], dev), 2, reset=torch.tensor([True, False], device=dev)).check()
     assert state.lens.tolist() == [1, 66] and state.ring.tolist()[1] == 4
+
+
+# ------------------------------------------------------------------ moves of very many rows
+def test_moves_of_more_workgroups_than_a_launch_has(dev):
+    """Past 2^32 threads, in tensors of 16 kv heads: the copies and paths of all rows are made, the first and the last too."""
+    R, Hkv, D = 2**20, 16, 8
+    x = torch.randn(40, Hkv, 64, D, device=dev).half()
+    layers = PageLayers([x])
+    want = x.clone()
+    copies = torch.zeros(R, 3, dtype=torch.int32, device=dev)
+    rows = [0, 1, R // 2, R - 20, R - 17, R - 16, R - 2, R - 1]
+    for i, r in enumerate(rows):
+        copies[r] = _i32([1 + i, 20 + i, 5 + i], dev)
+        want[20 + i, :, : 5 + i] = want[1 + i, :, : 5 + i]
+    paged_copy(copies, layers)
+    assert torch.equal(x, want)
+    # 512 heads of 256 channels: 64 workgroups a row, 2^18 rows fill a launch
+    Hkv, D, B = 512, 256, 2**18 + 5
+    x = torch.randn(8, Hkv, 64, D, device=dev).half()
+    layers, want = PageLayers([x]), x.clone()
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
+    path, counts, table, lens, starts = z(B, 2), z(B), z(B, 1), z(B), z(B + 1)
+    for i, r in enumerate((0, 9, 2**18 - 2, 2**18 - 1, 2**18, B - 1)):
+        path[r] = _i32([1, 3], dev)
+        counts[r], table[r], lens[r] = 2, 1 + i, 10
+        starts[r + 1 :] += 4  # tokens 6 .. 9 are drafted, those at 7 and 9 stay
+        want[1 + i, :, 6], want[1 + i, :, 7] = want[1 + i, :, 7].clone(), want[1 + i, :, 9].clone()
+    kept = paged_compact(path, counts, table, lens, starts, layers)
+    assert torch.equal(x, want) and torch.equal(kept, torch.where(lens > 0, 8, 0).int())
