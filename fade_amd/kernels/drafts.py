@@ -133,7 +133,7 @@ def verify_drafts(
         raise ValueError(f"{op}: tokens must be int64 or int32, got {tokens.dtype}")
     for name, t, size, dtype in (("tokens", tokens, T, tokens.dtype), ("parents", parents, T, i32), ("starts", starts, B + 1, i32),
                                  ("uniforms", uniforms, T, torch.float32), ("final", final, B, torch.float32)):
-        if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+        if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != size or not t.is_contiguous() or t.is_neg():
             raise ValueError(f"{op}: {name} must be a contiguous {dtype} [{size}], got {t.dtype} {list(t.shape)}")
     if not 1 <= M <= _lib.DRAFT_MAX_NODES:
         raise ValueError(f"{op}: max_path must be 1 to {_lib.DRAFT_MAX_NODES}, got {max_path}")

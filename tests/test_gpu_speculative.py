@@ -225,3 +225,16 @@ def test_moves_of_more_workgroups_than_a_launch_has(dev):
         want[1 + i, :, 6], want[1 + i, :, 7] = want[1 + i, :, 7].clone(), want[1 + i, :, 9].clone()
     kept = paged_compact(path, counts, table, lens, starts, layers)
     assert torch.equal(x, want) and torch.equal(kept, torch.where(lens > 0, 8, 0).int())
+
+
+def test_numbers_that_are_held_negated_are_refused(dev):
+    """One row's number as the imaginary part of a conjugate: memory of the other sign, which looks contiguous."""
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
+    odd = torch.complex(torch.zeros(1, device=dev), torch.full((1,), -0.5, device=dev)).conj().imag
+    assert odd.is_neg() and odd.is_contiguous() and odd.item() == 0.5
+    target = torch.full((1, 4), 0.25, device=dev)
+    starts = _i32([0, 1], dev)
+    assert verify_drafts(target, z(1), z(1), starts, torch.zeros(1, device=dev), odd.clone().resolve_neg(), 1).next.tolist() == [2]
+    for name in ("uniforms", "final"):
+        with pytest.raises(ValueError, match=name):
+            verify_drafts(target, z(1), z(1), starts, **{**dict(uniforms=torch.zeros(1, device=dev), final=torch.zeros(1, device=dev)), name: odd}, max_path=1)
