@@ -667,10 +667,11 @@ __global__ __launch_bounds__(64) void paged_few_kernel(Params p) {
 //
 // Draft trees (TREE) differ in the mask alone: steps over the row's new tokens take a
 // word of the query's bits for 32 keys, shifted to the step's place, asked for ahead of the
-// wait for the step.  16 rows of 16 tokens over 8192 keys (64 matrix rows of 256): 109 us, HBM; 61 rows of
-// 48 over up to 32000 keys at seven heads a kv head: 250 (162 at a copy's rate, 126 at a matrix
-// product's): matrix and vector instructions each a third of the cycles, 1.9 GHz; with zeros
-// for K and V, which cost no power, a sixth less, keys from L2 another sixth less.  Measured
+// wait for the step.  16 rows of 16 tokens over 8192 keys (64 matrix rows of 256): 113 us, HBM; 61 rows of
+// 24 to 48 over up to 32000 keys at seven heads a kv head, the long ones with the small trees: 257 (162 at a copy's
+// rate, 126 at a matrix product's), of it the join 16: matrix and vector instructions each a third of the
+// cycles, and power; with zeros for K and V, which cost no power, a sixth less, keys from L2 another sixth less.  Rows of
+// more than 256 matrix rows are read once per tile: the long ones with the large trees 397.  Measured
 // without gain: a last tile of few rows counted half or three quarters in the cut, 4 buffers.
 template <int DP>
 __device__ __forceinline__ int wide_k_unit(int row, int u) {
