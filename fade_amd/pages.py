@@ -322,7 +322,7 @@ def page_fork(
     B, ppr = table.shape
     R = B if source is None else source.numel()
     for name, t, size in (("lens", lens, B), ("table", table, B * ppr), ("free", free, free.numel()), ("ring", ring, 2), ("source", source, R), ("keep", keep, R), ("before", before, 1)):
-        if t is not None and (t.dtype is not torch.int32 or t.numel() != size or not t.is_contiguous() or (t.dim() != 1 and t is not table)):
+        if t is not None and (t.dtype is not torch.int32 or t.numel() != size or not t.is_contiguous() or (t.dim() != 1 and t is not table and t is not before)):
             raise ValueError(f"{op}: {name} must be a contiguous int32 tensor of {size} elements, got {t.dtype} {list(t.shape)}")
     sizes = (R * ppr, R, 3 * R, 2, 1)
     buf = table.new_empty(sum(sizes))  # (one allocation)
@@ -431,7 +431,8 @@ class TokenPagePool:
         """All pages free, as in a new pool (the tokens in them stay until they are overwritten), e.g. at the
         end of a batch: no state made so far may be used any more, and ``reset`` is taken again."""
         torch.arange(1, self.n_pages + 1, dtype=torch.int32, device=self.device, out=self.free)
-        self.ring = torch.tensor([0, self.n_pages], dtype=torch.int32, device=self.device)
+        self.ring = torch.zeros(2, dtype=torch.int32, device=self.device)
+        self.ring[1:].fill_(self.n_pages)
         self._shared = False
 
     def start(self, batch: int, pages_per_row: int) -> PageSlots:

@@ -144,7 +144,7 @@ def test_fork_behind_an_earlier_call(dev):
             assert got.table.tolist() == [[1, 2], [3, 0], [0, 0]] and got.lens.tolist() == [70, 3, 0] and not got.copies.any() and got.ring.tolist() == [0, 1] and torch.equal(f, free)
         else:
             assert got.table.tolist() == [[1, 2], [1, 4], [0, 0]] and got.lens.tolist() == [70, 70, 0]
-    got = page_fork(lens, table, free, ring, source=_i32([7], dev), before=_i32([4], dev))
+    got = page_fork(lens, table, free, ring, source=_i32([7], dev), before=_i32(4, dev))  # (of any shape, as page_slots' out takes it)
     with pytest.raises(RuntimeError, match="page_fork: an impossible source.*the call before it was not done .*n_tokens"):
         got.check()
     for bad in (_i32([0, 0], dev), _i32([0], dev).long(), ring):
