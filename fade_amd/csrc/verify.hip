@@ -274,7 +274,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(fade_verify_args a, Sh
   for (int i = threadIdx.x; i < n; i += kThreads) {
     // A token outside the vocabulary was drawn from nothing: it follows none, and so is never tried.  (Refused instead,
     // it would take draft's share from what is left, and the next token would not be the target's.)
-    const int x = token_of(a, row, i), up = x < 0 ? -1 : parent_of(a, row, i);
+    const int parent = parent_of(a, row, i), x = token_of(a, row, i), up = x < 0 ? -1 : parent;
     const float2 pq = SHARED ? sh.probs[row.s + i] : probs_of<E>(a, row, up, x);
     nodes.up[i] = static_cast<int16_t>(up);
     nodes.tok[i] = x;
