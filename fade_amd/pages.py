@@ -258,6 +258,7 @@ def page_slots(
                 raise ValueError(f"{op}: out.{name} must be contiguous int32 of {size} elements on {table.device}")
         _lib.written(op, *res)
         ptrs = [t.data_ptr() for t in res]
+        out.by = op
     _lib.written(op, free)
     a = _lib.PageSlotsArgs(B, ppr, n, n_free, lens.data_ptr(), new.data_ptr(), _lib.ptr(reset), table.data_ptr(), free.data_ptr(),
                            ring.data_ptr(), *ptrs)

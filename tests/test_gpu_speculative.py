@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from fade_amd.kernels import draft_tree, paged_append, paged_compact, paged_copy, verify_drafts
-from fade_amd.pages import PageLayers, TokenPagePool, page_fork
+from fade_amd.pages import PageLayers, TokenPagePool, page_fork, page_slots
 from fade_amd.rope import Vanilla
 from test_gpu_drafts import _drafted, _probs, _tree
 from test_gpu_paged import _i32, _starts
@@ -155,6 +155,9 @@ def test_fork_behind_an_earlier_call(dev):
     state = pool.step(pool.start(1, 2), _i32([70], dev), 70).check()
     with pytest.raises(RuntimeError, match="^TokenPagePool.fork: more copies needed"):
         pool.fork(state, _i32([0, 0], dev)).check()
+    out = pool.fork(state, _i32([0], dev)).check()
+    with pytest.raises(RuntimeError, match="^page_slots: a row would pass its table's pages"):
+        page_slots(state.lens, _i32([900], dev), state.table, pool.free, pool.ring.clone(), 0, out=out).check()
 
 
 # ------------------------------------------------------------------ the pool's layers and rows
